@@ -46,6 +46,8 @@ LIBRARIES: dict[str, tuple[str, list[str], list[str]]] = {
     "attention_expanded": ("nvcc", ["kernels/attention_expanded.cu"], []),
     "decay_chunks": ("nvcc", ["kernels/decay_chunks.cu"], []),
     "state_chunks": ("nvcc", ["kernels/state_chunks.cu"], []),
+    "attention_tree": ("nvcc", ["kernels/attention_tree.cu"], []),
+    "candidates": ("nvcc", ["kernels/drafts.cu", "kernels/beams.cu"], []),
 }
 
 _loaded: dict[str, ctypes.CDLL] = {}

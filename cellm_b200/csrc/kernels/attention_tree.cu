@@ -1,0 +1,341 @@
+// Attention of drafted trees over the paged cache: every node of a request's tree sees the request's committed keys (all of
+// them, or those of its window) and, among the nodes, its ancestors and itself,
+//     o_i = sum_j w_ij v_j,   w_i = softmax over the keys j that i sees of  scale q_i . k_j,
+// node i standing at position ctx + depth(i). The committed keys and values lie in pages, the nodes' own in rows beside the
+// cache (only what is accepted later moves into pages), so the keys are walked in blocks of two kinds: committed ones by
+// position, then the nodes by their place in the tree, each with a mask of one bit a key.
+//
+// Sums, maxima and the output's accumulators are 32-bit; a row is rounded once, when it is written (the tensor-core kernel
+// rounds the weights too). Where the keys are cut into pieces (few rows, long contexts), a piece leaves its maximum, sum and
+// unnormalised output in a workspace, and a second kernel merges them in their order.
+#include <algorithm>
+
+#include "draft_tree.cuh"
+
+namespace {
+
+// What all kernels of this file are given.
+struct TreeArgs {
+    void* out;                    // [T, nh * hd]
+    float* part_o;                // [nsplit, T * nh, hd], where the keys are cut
+    float* part_ml;               // [nsplit, T * nh, 2]
+    const void *q, *k_new, *v_new;   // rows of node t at q + t * q_ld, k_new + t * k_ld, ...
+    long long q_ld, k_ld, v_ld;   // in elements
+    const int* parents;           // [T]
+    const void *k_pool, *v_pool;  // [pages][nkv][page_size][hd]
+    const int *cu_seqlens, *ctx_lens, *block_table;
+    int bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, tiles, nsplit, window;
+    float scale_log2e;
+    int* err;
+};
+
+// A block's share of the work: request, key/value head, piece of the keys, tile of rows.
+struct TreeTile {
+    int b, kvh, split, tile, t_base, n, ctx;
+    bool live;
+};
+__device__ __forceinline__ TreeTile tree_tile(const TreeArgs& a) {
+    TreeTile t;
+    int i = blockIdx.x;
+    t.tile = i % a.tiles, i /= a.tiles;
+    t.split = i % a.nsplit, i /= a.nsplit;
+    t.kvh = i % a.nkv;
+    t.b = i / a.nkv;
+    t.t_base = a.cu_seqlens[t.b];
+    t.n = a.cu_seqlens[t.b + 1] - t.t_base;
+    t.ctx = a.ctx_lens[t.b];
+    t.live = t.n > 0 && t.t_base >= 0 && t.t_base + t.n <= a.T;
+    if (t.n > a.most || t.n < 0 || t.t_base < 0 || t.t_base + t.n > a.T) {
+        if (threadIdx.x == 0) atomicOr(a.err, CELLM_DEV_BAD_TREE);
+        t.live = false;
+    }
+    // keys beyond what a row of the block table can name are reported and left out
+    if (t.ctx < 0 || t.ctx > (long long)a.bt_stride * a.page_size) {
+        if (threadIdx.x == 0) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+        t.ctx = t.ctx < 0 ? 0 : (int)((long long)a.bt_stride * a.page_size);
+    }
+    return t;
+}
+
+// Which of a block's KT keys a node sees, a bit a key: committed ones from position key0 on, or (node0 >= 0) the nodes from node0 on.
+template <int KT>
+__device__ __forceinline__ uint64_t seen_bits(const TreeShape& tree, int node, int window, int ctx, int key0, int node0) {
+    static_assert(KT == 32 || KT == 64, "");
+    if (node0 >= 0) {
+        uint64_t m = tree.line[node][node0 >> 5];
+        if (KT == 64 && (node0 >> 5) + 1 < TREE_WORDS) m |= (uint64_t)tree.line[node][(node0 >> 5) + 1] << 32;
+        return m;
+    }
+    const int lo = window > 0 ? max(0, ctx + tree.depth[node] - window + 1) : 0;
+    const int below = min(max(lo - key0, 0), KT), upto = min(max(ctx - key0, 0), KT);
+    const uint64_t in = upto >= 64 ? ~0ull : (1ull << upto) - 1ull, out = below >= 64 ? ~0ull : (1ull << below) - 1ull;
+    return in & ~out;
+}
+
+// ---------------------------------------------------------------- any type, any head size up to 256
+// 128 threads take 32 rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit arithmetic: a
+// thread forms 4 x KT/16 scores out of shared memory, a row's maximum and sum go over half a warp, and the thread then owns 4 x
+// HDP/16 entries of the output.
+template <int HDP> struct PlainTile { static constexpr int KEYS = HDP <= 128 ? 64 : 32; };
+
+template <typename T>
+__device__ __forceinline__ void row_to_floats(float* dst, const T* src, int hd, int padded, int lane, int lanes, bool quads) {
+    if (quads) {
+        for (int d = lane * 4; d < padded; d += lanes * 4) {
+            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (src != nullptr && d < hd) {
+                if constexpr (sizeof(T) == 4) {
+                    f = *reinterpret_cast<const float4*>(src + d);
+                } else {
+                    const uint2 w = *reinterpret_cast<const uint2*>(src + d);
+                    f = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+                }
+            }
+            *reinterpret_cast<float4*>(dst + d) = f;
+        }
+    } else {
+        for (int d = lane; d < padded; d += lanes) dst[d] = src != nullptr && d < hd ? to_float(src[d]) : 0.f;
+    }
+}
+
+template <typename T, int HDP>
+__global__ void __launch_bounds__(128)
+attention_tree_plain_kernel(const TreeArgs a, int quads) {
+    constexpr int RT = 32, KT = PlainTile<HDP>::KEYS, LD = HDP + 4, KC = KT / 16;
+    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC);
+    extern __shared__ __align__(16) uint8_t raw[];
+    TreeShape& tree = *reinterpret_cast<TreeShape*>(raw);
+    float* qs = reinterpret_cast<float*>(raw + sizeof(TreeShape));     // [RT][LD]
+    float* ks = qs + RT * LD;                                          // [KT][LD]
+    float* vs = ks + KT * LD;                                          // [KT][LD]
+    float* ps = vs + KT * LD;                                          // [KT][RT + 4]
+    pdl_wait();
+    pdl_trigger();
+    const TreeTile t = tree_tile(a);
+    const int G = a.nh / a.nkv, rows = t.n * G;
+    if (!t.live || t.tile * RT >= rows) return;
+    read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
+
+    const int hd = a.hd, rg = threadIdx.x >> 4, c = threadIdx.x & 15;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = warp; r < RT; r += 4) {
+        const int row = t.tile * RT + r;
+        const T* src = row < rows ? static_cast<const T*>(a.q) + (long long)(t.t_base + row / G) * a.q_ld + (long long)(t.kvh * G + row % G) * hd : nullptr;
+        row_to_floats(qs + r * LD, src, hd, HDP, lane, 32, quads);
+    }
+    // a thread's rows are rg, rg + 8, rg + 16, rg + 24 of the tile
+    int node[4];
+    float m[4], l[4], o[4][NV * VEC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = t.tile * RT + rg + i * 8;
+        node[i] = row < rows && tree.depth[row / G] >= 0 ? row / G : -1;
+        m[i] = -INFINITY, l[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < NV * VEC; ++d) o[i][d] = 0.f;
+    }
+    const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
+    const int first = lo / KT, committed = lo < t.ctx ? (t.ctx + KT - 1) / KT - first : 0, blocks = committed + (t.n + KT - 1) / KT;
+    const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), end = min(blocks, begin + per);
+    const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
+    for (int blk = begin; blk < end; ++blk) {
+        const bool paged = blk < committed;
+        const int key0 = (first + blk) * KT, node0 = paged ? -1 : (blk - committed) * KT;
+        __syncthreads();
+        for (int r = warp; r < KT; r += 4) {
+            const T *k = nullptr, *v = nullptr;
+            if (paged) {
+                const int j = key0 + r;
+                if (j >= lo && j < t.ctx) {
+                    const int page = bt[j / a.page_size];
+                    if (page < 0 || page >= a.num_pages) {
+                        if (lane == 0) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                    } else {
+                        const size_t off = (((size_t)page * a.nkv + t.kvh) * a.page_size + j % a.page_size) * hd;
+                        k = static_cast<const T*>(a.k_pool) + off, v = static_cast<const T*>(a.v_pool) + off;
+                    }
+                }
+            } else if (node0 + r < t.n && tree.depth[node0 + r] >= 0) {
+                k = static_cast<const T*>(a.k_new) + (long long)(t.t_base + node0 + r) * a.k_ld + (long long)t.kvh * hd;
+                v = static_cast<const T*>(a.v_new) + (long long)(t.t_base + node0 + r) * a.v_ld + (long long)t.kvh * hd;
+            }
+            row_to_floats(ks + r * LD, k, hd, HDP, lane, 32, quads);
+            row_to_floats(vs + r * LD, v, hd, HDP, lane, 32, quads);
+        }
+        __syncthreads();
+        float s[4][KC];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int k = 0; k < KC; ++k) s[i][k] = 0.f;
+#pragma unroll 2
+        for (int d = 0; d < HDP; d += 4) {
+            float4 q4[4], k4[KC];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (rg + i * 8) * LD + d);
+#pragma unroll
+            for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const float4*>(ks + (c + k * 16) * LD + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < KC; ++k)
+                    s[i][k] = fmaf(q4[i].w, k4[k].w, fmaf(q4[i].z, k4[k].z, fmaf(q4[i].y, k4[k].y, fmaf(q4[i].x, k4[k].x, s[i][k]))));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint64_t seen = node[i] >= 0 ? seen_bits<KT>(tree, node[i], a.window, t.ctx, key0, node0) : 0ull;
+            float top = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                s[i][k] = (seen >> (c + k * 16) & 1ull) ? s[i][k] * a.scale_log2e : -INFINITY;
+                top = fmaxf(top, s[i][k]);
+            }
+#pragma unroll
+            for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float now = fmaxf(m[i], top), use = now == -INFINITY ? 0.f : now, corr = exp2f(m[i] - use);
+            m[i] = now;
+            float sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < KC; ++k) {
+                const float p = exp2f(s[i][k] - use);
+                sum += p;
+                ps[(c + k * 16) * (RT + 4) + rg * 4 + i] = p;
+            }
+            l[i] = l[i] * corr + sum;
+#pragma unroll
+            for (int d = 0; d < NV * VEC; ++d) o[i][d] *= corr;
+        }
+        __syncwarp();                          // a half-warp writes and reads the columns of its own rows alone
+#pragma unroll 4
+        for (int k = 0; k < KT; ++k) {
+            const float4 p = *reinterpret_cast<const float4*>(ps + k * (RT + 4) + rg * 4);
+#pragma unroll
+            for (int g = 0; g < NV; ++g) {
+                float v[VEC];
+                const float* src = vs + k * LD + (g * 16 + c) * VEC;
+                if constexpr (VEC == 4) {
+                    const float4 w = *reinterpret_cast<const float4*>(src);
+                    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
+                } else {
+                    const float2 w = *reinterpret_cast<const float2*>(src);
+                    v[0] = w.x, v[1] = w.y;
+                }
+#pragma unroll
+                for (int x = 0; x < VEC; ++x) {
+                    o[0][g * VEC + x] = fmaf(p.x, v[x], o[0][g * VEC + x]);
+                    o[1][g * VEC + x] = fmaf(p.y, v[x], o[1][g * VEC + x]);
+                    o[2][g * VEC + x] = fmaf(p.z, v[x], o[2][g * VEC + x]);
+                    o[3][g * VEC + x] = fmaf(p.w, v[x], o[3][g * VEC + x]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+        const int row = t.tile * RT + rg + i * 8;
+        if (row >= rows) continue;
+        const long long gr = (long long)(t.t_base + row / G) * a.nh + t.kvh * G + row % G;
+        if (a.nsplit > 1) {
+            float* dst = a.part_o + ((long long)t.split * a.T * a.nh + gr) * hd;
+#pragma unroll
+            for (int g = 0; g < NV; ++g)
+#pragma unroll
+                for (int x = 0; x < VEC; ++x)
+                    if ((g * 16 + c) * VEC + x < hd) dst[(g * 16 + c) * VEC + x] = o[i][g * VEC + x];
+            if (c == 0) {
+                float* ml = a.part_ml + ((long long)t.split * a.T * a.nh + gr) * 2;
+                ml[0] = m[i], ml[1] = l[i];
+            }
+        } else {
+            const float inv = l[i] > 0.f ? 1.f / l[i] : l[i];          // 0 where nothing is seen; NaN stays
+            T* dst = static_cast<T*>(a.out) + gr * hd;
+#pragma unroll
+            for (int g = 0; g < NV; ++g)
+#pragma unroll
+                for (int x = 0; x < VEC; ++x)
+                    if ((g * 16 + c) * VEC + x < hd) dst[(g * 16 + c) * VEC + x] = from_float<T>(o[i][g * VEC + x] * inv);
+        }
+    }
+}
+
+// The pieces of a row merged in their order: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A warp takes a row.
+template <typename T>
+__global__ void __launch_bounds__(256)
+attention_tree_merge_kernel(T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, long long rows, int hd, int nsplit) {
+    pdl_wait();
+    pdl_trigger();
+    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (r >= rows) return;
+    float M = -INFINITY;
+    for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, part_ml[(s * rows + r) * 2]);
+    M = warp_max(M);
+    const float use = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    for (int s = 0; s < nsplit; ++s) L = fmaf(exp2f(part_ml[(s * rows + r) * 2] - use), part_ml[(s * rows + r) * 2 + 1], L);
+    const float inv = L > 0.f ? 1.f / L : L;
+    for (int d = lane; d < hd; d += 32) {
+        float acc = 0.f;
+        for (int s = 0; s < nsplit; ++s) {
+            const float w = exp2f(part_ml[(s * rows + r) * 2] - use);
+            if (w != 0.f) acc = fmaf(w, part_o[(s * rows + r) * hd + d], acc);       // (a piece that sees nothing holds zeros)
+        }
+        out[r * hd + d] = from_float<T>(acc * inv);
+    }
+}
+
+template <typename T, int HDP>
+int launch_plain(const TreeArgs& a, cudaStream_t stream) {
+    constexpr int KT = PlainTile<HDP>::KEYS, LD = HDP + 4;
+    const size_t smem = sizeof(TreeShape) + (size_t)((32 + 2 * KT) * LD + KT * 36) * 4;
+    cudaError_t e = cudaFuncSetAttribute(attention_tree_plain_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool;
+    const int quads = a.hd % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && at % (4 * sizeof(T)) == 0;
+    CELLM_RUN((attention_tree_plain_kernel<T, HDP>), (unsigned)((long long)a.B * a.nkv * a.nsplit * a.tiles), 128, smem, stream, a, quads);
+    return CELLM_OK;
+}
+
+template <typename T>
+int launch_plain_sized(const TreeArgs& a, cudaStream_t stream) {
+    if (a.hd <= 32) return launch_plain<T, 32>(a, stream);
+    if (a.hd <= 64) return launch_plain<T, 64>(a, stream);
+    if (a.hd <= 96) return launch_plain<T, 96>(a, stream);
+    if (a.hd <= 128) return launch_plain<T, 128>(a, stream);
+    return launch_plain<T, 256>(a, stream);
+}
+
+template <typename T>
+int launch_merge(const TreeArgs& a, cudaStream_t stream) {
+    const long long rows = (long long)a.T * a.nh;
+    CELLM_RUN(attention_tree_merge_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, stream, (T*)a.out, a.part_o, a.part_ml, rows, a.hd, a.nsplit);
+    return CELLM_OK;
+}
+
+}  // namespace
+
+// out [T, nh * hd], q rows q_ld elements apart, the nodes' keys and values in rows k_ld and v_ld apart ([nkv * hd] each), parents
+// [T]; request b owns the nodes cu_seqlens[b] .. cu_seqlens[b + 1] (at most 256, `most` of them in the largest tree) behind
+// ctx_lens[b] committed tokens in the pages of its row of the block table. nsplit pieces of the keys need part_o [nsplit, T * nh,
+// hd] and part_ml [nsplit, T * nh, 2] floats.
+CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, const void* q, long long q_ld, const void* k_new, long long k_ld,
+                                   const void* v_new, long long v_ld, const int* parents, const void* k_pool, const void* v_pool,
+                                   const int* cu_seqlens, const int* ctx_lens, const int* block_table, int bt_stride, int B, int T, int most,
+                                   int num_pages, int page_size, int nh, int nkv, int hd, float scale, int window, int nsplit, int dtype, int* err,
+                                   cudaStream_t stream) {
+    if (T <= 0 || B <= 0 || most <= 0) return CELLM_OK;
+    if (dtype != CELLM_F32 && dtype != CELLM_BF16) return CELLM_ERR_DTYPE;
+    if (nkv <= 0 || nh <= 0 || nh % nkv || hd <= 0 || hd > 256 || page_size <= 0 || most > TREE_MAX || bt_stride < 0 || window < 0) return CELLM_ERR_SIZE;
+    if (nsplit < 1 || nsplit > 128) return CELLM_ERR_SIZE;
+    if (nsplit > 1 && (!part_o || !part_ml)) return CELLM_ERR_ARG;
+    if (!out || !q || !k_new || !v_new || !parents || !cu_seqlens || !ctx_lens || !err) return CELLM_ERR_ARG;
+    TreeArgs a = {out, part_o, part_ml, q, k_new, v_new, q_ld, k_ld, v_ld, parents, k_pool, v_pool, cu_seqlens, ctx_lens, block_table,
+                  bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, 0, nsplit, window, scale * 1.4426950408889634f, err};
+    a.tiles = (most * (nh / nkv) + 31) / 32;
+    if ((long long)B * nkv * nsplit * a.tiles > 0x7fffffffLL) return CELLM_ERR_SIZE;
+    int rc = dtype == CELLM_F32 ? launch_plain_sized<float>(a, stream) : launch_plain_sized<__nv_bfloat16>(a, stream);
+    if (rc != CELLM_OK || nsplit == 1) return rc;
+    return dtype == CELLM_F32 ? launch_merge<float>(a, stream) : launch_merge<__nv_bfloat16>(a, stream);
+}

@@ -28,7 +28,8 @@ enum {
     CELLM_DEV_BAD_PAGE = 2,    // page id outside the pool
     CELLM_DEV_BAD_SLOT = 4,    // state slot outside the pool
     CELLM_DEV_WAIT_TIMEOUT = 8,// a bounded wait inside a kernel gave up
-    CELLM_DEV_BAD_LAYOUT = 16  // shared memory not aligned as the kernel's tiles need
+    CELLM_DEV_BAD_LAYOUT = 16, // shared memory not aligned as the kernel's tiles need
+    CELLM_DEV_BAD_TREE = 32    // a drafted tree with too many nodes, or a parent that does not stand before its child
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }

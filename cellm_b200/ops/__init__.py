@@ -11,6 +11,8 @@ from .recurrent import (embed_pairs, norm_pair, scaled_add2, pair_norm_mean, con
                         gated_group_norm, head_norm_silu)
 from .stream import add_scaled_norm, stream_add_rows, token_gate_mul, scaled_rms_add, weighted_sum2, xielu, head_gate_mul, post_norm
 from .attention import attention
+from .drafts import accept_drafts, attention_tree
+from .beams import beam_select, reorder_pages, reorder_states
 from .gemm_bf16 import gemm_swiglu_bf16, tensor_core_ok
 
 __all__ = ["embed", "add_rmsnorm", "residual_add", "swiglu", "short_conv", "qk_norm_rope",
@@ -21,4 +23,5 @@ __all__ = ["embed", "add_rmsnorm", "residual_add", "swiglu", "short_conv", "qk_n
            "weighted_sum2", "xielu", "head_gate_mul", "post_norm", "embed_norm", "turned_attn_prep", "attention_plain_chunked", "attention_flash_chunked",
            "attention_tc_chunked", "rotate_heads", "decay_scan", "ssd_prep", "gated_group_norm", "head_norm_silu",
            "stream_cast", "gated_norm_add", "mingru_scan", "head_product", "gated_act", "attention_latent",
-           "norm_add_norm", "soft_cap_", "latent_rows", "attention_expanded"]
+           "norm_add_norm", "soft_cap_", "latent_rows", "attention_expanded",
+           "attention_tree", "accept_drafts", "beam_select", "reorder_states", "reorder_pages"]

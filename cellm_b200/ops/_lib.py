@@ -117,6 +117,16 @@ _SIGNATURES = {
         "cellm_decay_chunks": [P, P, L, I, P, L, P, L, P, L, P, L, P, L, P, P, I, I, I, I, I, I, I, P, P, P, P],
         "cellm_decay_chunks_supports": [I, I],
     },
+    "attention_tree": {
+        "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, P, P],
+    },
+    "candidates": {
+        "cellm_accept_drafts": [P, P, P, P, P, P, P, I, I, I, P, L, L, I, P, P, L, L, I, P, P, P, I, I, I, I, I, P, P],
+        "cellm_beam_parts": [I],
+        "cellm_beam_select": [P, P, P, P, P, P, L, I, I, I, I, P, P, I, I, P],
+        "cellm_reorder_states": [P, P, P, I, I, I, I, L, P, P],
+        "cellm_reorder_pages": [P, P, I, P, P, P, I, I, I, I, I, I, I, P, P],
+    },
     "attention_expanded": {
         "cellm_latent_rows": [P, P, P, P, P, I, I, I, I, I, I, I, P, P],
         "cellm_attention_expanded": [P, P, L, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, P, P, P, P],
@@ -197,6 +207,29 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.device.index or 0)
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def launch(library: str, name: str, t: torch.Tensor, *args, kernels: int = 1) -> None:
+    """Calls the entry point `name` with `args` and the current stream of `t`'s device, on that device, and counts its kernels."""
+    f = fn(library, "cellm_" + name)
+    if t.device.index == _current_device():
+        code = f(*args, stream_of(t))
+    else:
+        with torch.cuda.device(t.device):
+            code = f(*args, stream_of(t))
+    check(code, name)
+    if kernels > 1:
+        LAUNCHES[0] += kernels - 1
+
+
+def require_ints(name: str, device, **tensors) -> None:
+    """int32 index arrays, dense, on `device`."""
+    for what, t in tensors.items():
+        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
+            raise ValueError(f"{name}: {what} must be dense int32 on {device} (got {t.dtype}, {t.device}, contiguous={t.is_contiguous()})")
 
 
 def require_cuda(*tensors) -> None:
