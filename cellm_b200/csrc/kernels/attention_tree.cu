@@ -9,8 +9,10 @@
 // rounds the weights too). Where the keys are cut into pieces (few rows, long contexts), a piece leaves its maximum, sum and
 // unnormalised output in a workspace, and a second kernel merges them in their order.
 #include <algorithm>
+#include <climits>
 
 #include "draft_tree.cuh"
+#include "mma_tiles.cuh"
 
 namespace {
 
@@ -103,9 +105,9 @@ __global__ void __launch_bounds__(128)
 attention_tree_plain_kernel(const TreeArgs a, int quads) {
     constexpr int RT = 32, KT = PlainTile<HDP>::KEYS, LD = HDP + 4, KC = KT / 16;
     constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC);
-    extern __shared__ __align__(16) uint8_t raw[];
-    TreeShape& tree = *reinterpret_cast<TreeShape*>(raw);
-    float* qs = reinterpret_cast<float*>(raw + sizeof(TreeShape));     // [RT][LD]
+    extern __shared__ __align__(16) uint8_t plain_smem[];
+    TreeShape& tree = *reinterpret_cast<TreeShape*>(plain_smem);
+    float* qs = reinterpret_cast<float*>(plain_smem + sizeof(TreeShape));     // [RT][LD]
     float* ks = qs + RT * LD;                                          // [KT][LD]
     float* vs = ks + KT * LD;                                          // [KT][LD]
     float* ps = vs + KT * LD;                                          // [KT][RT + 4]
@@ -260,6 +262,243 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     }
 }
 
+// ---------------------------------------------------------------- bfloat16, head sizes 32, 64, 96, 128: mma.sync
+// Four warps take 16 * RG rows through blocks of 64 keys that all threads bring in with cp.async (a ring of ST stages, one barrier
+// a block). RG groups of 16 rows share a block; the 4 / RG warps of a group take its keys in equal parts, each with a softmax
+// state of its own, and meet in shared memory at the end. Few rows (small trees) so still use every warp.
+template <int HD, int RG>
+struct MmaTile {
+    static constexpr int KG = 4 / RG, RT = 16 * RG;
+    static constexpr int ST = HD <= 32 ? 4 : HD <= 96 ? 3 : 2;
+    static constexpr int KV = FA_BN * HD * 2;
+    static constexpr int q_off = 0, kv_off = RT * HD * 2, tree_off = kv_off + ST * 2 * KV, bytes = tree_off + (int)sizeof(TreeShape);
+    static_assert(4 * 16 * (HD + 2) * 4 <= ST * 2 * KV, "the warps' outputs must fit the ring");
+};
+
+template <int HD, int RG>
+__global__ void __launch_bounds__(128)
+attention_tree_mma_kernel(const TreeArgs a) {
+    using L = MmaTile<HD, RG>;
+    constexpr int BN = FA_BN, CH = HD / 8, NT = HD / 8, ST = L::ST, KG = L::KG, WK = BN / KG, ITERS = BN * CH / 128;
+    extern __shared__ __align__(128) uint8_t mma_smem[];
+    uint8_t *q_s = mma_smem + L::q_off, *kv_s = mma_smem + L::kv_off;
+    TreeShape& tree = *reinterpret_cast<TreeShape*>(mma_smem + L::tree_off);
+    pdl_wait();
+    pdl_trigger();
+    const TreeTile t = tree_tile(a);
+    const int G = a.nh / a.nkv, rows = t.n * G, row0 = t.tile * L::RT;
+    if (!t.live || row0 >= rows) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rg = warp % RG, kg = warp / RG;
+
+    const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
+    const int first = lo / BN, committed = lo < t.ctx ? (t.ctx + BN - 1) / BN - first : 0, blocks = committed + (t.n + BN - 1) / BN;
+    const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), n_blk = min(blocks, begin + per) - begin;
+    const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
+    const int shift = (a.page_size & (a.page_size - 1)) == 0 ? __ffs(a.page_size) - 1 : -1;
+    const size_t page_elems = (size_t)a.nkv * a.page_size * HD;
+    // this thread's rows of a block lie 128 / CH apart; the table's entries of the block after the next are under way while
+    // a block is computed
+    const int row_t = threadIdx.x / CH, chunk_t = threadIdx.x % CH;
+    constexpr bool EVEN = 128 % CH == 0;
+    auto row_of = [&](int it) { return EVEN ? row_t + it * (128 / CH) : (threadIdx.x + it * 128) / CH; };
+    auto chunk_of = [&](int it) { return EVEN ? chunk_t : (threadIdx.x + it * 128) % CH; };
+    int entry[ITERS];
+    auto look_up = [&](int i) {
+#pragma unroll
+        for (int it = 0; it < ITERS; ++it) {
+            const int blk = begin + i, j = (first + blk) * BN + row_of(it);
+            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
+        }
+    };
+    auto load_kv = [&](int i) {
+        if (i < n_blk) {
+            uint8_t* ks = kv_s + (size_t)(i % ST) * 2 * L::KV;
+            const int blk = begin + i;
+#pragma unroll
+            for (int it = 0; it < ITERS; ++it) {
+                const int row = row_of(it), chunk = chunk_of(it);
+                const __nv_bfloat16 *k = static_cast<const __nv_bfloat16*>(a.k_pool), *v = static_cast<const __nv_bfloat16*>(a.v_pool);
+                bool have = false;
+                if (blk < committed) {
+                    const int j = (first + blk) * BN + row, page = entry[it];
+                    if (page >= 0 && page < a.num_pages) {
+                        const size_t off = (size_t)page * page_elems + ((size_t)t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * HD + chunk * 8;
+                        k += off, v += off, have = true;
+                    } else if (page != -2) {
+                        atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                    }
+                } else {
+                    const int node = (blk - committed) * BN + row;
+                    if (node < t.n && tree.depth[node] >= 0) {
+                        k = static_cast<const __nv_bfloat16*>(a.k_new) + (t.t_base + node) * a.k_ld + t.kvh * HD + chunk * 8;
+                        v = static_cast<const __nv_bfloat16*>(a.v_new) + (t.t_base + node) * a.v_ld + t.kvh * HD + chunk * 8;
+                        have = true;
+                    }
+                }
+                cp_async16(ks + tile_offset<HD>(row, chunk), k, have ? 16 : 0);
+                cp_async16(ks + L::KV + tile_offset<HD>(row, chunk), v, have ? 16 : 0);
+            }
+        }
+        cp_async_commit();
+    };
+    // Committed blocks leave before the tree's shape is known; the nodes' own wait for it.
+    look_up(0);
+    for (int i = threadIdx.x; i < L::RT * CH; i += 128) {
+        const int r = i / CH, chunk = i % CH, row = min(row0 + r, rows - 1);
+        cp_async16(q_s + tile_offset<HD>(r, chunk), static_cast<const __nv_bfloat16*>(a.q) + (t.t_base + row / G) * a.q_ld + (t.kvh * G + row % G) * HD + chunk * 8, 16);
+    }
+    const int old = max(0, min(min(n_blk, ST - 1), committed - begin));
+    for (int i = 0; i < old; ++i) {
+        load_kv(i);
+        look_up(i + 1);
+    }
+    read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
+    for (int i = old; i < ST - 1; ++i) {
+        load_kv(i);
+        look_up(i + 1);
+    }
+    const int ra = row0 + rg * 16 + (lane >> 2), rb = ra + 8;
+    const int node_a = ra < rows && tree.depth[ra / G] >= 0 ? ra / G : -1, node_b = rb < rows && tree.depth[rb / G] >= 0 ? rb / G : -1;
+    const int open_from = a.window > 0 ? t.ctx + t.n - a.window : 0;        // no row's window starts behind it
+    float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.f, l_b = 0.f;
+    float o[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    uint32_t qf[HD / 16][4];
+
+    for (int i = 0; i < n_blk; ++i) {
+        cp_async_wait<ST - 2>();
+        __syncthreads();
+        if (i == 0) {
+#pragma unroll
+            for (int ks = 0; ks < HD / 16; ++ks) ldmatrix_x4(qf[ks], q_s + tile_offset<HD>(rg * 16 + (lane & 15), ks * 2 + (lane >> 4)));
+        }
+        load_kv(i + ST - 1);               // into the stage that everybody left before the barrier
+        look_up(i + ST);
+        const uint8_t *k_s = kv_s + (size_t)(i % ST) * 2 * L::KV, *v_s = k_s + L::KV;
+        const int k0 = kg * WK;
+        float s[WK / 8][4];
+#pragma unroll
+        for (int n = 0; n < WK / 8; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks) {
+#pragma unroll
+            for (int n2 = 0; n2 < WK / 16; ++n2) {
+                uint32_t kf[4];
+                ldmatrix_x4(kf, k_s + tile_offset<HD>(k0 + n2 * 16 + (lane & 7) + ((lane >> 4) << 3), ks * 2 + ((lane >> 3) & 1)));
+                mma_bf16(s[2 * n2], qf[ks], kf[0], kf[1]);
+                mma_bf16(s[2 * n2 + 1], qf[ks], kf[2], kf[3]);
+            }
+        }
+        const int blk = begin + i, key0 = (first + blk) * BN;
+        const bool paged = blk < committed;
+        if (!paged || key0 + BN > t.ctx || key0 < open_from) {
+            const int node0 = paged ? -1 : (blk - committed) * BN;
+            const uint64_t see_a = node_a >= 0 ? seen_bits<BN>(tree, node_a, a.window, t.ctx, key0, node0) >> (k0 + (lane & 3) * 2) : 0ull;
+            const uint64_t see_b = node_b >= 0 ? seen_bits<BN>(tree, node_b, a.window, t.ctx, key0, node0) >> (k0 + (lane & 3) * 2) : 0ull;
+#pragma unroll
+            for (int n = 0; n < WK / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    s[n][e] = (see_a >> (n * 8 + e) & 1ull) ? s[n][e] * a.scale_log2e : -INFINITY;
+                    s[n][2 + e] = (see_b >> (n * 8 + e) & 1ull) ? s[n][2 + e] * a.scale_log2e : -INFINITY;
+                }
+        } else {
+#pragma unroll
+            for (int n = 0; n < WK / 8; ++n) s[n][0] *= a.scale_log2e, s[n][1] *= a.scale_log2e, s[n][2] *= a.scale_log2e, s[n][3] *= a.scale_log2e;
+        }
+        float mx_a = -INFINITY, mx_b = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < WK / 8; ++n) mx_a = fmaxf(mx_a, fmaxf(s[n][0], s[n][1])), mx_b = fmaxf(mx_b, fmaxf(s[n][2], s[n][3]));
+        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1));
+        mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
+        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1));
+        mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
+        const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
+        const float use_a = mn_a == -INFINITY ? 0.f : mn_a, use_b = mn_b == -INFINITY ? 0.f : mn_b;
+        const float corr_a = fast_exp2(m_a - use_a), corr_b = fast_exp2(m_b - use_b);
+        m_a = mn_a, m_b = mn_b;
+        float sum_a = 0.f, sum_b = 0.f;
+        uint32_t pf[WK / 16][4];
+#pragma unroll
+        for (int n = 0; n < WK / 8; ++n) {
+            const float p0 = fast_exp2(s[n][0] - use_a), p1 = fast_exp2(s[n][1] - use_a);
+            const float p2 = fast_exp2(s[n][2] - use_b), p3 = fast_exp2(s[n][3] - use_b);
+            sum_a += p0 + p1, sum_b += p2 + p3;
+            pf[n >> 1][(n & 1) * 2] = pack_bf16(p0, p1);               // the weights' rounding: what the tensor cores' operand holds
+            pf[n >> 1][(n & 1) * 2 + 1] = pack_bf16(p2, p3);
+        }
+        l_a = l_a * corr_a + sum_a, l_b = l_b * corr_b + sum_b;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) o[n][0] *= corr_a, o[n][1] *= corr_a, o[n][2] *= corr_b, o[n][3] *= corr_b;
+#pragma unroll
+        for (int kk = 0; kk < WK / 16; ++kk) {
+#pragma unroll
+            for (int n2 = 0; n2 < NT / 2; ++n2) {
+                uint32_t vf[4];
+                ldmatrix_x4_trans(vf, v_s + tile_offset<HD>(k0 + kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3), n2 * 2 + (lane >> 4)));
+                mma_bf16(o[2 * n2], pf[kk], vf[0], vf[1]);
+                mma_bf16(o[2 * n2 + 1], pf[kk], vf[2], vf[3]);
+            }
+        }
+    }
+    cp_async_wait<0>();
+    l_a += __shfl_xor_sync(0xffffffffu, l_a, 1);
+    l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
+    l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
+    l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
+
+    // the warps' results meet in shared memory, where the ring was; 16 lanes of a warp then write a row together
+    __syncthreads();
+    float* o_s = reinterpret_cast<float*>(kv_s);                                       // [4][16][HD]
+    float* ml_s = o_s + 4 * 16 * HD;                                                   // [4][16][2]
+    {
+        const int r = lane >> 2, col = (lane & 3) * 2;
+        float* ow = o_s + warp * 16 * HD;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            *reinterpret_cast<float2*>(ow + r * HD + n * 8 + col) = make_float2(o[n][0], o[n][1]);
+            *reinterpret_cast<float2*>(ow + (r + 8) * HD + n * 8 + col) = make_float2(o[n][2], o[n][3]);
+        }
+        if ((lane & 3) == 0) {
+            ml_s[(warp * 16 + r) * 2] = m_a, ml_s[(warp * 16 + r) * 2 + 1] = l_a;
+            ml_s[(warp * 16 + r + 8) * 2] = m_b, ml_s[(warp * 16 + r + 8) * 2 + 1] = l_b;
+        }
+    }
+    __syncthreads();
+    for (int r = threadIdx.x >> 4; r < L::RT; r += 8) {
+        const int row = row0 + r, c = threadIdx.x & 15;
+        if (row >= rows) break;
+        const bool seen = tree.depth[row / G] >= 0;
+        float M = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) M = fmaxf(M, ml_s[((g * RG + r / 16) * 16 + r % 16) * 2]);
+        const float use = M == -INFINITY ? 0.f : M;
+        float f[KG], l = 0.f;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            const float* ml = ml_s + ((g * RG + r / 16) * 16 + r % 16) * 2;
+            f[g] = exp2f(ml[0] - use);
+            l += f[g] * ml[1];
+        }
+        const long long gr = (long long)(t.t_base + row / G) * a.nh + t.kvh * G + row % G;
+        const float inv = !seen || l == 0.f ? 0.f : 1.f / l;
+        if (a.nsplit > 1 && c == 0)
+            *reinterpret_cast<float2*>(a.part_ml + ((long long)t.split * a.T * a.nh + gr) * 2) = seen ? make_float2(M, l) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int d = c * 2; d < HD; d += 32) {
+            float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < KG; ++g) {
+                const float2 v = *reinterpret_cast<const float2*>(o_s + ((g * RG + r / 16) * 16 + r % 16) * HD + d);
+                acc.x = fmaf(f[g], v.x, acc.x), acc.y = fmaf(f[g], v.y, acc.y);
+            }
+            if (a.nsplit > 1) *reinterpret_cast<float2*>(a.part_o + ((long long)t.split * a.T * a.nh + gr) * HD + d) = seen ? acc : make_float2(0.f, 0.f);
+            else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + gr * HD + d) = seen ? pack_bf16(acc.x * inv, acc.y * inv) : 0u;
+        }
+    }
+}
+
 // The pieces of a row merged in their order: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A warp takes a row.
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -307,6 +546,46 @@ int launch_plain_sized(const TreeArgs& a, cudaStream_t stream) {
     return launch_plain<T, 256>(a, stream);
 }
 
+template <int HD, int RG>
+int launch_mma(TreeArgs a, cudaStream_t stream) {
+    using L = MmaTile<HD, RG>;
+    cudaError_t e = cudaFuncSetAttribute(attention_tree_mma_kernel<HD, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes);
+    if (e != cudaSuccess) return (int)e;
+    a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
+    CELLM_RUN((attention_tree_mma_kernel<HD, RG>), (unsigned)((long long)a.B * a.nkv * a.nsplit * a.tiles), 128, L::bytes, stream, a);
+    return CELLM_OK;
+}
+template <int HD>
+int launch_mma_rows(const TreeArgs& a, cudaStream_t stream) {
+    const int rows = a.most * (a.nh / a.nkv);
+    return rows <= 16 ? launch_mma<HD, 1>(a, stream) : rows <= 32 ? launch_mma<HD, 2>(a, stream) : launch_mma<HD, 4>(a, stream);
+}
+// Whether the tensor-core kernel takes a call: its copies are 16 bytes wide.
+bool mma_takes(const TreeArgs& a) {
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
+    return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0;
+}
+int launch_bf16(const TreeArgs& a, cudaStream_t stream) {
+    if (!mma_takes(a)) return launch_plain_sized<__nv_bfloat16>(a, stream);
+    if (a.hd == 32) return launch_mma_rows<32>(a, stream);
+    if (a.hd == 64) return launch_mma_rows<64>(a, stream);
+    if (a.hd == 96) return launch_mma_rows<96>(a, stream);
+    return launch_mma_rows<128>(a, stream);
+}
+
+// How many pieces the keys of a tile of rows are cut into: of all counts the one whose rounds of blocks, each as long as its keys
+// and a few blocks' worth of start and merge, take the least time.
+int pieces(long long tiles, int key_blocks, long long at_once) {
+    constexpr int START = 3;
+    int best = 1;
+    long long least = LLONG_MAX;
+    for (int n = 1; n <= 64 && n <= std::max(1, key_blocks); ++n) {
+        const long long cost = (tiles * n + at_once - 1) / at_once * ((key_blocks + n - 1) / n + START) + (n > 1 ? START : 0);
+        if (cost < least) least = cost, best = n;
+    }
+    return best;
+}
+
 template <typename T>
 int launch_merge(const TreeArgs& a, cudaStream_t stream) {
     const long long rows = (long long)a.T * a.nh;
@@ -315,6 +594,16 @@ int launch_merge(const TreeArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+// The pieces the keys are best cut into: B trees of up to `most` nodes, `keys` the most that a node sees.
+CELLM_API int cellm_attention_tree_pieces(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
+    if (B <= 0 || most <= 0 || nkv <= 0 || nh < nkv) return 1;
+    const int rows = most * (nh / nkv);
+    const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
+    const int tile = !mma || (rows > 16 && rows <= 32) ? 32 : rows <= 16 ? 16 : 64;
+    const int an_sm = !mma ? 2 : hd == 32 ? 4 : hd == 64 ? 3 : 2;             // blocks that an SM holds, by their shared memory
+    return pieces((long long)B * nkv * ((rows + tile - 1) / tile), (keys + 63) / 64, (long long)an_sm * sms);
+}
 
 // out [T, nh * hd], q rows q_ld elements apart, the nodes' keys and values in rows k_ld and v_ld apart ([nkv * hd] each), parents
 // [T]; request b owns the nodes cu_seqlens[b] .. cu_seqlens[b + 1] (at most 256, `most` of them in the largest tree) behind
@@ -335,7 +624,7 @@ CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, con
                   bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, 0, nsplit, window, scale * 1.4426950408889634f, err};
     a.tiles = (most * (nh / nkv) + 31) / 32;
     if ((long long)B * nkv * nsplit * a.tiles > 0x7fffffffLL) return CELLM_ERR_SIZE;
-    int rc = dtype == CELLM_F32 ? launch_plain_sized<float>(a, stream) : launch_plain_sized<__nv_bfloat16>(a, stream);
+    int rc = dtype == CELLM_F32 ? launch_plain_sized<float>(a, stream) : launch_bf16(a, stream);
     if (rc != CELLM_OK || nsplit == 1) return rc;
     return dtype == CELLM_F32 ? launch_merge<float>(a, stream) : launch_merge<__nv_bfloat16>(a, stream);
 }

@@ -118,6 +118,7 @@ _SIGNATURES = {
         "cellm_decay_chunks_supports": [I, I],
     },
     "attention_tree": {
+        "cellm_attention_tree_pieces": [I, I, I, I, I, I, I, I],
         "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, P, P],
     },
     "candidates": {

@@ -11,11 +11,10 @@ from typing import Optional, Sequence
 
 import torch
 
-from ._lib import DTYPE_TAG, launch, ptr, require_ints
+from ._lib import DTYPE_TAG, fn, launch, ptr, require_ints
 from ._state import sm_count
 
 MAX_TREE = 256                     # nodes of a tree (TREE_MAX in draft_tree.cuh)
-_TILE = 32                         # rows of a block of the kernel for any type
 
 
 def _rows(name: str, what: str, t: torch.Tensor, T: int, width: int, like: torch.Tensor) -> int:
@@ -25,12 +24,6 @@ def _rows(name: str, what: str, t: torch.Tensor, T: int, width: int, like: torch
         raise ValueError(f"{name}: {what} must be [{T}, {width}] rows of {like.dtype} on {like.device} with dense rows "
                          f"(got {tuple(t.shape)}, strides {t.stride()}, {t.dtype}, {t.device})")
     return t.stride(0) if T > 1 else width
-
-
-def _pieces(device, blocks_whole: int, key_blocks: int) -> int:
-    """Into how many pieces the keys are cut: blocks that fill the SMs twice, of at least two blocks of keys each."""
-    want = -(-2 * sm_count(device) // max(blocks_whole, 1))
-    return max(1, min(want, key_blocks // 2, 64))
 
 
 def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, parents: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -69,8 +62,7 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     entries = block_table.shape[1]
     keys = min(max_ctx or entries * page_size, entries * page_size)
     keys = min(keys, window) if window else keys
-    tiles = -(-most * (nh // nkv) // _TILE)
-    nsplit = _pieces(device, B * nkv * tiles, -(-(keys + most) // 64))
+    nsplit = fn("attention_tree", "cellm_attention_tree_pieces")(B, most, nh, nkv, hd, keys + most, DTYPE_TAG[q.dtype], sm_count(device))
     part_o = part_ml = None
     if nsplit > 1:
         ws = torch.empty(nsplit * T * nh * (hd + 2), dtype=torch.float32, device=device)
