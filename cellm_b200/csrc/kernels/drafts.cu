@@ -118,3 +118,11 @@ CELLM_API int cellm_accept_drafts(int* out_count, int* out_path, int* out_next, 
 #undef GO
     return CELLM_OK;
 }
+
+// The same with its arguments in order as 64-bit words (see common.cuh).
+CELLM_API int cellm_accept_drafts_packed(const long long* a, cudaStream_t stream) {
+    return cellm_accept_drafts((int*)a[0], (int*)a[1], (int*)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (const int*)a[6], (int)a[7],
+        (int)a[8], (int)a[9], (const void*)a[10], (long long)a[11], (long long)a[12], (int)a[13], (void*)a[14], (const void*)a[15], (long long)a[16],
+        (long long)a[17], (int)a[18], (void*)a[19], (const int*)a[20], (const int*)a[21], (int)a[22], (int)a[23], (int)a[24], (int)a[25], (int)a[26],
+        (int*)a[27], stream);
+}

@@ -213,24 +213,31 @@ def stream_of(t: torch.Tensor) -> int:
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 
-def launch(library: str, name: str, t: torch.Tensor, *args, kernels: int = 1) -> None:
-    """Calls the entry point `name` with `args` and the current stream of `t`'s device, on that device, and counts its kernels."""
-    f = fn(library, "cellm_" + name)
-    if t.device.index == _current_device():
-        code = f(*args, stream_of(t))
+def launch_packed(library: str, name: str, device_index: int, packed: bytes, kernels: int = 1) -> None:
+    """Calls the entry point `name`_packed with its arguments as 64-bit words and the current stream of the device, on that device, and
+    counts its kernels."""
+    f = _funcs.get(name)
+    if f is None:
+        f = getattr(_build.load(library), f"cellm_{name}_packed")
+        f.argtypes, f.restype = [ctypes.c_char_p, P], c_int
+        _funcs[name] = f
+    stream = _raw_stream(device_index) if _raw_stream is not None else torch.cuda.current_stream(device_index).cuda_stream
+    if device_index == _current_device():
+        code = f(packed, stream)
     else:
-        with torch.cuda.device(t.device):
-            code = f(*args, stream_of(t))
-    check(code, name)
-    if kernels > 1:
-        LAUNCHES[0] += kernels - 1
+        with torch.cuda.device(device_index):
+            code = f(packed, stream)
+    if code != 0:
+        check(code, name)
+    LAUNCHES[0] += kernels
 
 
-def require_ints(name: str, device, **tensors) -> None:
-    """int32 index arrays, dense, on `device`."""
-    for what, t in tensors.items():
-        if t.dtype != torch.int32 or t.device != device or not t.is_contiguous():
-            raise ValueError(f"{name}: {what} must be dense int32 on {device} (got {t.dtype}, {t.device}, contiguous={t.is_contiguous()})")
+def dense_ints(index: int, *tensors) -> bool:
+    """Whether all are dense int32 on device `index`."""
+    for t in tensors:
+        if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+            return False
+    return True
 
 
 def require_cuda(*tensors) -> None:

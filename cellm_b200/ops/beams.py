@@ -1,13 +1,15 @@
 """Beam search: the best continuations of a request's beams, and the beams' cached state in their new order."""
 from __future__ import annotations
 
+from struct import Struct
 from typing import Optional
 
 import torch
 
-from ._lib import DTYPE_TAG, fn, launch, ptr, require_ints
+from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
 
 MAX_BEAMS, MAX_KEEP = 32, 64       # (as in beams.cu)
+_SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("15q").pack, Struct("9q").pack, Struct("14q").pack
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Optional[torch.Tensor] = None, pad: int = 0):
@@ -18,34 +20,29 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Opt
     Scores are compared in 64 bits; the sums behind them carry about 2^-25.
 
     Returns (scores float32, parents int32, tokens int32), each [R, keep]; where a request has fewer continuations, -inf and -1."""
-    name = "beam_select"
-    if not logits.is_cuda or logits.dim() != 2 or logits.dtype not in DTYPE_TAG or (logits.shape[1] > 1 and logits.stride(1) != 1):
-        raise ValueError(f"{name}: float32 or bfloat16 logits [requests * beams, V] on the GPU, rows dense")
-    device, (rows, V) = logits.device, logits.shape
-    if scores.dtype != torch.float32 or scores.device != device or scores.dim() != 2 or not scores.is_contiguous() or scores.numel() != rows:
-        raise ValueError(f"{name}: dense float32 scores [requests, beams] for {rows} rows of logits on {device} (got {tuple(scores.shape)} {scores.dtype})")
-    R, K = scores.shape
+    index, shape, stride, pair = logits.get_device(), logits.shape, logits.stride(), scores.shape
+    if index < 0 or len(shape) != 2 or logits.dtype not in DTYPE_TAG or (stride[1] != 1 and shape[1] > 1):
+        raise ValueError("beam_select: float32 or bfloat16 logits [requests * beams, V] on the GPU, rows dense")
+    rows, V = shape
+    if len(pair) != 2 or pair[0] * pair[1] != rows or scores.dtype is not torch.float32 or scores.get_device() != index or not scores.is_contiguous():
+        raise ValueError(f"beam_select: dense float32 scores [requests, beams] for {rows} rows of logits on {logits.device} (got {tuple(pair)} {scores.dtype})")
+    R, K = pair
     if not 0 < K <= MAX_BEAMS or not 0 < keep <= MAX_KEEP or V < 1 or not 0 <= pad < V:
-        raise ValueError(f"{name}: up to {MAX_BEAMS} beams, up to {MAX_KEEP} kept and a padding token of the vocabulary (got {K}, {keep}, {pad} of {V})")
-    if done is not None and (done.dtype != torch.bool or done.device != device or done.shape != scores.shape or not done.is_contiguous()):
-        raise ValueError(f"{name}: done must be dense bool {tuple(scores.shape)} on {device}")
-    out_scores = torch.empty((R, keep), dtype=torch.float32, device=device)
-    picked = torch.empty((2, R, keep), dtype=torch.int32, device=device)
+        raise ValueError(f"beam_select: up to {MAX_BEAMS} beams, up to {MAX_KEEP} kept and a padding token of the vocabulary (got {K}, {keep}, {pad} of {V})")
+    if done is not None and (done.dtype is not torch.bool or done.get_device() != index or done.shape != pair or not done.is_contiguous()):
+        raise ValueError(f"beam_select: done must be dense bool {tuple(pair)} on {logits.device}")
+    best = scores.new_empty((R, keep))
+    parents = torch.empty_like(best, dtype=torch.int32)
+    tokens = torch.empty_like(parents)
     if R:
         parts = fn("candidates", "cellm_beam_parts")(V)
-        # the rows' sums (two 64-bit numbers a part), then their lanes' maxima (32 floats a part)
-        ws = torch.empty(rows * parts * 36, dtype=torch.float32, device=device)
+        # the rows' sums (16 bytes a part), then their lanes' maxima (32 floats a part)
+        ws = scores.new_empty(rows * parts * 36)
         at = ws.data_ptr()
-        launch("candidates", name, logits, ptr(out_scores), picked.data_ptr(), picked.data_ptr() + 4 * R * keep, at + 16 * rows * parts, at, ptr(logits),
-               logits.stride(0) if rows > 1 else V, V, R, K, int(keep), ptr(scores), ptr(done), int(pad), DTYPE_TAG[logits.dtype], kernels=2)
-    return out_scores, picked[0], picked[1]
-
-
-def _beams(name: str, parents: torch.Tensor, err: torch.Tensor):
-    if parents.dim() != 2 or not parents.is_cuda or not 0 < parents.shape[1] <= MAX_BEAMS or err.numel() < 1:
-        raise ValueError(f"{name}: parents int32 [requests, beams] with up to {MAX_BEAMS} beams on the GPU, and an error word")
-    require_ints(name, parents.device, parents=parents, err=err)
-    return parents.shape
+        launch_packed("candidates", "beam_select", index,
+                      _SELECT_ARGS(best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at + 16 * rows * parts, at, logits.data_ptr(), stride[0] if rows > 1 else V, V,
+                                   R, K, keep, scores.data_ptr(), 0 if done is None else done.data_ptr(), pad, DTYPE_TAG[logits.dtype]), 2)
+    return best, parents, tokens
 
 
 def reorder_states(state: torch.Tensor, slot_ids: torch.Tensor, parents: torch.Tensor, err: torch.Tensor) -> None:
@@ -53,15 +50,17 @@ def reorder_states(state: torch.Tensor, slot_ids: torch.Tensor, parents: torch.T
     keeps a group's states), of any element type; slot_ids int32 [requests * beams] (or [requests, beams]), a slot for each beam and no
     slot for two. A parent of -1, or the beam itself, leaves its state as it is. A parent or slot out of range is reported in `err` and
     the beam left alone."""
-    name = "reorder_states"
-    R, K = _beams(name, parents, err)
-    require_ints(name, parents.device, slot_ids=slot_ids)
-    if state.dim() < 2 or state.device != parents.device or not state.is_contiguous() or slot_ids.numel() != R * K or state.element_size() % 2:
-        raise ValueError(f"{name}: a dense state [items, slots, ...] of elements of 2, 4 or 8 bytes on {parents.device} and {R * K} slots")
-    items, slots = state.shape[:2]
-    if state.numel() == 0 or R == 0:
-        return
-    launch("candidates", name, state, ptr(state), ptr(slot_ids), ptr(parents), R, K, items, slots, state.numel() // (items * slots) * state.element_size(), ptr(err))
+    index, shape, pair = parents.get_device(), state.shape, parents.shape
+    if index < 0 or len(pair) != 2 or not 0 < pair[1] <= MAX_BEAMS or not dense_ints(index, parents, slot_ids, err) or err.numel() < 1:
+        raise ValueError(f"reorder_states: dense int32 parents [requests, beams] with up to {MAX_BEAMS} beams, slots and an error word on one GPU")
+    R, K = pair
+    e = state.element_size()
+    if len(shape) < 2 or state.get_device() != index or not state.is_contiguous() or slot_ids.numel() != R * K or e % 2:
+        raise ValueError(f"reorder_states: a dense state [items, slots, ...] of elements of 2, 4 or 8 bytes on {parents.device} and {R * K} slots")
+    n = state.numel()
+    if n and R:
+        launch_packed("candidates", "reorder_states", index,
+                      _STATES_ARGS(state.data_ptr(), slot_ids.data_ptr(), parents.data_ptr(), R, K, shape[0], shape[1], n // (shape[0] * shape[1]) * e, err.data_ptr()))
 
 
 def reorder_pages(k_pool: torch.Tensor, v_pool: Optional[torch.Tensor], block_table: torch.Tensor, starts: torch.Tensor, ends: torch.Tensor,
@@ -71,21 +70,22 @@ def reorder_pages(k_pool: torch.Tensor, v_pool: Optional[torch.Tensor], block_ta
     on pages of its own; what lies before `starts` (the prompt) is the same for all beams of a request and stays. A parent of -1, or the
     beam itself, leaves the rows as they are, an entry of -1 (a page given back) the rows on it. A parent, page or row out of range
     is reported in `err` and passed over."""
-    name = "reorder_pages"
-    R, K = _beams(name, parents, err)
-    device = parents.device
-    require_ints(name, device, block_table=block_table, starts=starts, ends=ends)
-    if block_table.dim() != 2 or block_table.shape[0] != R * K or starts.numel() != R or ends.numel() != R:
-        raise ValueError(f"{name}: block_table [{R * K}, entries], starts [{R}] and ends [{R}]")
-    pools = [p for p in (k_pool, v_pool) if p is not None]
+    index, pair, table = parents.get_device(), parents.shape, block_table.shape
+    if index < 0 or len(pair) != 2 or not 0 < pair[1] <= MAX_BEAMS or not dense_ints(index, parents, block_table, starts, ends, err) or err.numel() < 1:
+        raise ValueError(f"reorder_pages: dense int32 parents [requests, beams] with up to {MAX_BEAMS} beams, block_table, starts, ends and an error word on one GPU")
+    R, K = pair
+    if len(table) != 2 or table[0] != R * K or starts.numel() != R or ends.numel() != R:
+        raise ValueError(f"reorder_pages: block_table [{R * K}, entries], starts [{R}] and ends [{R}]")
+    own = k_pool.shape[:-1]
+    pools = (k_pool,) if v_pool is None else (k_pool, v_pool)
     for p in pools:
-        if p.dim() not in (4, 5) or p.device != device or not p.is_contiguous() or p.element_size() % 2 or p.shape[:-1] != k_pool.shape[:-1]:
-            raise ValueError(f"{name}: dense pools [items, pages, kv heads, page size, head size] of elements of 2, 4 or 8 bytes on {device}, alike but for the head size")
-    if R == 0 or block_table.shape[1] == 0:
+        if len(own) not in (3, 4) or p.shape[:-1] != own or p.get_device() != index or not p.is_contiguous() or p.element_size() % 2:
+            raise ValueError("reorder_pages: dense pools [items, pages, kv heads, page size, head size] of elements of 2, 4 or 8 bytes, alike but for the head size, "
+                             f"on {parents.device}")
+    if R == 0 or table[1] == 0:
         return
     for p in pools:
-        items = p.shape[0] if p.dim() == 5 else 1
-        pages, nkv, page_size, width = p.shape[-4:]
         if p.numel():
-            launch("candidates", name, p, ptr(p), ptr(block_table), block_table.shape[1], ptr(starts), ptr(ends), ptr(parents), R, K, items, pages, nkv, page_size,
-                   width * p.element_size(), ptr(err))
+            launch_packed("candidates", "reorder_pages", index,
+                          _PAGES_ARGS(p.data_ptr(), block_table.data_ptr(), table[1], starts.data_ptr(), ends.data_ptr(), parents.data_ptr(), R, K,
+                                      own[0] if len(own) == 4 else 1, own[-3], own[-2], own[-1], p.shape[-1] * p.element_size(), err.data_ptr()))

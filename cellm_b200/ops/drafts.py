@@ -7,23 +7,28 @@ that is what its query and key are to be rotated by (`qk_norm_rope` with nkv = 0
 and values stay beside the cache until `accept_drafts` has found which of them are kept."""
 from __future__ import annotations
 
+from struct import Struct
 from typing import Optional, Sequence
 
 import torch
 
-from ._lib import DTYPE_TAG, fn, launch, ptr, require_ints
-from ._state import sm_count
+from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
+from ._state import _SM_COUNT, sm_count
 
 MAX_TREE = 256                     # nodes of a tree (TREE_MAX in draft_tree.cuh)
+_TREE_ARGS, _ACCEPT_ARGS = Struct("24qd4q").pack, Struct("28q").pack
 
 
-def _rows(name: str, what: str, t: torch.Tensor, T: int, width: int, like: torch.Tensor) -> int:
-    """The row pitch of `t` [T, width], or [T, heads, head size] with dense heads, in elements."""
-    inner = t.stride(-1) == 1 and (t.dim() == 2 or (t.dim() == 3 and t.stride(1) == t.shape[2]))
-    if t.dtype != like.dtype or t.device != like.device or t.shape[0] != T or t.numel() != T * width or (T and not inner):
-        raise ValueError(f"{name}: {what} must be [{T}, {width}] rows of {like.dtype} on {like.device} with dense rows "
-                         f"(got {tuple(t.shape)}, strides {t.stride()}, {t.dtype}, {t.device})")
-    return t.stride(0) if T > 1 else width
+def _pitch(t: torch.Tensor, T: int, width: int, dtype, index: int) -> int:
+    """The row pitch of `t`, [T, width] or [T, heads, head size] with dense rows of `width` values, in elements; -1: it is none."""
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not dtype or t.get_device() != index or shape[0] != T:
+        return -1
+    if len(shape) == 2:
+        ok = shape[1] == width and (stride[1] == 1 or width == 1)
+    else:
+        ok = len(shape) == 3 and shape[1] * shape[2] == width and stride[2] == 1 and (stride[1] == shape[2] or shape[1] == 1)
+    return (stride[0] if T > 1 else width) if ok or T == 0 else -1
 
 
 def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, parents: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -37,56 +42,66 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     most 256, and `tree_lens` is the host's copy of their numbers. `max_ctx`: the longest context if the host knows it (0: what the
     block table can name). float32 or bfloat16, heads of up to 256. Returns [T, nh * hd]. A row of K or V that is not finite may reach
     every node of its tree. Nothing is read or written of padding and of page entries that no node sees."""
-    name = "attention_tree"
-    if not q.is_cuda or k_pool.dim() != 4 or q.dtype not in DTYPE_TAG:
-        raise ValueError(f"{name}: float32 or bfloat16 rows on the GPU over pools [pages, kv heads, page size, head size]")
-    pages, nkv, page_size, hd = k_pool.shape
-    T, B, device = q.shape[0], len(tree_lens), q.device
+    dtype, index, shape, table, T, B = q.dtype, q.get_device(), k_pool.shape, block_table.shape, q.shape[0], len(tree_lens)
+    if index < 0 or dtype not in DTYPE_TAG or len(shape) != 4:
+        raise ValueError("attention_tree: float32 or bfloat16 rows on the GPU over pools [pages, kv heads, page size, head size]")
+    pages, nkv, page_size, hd = shape
     if nkv <= 0 or nh <= 0 or nh % nkv or not 0 < hd <= 256:
-        raise ValueError(f"{name}: {nh} heads over {nkv} of {hd}: whole groups of heads of up to 256 only")
-    for pool in (k_pool, v_pool):
-        if pool.dtype != q.dtype or pool.device != device or not pool.is_contiguous() or pool.shape != k_pool.shape:
-            raise ValueError(f"{name}: dense pools of {q.dtype} and one shape on {device}")
-    q_ld, k_ld, v_ld = (_rows(name, what, t, T, w, q) for what, t, w in (("q", q, nh * hd), ("k_new", k_new, nkv * hd), ("v_new", v_new, nkv * hd)))
-    require_ints(name, device, parents=parents, cu_seqlens=cu_seqlens, ctx_lens=ctx_lens, block_table=block_table, err=err)
-    if parents.numel() != T or cu_seqlens.numel() != B + 1 or ctx_lens.numel() != B or block_table.dim() != 2 or block_table.shape[0] != B or err.numel() < 1:
-        raise ValueError(f"{name}: parents [{T}], cu_seqlens [{B + 1}], ctx_lens [{B}], block_table [{B}, entries] and an error word")
-    most = max(tree_lens, default=0)
-    if most > MAX_TREE or min(tree_lens, default=0) < 0 or sum(tree_lens) > T:
-        raise ValueError(f"{name}: trees of 0 to {MAX_TREE} nodes, {T} in all (got {list(tree_lens)})")
+        raise ValueError(f"attention_tree: {nh} heads over {nkv} of {hd}: whole groups of heads of up to 256 only")
+    if v_pool.shape != shape or k_pool.dtype is not dtype or v_pool.dtype is not dtype or k_pool.get_device() != index or v_pool.get_device() != index \
+            or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+        raise ValueError(f"attention_tree: dense pools of {dtype} and one shape on {q.device}")
+    q_ld, k_ld, v_ld = _pitch(q, T, nh * hd, dtype, index), _pitch(k_new, T, nkv * hd, dtype, index), _pitch(v_new, T, nkv * hd, dtype, index)
+    if q_ld < 0 or k_ld < 0 or v_ld < 0:
+        raise ValueError(f"attention_tree: q [{T}, {nh * hd}], k_new and v_new [{T}, {nkv * hd}] of {dtype} on {q.device} with dense rows (got "
+                         + ", ".join(f"{tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}" for t in (q, k_new, v_new)) + ")")
+    if not dense_ints(index, parents, cu_seqlens, ctx_lens, block_table, err):
+        raise ValueError(f"attention_tree: parents, cu_seqlens, ctx_lens, block_table and err must be dense int32 on {q.device}")
+    if parents.numel() != T or cu_seqlens.numel() != B + 1 or ctx_lens.numel() != B or len(table) != 2 or table[0] != B or err.numel() < 1:
+        raise ValueError(f"attention_tree: parents [{T}], cu_seqlens [{B + 1}], ctx_lens [{B}], block_table [{B}, entries] and an error word")
+    most = max(tree_lens) if B else 0
+    if B and (most > MAX_TREE or min(tree_lens) < 0 or sum(tree_lens) > T):
+        raise ValueError(f"attention_tree: trees of 0 to {MAX_TREE} nodes, {T} in all (got {list(tree_lens)})")
     if window < 0 or max_ctx < 0:
-        raise ValueError(f"{name}: window and max_ctx must not be negative")
-    out = torch.empty((T, nh * hd), dtype=q.dtype, device=device)
+        raise ValueError("attention_tree: window and max_ctx must not be negative")
+    out = q.new_empty((T, nh * hd))
     if most == 0:
         return out
-    entries = block_table.shape[1]
-    keys = min(max_ctx or entries * page_size, entries * page_size)
-    keys = min(keys, window) if window else keys
-    nsplit = fn("attention_tree", "cellm_attention_tree_pieces")(B, most, nh, nkv, hd, keys + most, DTYPE_TAG[q.dtype], sm_count(device))
-    part_o = part_ml = None
+    entries, tag = table[1], DTYPE_TAG[dtype]
+    keys = entries * page_size
+    if 0 < max_ctx < keys:
+        keys = max_ctx
+    if 0 < window < keys:
+        keys = window
+    nsplit = fn("attention_tree", "cellm_attention_tree_pieces")(B, most, nh, nkv, hd, keys + most, tag, _SM_COUNT.get(index) or sm_count(index))
+    part_o = part_ml = 0
     if nsplit > 1:
-        ws = torch.empty(nsplit * T * nh * (hd + 2), dtype=torch.float32, device=device)
-        part_o, part_ml = ws.data_ptr(), ws.data_ptr() + 4 * nsplit * T * nh * hd
-    launch("attention_tree", name, q, ptr(out), part_o, part_ml, ptr(q), q_ld, ptr(k_new), k_ld, ptr(v_new), v_ld, ptr(parents), ptr(k_pool), ptr(v_pool),
-           ptr(cu_seqlens), ptr(ctx_lens), ptr(block_table), entries, B, T, most, pages, page_size, nh, nkv, hd, float(scale), int(window), nsplit,
-           DTYPE_TAG[q.dtype], ptr(err), kernels=2 if nsplit > 1 else 1)
+        ws = q.new_empty(nsplit * T * nh * (hd + 2), dtype=torch.float32)
+        part_o = ws.data_ptr()
+        part_ml = part_o + 4 * nsplit * T * nh * hd
+    launch_packed("attention_tree", "attention_tree", index,
+                  _TREE_ARGS(out.data_ptr(), part_o, part_ml, q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, parents.data_ptr(), k_pool.data_ptr(),
+                             v_pool.data_ptr(), cu_seqlens.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), entries, B, T, most, pages, page_size, nh, nkv, hd,
+                             scale, window, nsplit, tag, err.data_ptr()), 2 if nsplit > 1 else 1)
     return out
 
 
-def _draft_rows(new: Optional[torch.Tensor], pool: Optional[torch.Tensor], T: int, what: str):
-    """Pointer, bytes between items and nodes, bytes of a head's row, pointer to the pool: of one of keys and values."""
-    if new is None:
-        return None, 0, 0, 0, None
-    if new.dim() == 3:
-        new = new.unsqueeze(0)
-    items, pages, nkv, page_size, width = pool.shape
-    if new.dim() != 4 or new.shape != (items, T, nkv, width) or new.dtype != pool.dtype or new.device != pool.device or not pool.is_contiguous():
-        raise ValueError(f"accept_drafts: {what}_new must be [{items}, {T}, {nkv}, {width}] {pool.dtype} beside its dense pool {tuple(pool.shape)} "
-                         f"(got {tuple(new.shape)} {new.dtype})")
-    if new.numel() and (new.stride(3) != 1 or (nkv > 1 and new.stride(2) != width)):
-        raise ValueError(f"accept_drafts: a node's {what} heads must lie side by side")
+def _layers(new: torch.Tensor, pool: torch.Tensor, T: int, index: int):
+    """Bytes between items and between nodes of `new` [items, T, heads, size] beside its pool [items, pages, heads, page size, size], and
+    bytes of a head's row; None where the two do not fit. Either may lack its first axis."""
+    shape, stride, own = new.shape, new.stride(), pool.shape
+    if len(shape) == 3:
+        shape, stride = (1, *shape), (0, *stride)
+    if len(own) == 4:
+        own = (1, *own)
+    if len(shape) != 4 or len(own) != 5 or new.dtype is not pool.dtype or new.get_device() != index or pool.get_device() != index or not pool.is_contiguous():
+        return None
+    if shape[0] != own[0] or shape[1] != T or shape[2] != own[2] or shape[3] != own[4]:
+        return None
+    if T and own[0] and ((stride[3] != 1 and shape[3] > 1) or (stride[2] != shape[3] and shape[2] > 1)):
+        return None
     e = new.element_size()
-    return new.data_ptr(), new.stride(0) * e if items > 1 else 0, new.stride(1) * e if T > 1 else 0, width * e, pool.data_ptr()
+    return (stride[0] * e if own[0] > 1 else 0), (stride[1] * e if T > 1 else 0), shape[3] * e, own
 
 
 def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Tensor, cu_seqlens: torch.Tensor, longest: int, err: torch.Tensor,
@@ -101,32 +116,33 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
     the last one, -1 where there is none). With the nodes' keys and values k_new and v_new [items, T, nkv, hd] (or without the first
     axis) and the pools [items, pages, nkv, page size, hd] (or without it) the standing nodes' rows are written to places ctx_lens[b],
     ctx_lens[b] + 1, ... of the request's pages; v_new and v_pool None: keys alone."""
-    name = "accept_drafts"
-    device = tokens.device
-    if not tokens.is_cuda or longest < 1:
-        raise ValueError(f"{name}: arrays on the GPU and a longest path of at least one node")
-    require_ints(name, device, tokens=tokens, parents=parents, choices=choices, cu_seqlens=cu_seqlens, err=err)
-    T, B = tokens.numel(), cu_seqlens.numel() - 1
+    index, T, B = tokens.get_device(), tokens.numel(), cu_seqlens.numel() - 1
+    if index < 0 or longest < 1 or not dense_ints(index, tokens, parents, choices, cu_seqlens, err):
+        raise ValueError("accept_drafts: dense int32 arrays on one GPU and a longest path of at least one node")
     if parents.numel() != T or choices.numel() != T or B < 0 or err.numel() < 1:
-        raise ValueError(f"{name}: tokens, parents and choices of one length, cu_seqlens [requests + 1], an error word")
-    items = nkv = pages = page_size = entries = 0
+        raise ValueError("accept_drafts: tokens, parents and choices of one length, cu_seqlens [requests + 1], an error word")
     if (k_new is None) != (k_pool is None) or (v_new is None) != (v_pool is None) or (v_new is not None and k_new is None):
-        raise ValueError(f"{name}: rows and pool of the keys (and of the values) together")
+        raise ValueError("accept_drafts: rows and pool of the keys (and of the values) together")
+    rows = (0,) * 10
+    where = (0,) * 7
     if k_new is not None:
-        if ctx_lens is None or block_table is None:
-            raise ValueError(f"{name}: rows are written behind ctx_lens on the pages of block_table")
-        require_ints(name, device, ctx_lens=ctx_lens, block_table=block_table)
-        if ctx_lens.numel() != B or block_table.dim() != 2 or block_table.shape[0] != B or k_pool.device != device:
-            raise ValueError(f"{name}: ctx_lens [{B}] and block_table [{B}, entries] on {device}")
-        k_pool = k_pool.unsqueeze(0) if k_pool.dim() == 4 else k_pool
-        v_pool = v_pool.unsqueeze(0) if v_pool is not None and v_pool.dim() == 4 else v_pool
-        if k_pool.dim() != 5 or (v_pool is not None and v_pool.shape[:4] != k_pool.shape[:4]):
-            raise ValueError(f"{name}: pools [items, pages, kv heads, page size, head size] of one shape but for the head size")
-        items, pages, nkv, page_size, _ = k_pool.shape
-        entries = block_table.shape[1]
-    k, v = _draft_rows(k_new, k_pool, T, "k"), _draft_rows(v_new, v_pool, T, "v")
-    out = torch.empty((B, longest + 2), dtype=torch.int32, device=device).view(-1)
-    count, after, path = out[:B], out[B:2 * B], out[2 * B:].view(B, longest)
-    launch("candidates", name, tokens, ptr(count), ptr(path), ptr(after), ptr(tokens), ptr(parents), ptr(choices), ptr(cu_seqlens), B, T, int(longest), *k, *v,
-           ptr(ctx_lens), ptr(block_table), entries, items, nkv, pages, page_size, ptr(err))
+        if ctx_lens is None or block_table is None or not dense_ints(index, ctx_lens, block_table) or ctx_lens.numel() != B or block_table.dim() != 2 \
+                or block_table.shape[0] != B:
+            raise ValueError(f"accept_drafts: rows are written behind ctx_lens [{B}] on the pages of block_table [{B}, entries], dense int32 on {tokens.device}")
+        k = _layers(k_new, k_pool, T, index)
+        v = (0, 0, 0, None) if v_new is None else _layers(v_new, v_pool, T, index)
+        if k is None or v is None or (v_new is not None and v[3][:4] != k[3][:4]):
+            raise ValueError("accept_drafts: k_new and v_new [items, T, kv heads, head size], a node's heads side by side, of the type of their dense pools [items, pages, "
+                             f"kv heads, page size, head size] (got {[tuple(t.shape) for t in (k_new, v_new, k_pool, v_pool) if t is not None]})")
+        items, pages, nkv, page_size, _ = k[3]
+        rows = (k_new.data_ptr(), k[0], k[1], k[2], k_pool.data_ptr()) + ((v_new.data_ptr(), v[0], v[1], v[2], v_pool.data_ptr()) if v_new is not None else (0,) * 5)
+        where = (ctx_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], items, nkv, pages, page_size)
+    path = tokens.new_empty((B, longest))
+    count = torch.empty_like(ctx_lens) if ctx_lens is not None and ctx_lens.dim() == 1 and ctx_lens.numel() == B and ctx_lens.dtype is torch.int32 \
+        and ctx_lens.get_device() == index else tokens.new_empty(B)
+    after = torch.empty_like(count)
+    if B:
+        launch_packed("candidates", "accept_drafts", index,
+                      _ACCEPT_ARGS(count.data_ptr(), path.data_ptr(), after.data_ptr(), tokens.data_ptr(), parents.data_ptr(), choices.data_ptr(), cu_seqlens.data_ptr(),
+                                   B, T, longest, *rows, *where, err.data_ptr()))
     return count, path, after
