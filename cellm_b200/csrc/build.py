@@ -46,7 +46,7 @@ LIBRARIES: dict[str, tuple[str, list[str], list[str]]] = {
     "attention_expanded": ("nvcc", ["kernels/attention_expanded.cu"], []),
     "decay_chunks": ("nvcc", ["kernels/decay_chunks.cu"], []),
     "state_chunks": ("nvcc", ["kernels/state_chunks.cu"], []),
-    "attention_tree": ("nvcc", ["kernels/attention_tree.cu"], []),
+    "attention_tree": ("nvcc", ["kernels/attention_tree.cu", "kernels/attention_tree_tc.cu"], []),
     "candidates": ("nvcc", ["kernels/drafts.cu", "kernels/beams.cu"], []),
 }
 

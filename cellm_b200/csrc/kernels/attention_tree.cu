@@ -11,68 +11,10 @@
 #include <algorithm>
 #include <climits>
 
-#include "draft_tree.cuh"
+#include "attention_tree.cuh"
 #include "mma_tiles.cuh"
 
 namespace {
-
-// What all kernels of this file are given.
-struct TreeArgs {
-    void* out;                    // [T, nh * hd]
-    float* part_o;                // [nsplit, T * nh, hd], where the keys are cut
-    float* part_ml;               // [nsplit, T * nh, 2]
-    const void *q, *k_new, *v_new;   // rows of node t at q + t * q_ld, k_new + t * k_ld, ...
-    long long q_ld, k_ld, v_ld;   // in elements
-    const int* parents;           // [T]
-    const void *k_pool, *v_pool;  // [pages][nkv][page_size][hd]
-    const int *cu_seqlens, *ctx_lens, *block_table;
-    int bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, tiles, nsplit, window;
-    float scale_log2e;
-    int* err;
-};
-
-// A block's share of the work: request, key/value head, piece of the keys, tile of rows.
-struct TreeTile {
-    int b, kvh, split, tile, t_base, n, ctx;
-    bool live;
-};
-__device__ __forceinline__ TreeTile tree_tile(const TreeArgs& a) {
-    TreeTile t;
-    int i = blockIdx.x;
-    t.tile = i % a.tiles, i /= a.tiles;
-    t.split = i % a.nsplit, i /= a.nsplit;
-    t.kvh = i % a.nkv;
-    t.b = i / a.nkv;
-    t.t_base = a.cu_seqlens[t.b];
-    t.n = a.cu_seqlens[t.b + 1] - t.t_base;
-    t.ctx = a.ctx_lens[t.b];
-    t.live = t.n > 0 && t.t_base >= 0 && t.t_base + t.n <= a.T;
-    if (t.n > a.most || t.n < 0 || t.t_base < 0 || t.t_base + t.n > a.T) {
-        if (threadIdx.x == 0) atomicOr(a.err, CELLM_DEV_BAD_TREE);
-        t.live = false;
-    }
-    // keys beyond what a row of the block table can name are reported and left out
-    if (t.ctx < 0 || t.ctx > (long long)a.bt_stride * a.page_size) {
-        if (threadIdx.x == 0) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
-        t.ctx = t.ctx < 0 ? 0 : (int)((long long)a.bt_stride * a.page_size);
-    }
-    return t;
-}
-
-// Which of a block's KT keys a node sees, a bit a key: committed ones from position key0 on, or (node0 >= 0) the nodes from node0 on.
-template <int KT>
-__device__ __forceinline__ uint64_t seen_bits(const TreeShape& tree, int node, int window, int ctx, int key0, int node0) {
-    static_assert(KT == 32 || KT == 64, "");
-    if (node0 >= 0) {
-        uint64_t m = tree.line[node][node0 >> 5];
-        if (KT == 64 && (node0 >> 5) + 1 < TREE_WORDS) m |= (uint64_t)tree.line[node][(node0 >> 5) + 1] << 32;
-        return m;
-    }
-    const int lo = window > 0 ? max(0, ctx + tree.depth[node] - window + 1) : 0;
-    const int below = min(max(lo - key0, 0), KT), upto = min(max(ctx - key0, 0), KT);
-    const uint64_t in = upto >= 64 ? ~0ull : (1ull << upto) - 1ull, out = below >= 64 ? ~0ull : (1ull << below) - 1ull;
-    return in & ~out;
-}
 
 // ---------------------------------------------------------------- any type, any head size up to 256
 // 128 threads take 32 rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit arithmetic: a
@@ -565,7 +507,15 @@ bool mma_takes(const TreeArgs& a) {
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
     return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0;
 }
+// Trees that fill tiles of 128 rows go to the tcgen05 kernel.
+bool tc_rows(int rows) { return rows > 64; }
 int launch_bf16(const TreeArgs& a, cudaStream_t stream) {
+    const int G = a.nh / a.nkv;
+    if (tc_rows(a.most * G) && attention_tree_tc_takes(a) && (a.most > 128 / G || a.nsplit % 2 == 0)) {
+        TreeArgs b = a;
+        if (a.most <= 128 / G) b.nsplit /= 2;               // its two tiles leave a piece each
+        return attention_tree_tc_launch(b, stream);
+    }
     if (!mma_takes(a)) return launch_plain_sized<__nv_bfloat16>(a, stream);
     if (a.hd == 32) return launch_mma_rows<32>(a, stream);
     if (a.hd == 64) return launch_mma_rows<64>(a, stream);
@@ -598,7 +548,12 @@ int launch_merge(const TreeArgs& a, cudaStream_t stream) {
 // The pieces the keys are best cut into: B trees of up to `most` nodes, `keys` the most that a node sees.
 CELLM_API int cellm_attention_tree_pieces(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
     if (B <= 0 || most <= 0 || nkv <= 0 || nh < nkv) return 1;
-    const int rows = most * (nh / nkv);
+    const int G = nh / nkv, rows = most * G;
+    if (dtype == CELLM_BF16 && hd == 64 && tc_rows(rows) && G <= 128 && 128 / G * G >= 96) {
+        const int tile = 128 / G, two = most > tile;
+        const int n = pieces((long long)B * nkv * ((most + (1 + two) * tile - 1) / ((1 + two) * tile)), ((keys + 127) / 128 + 1 - two) / (2 - two), sms);
+        return two ? n : 2 * n;
+    }
     const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
     const int tile = !mma || (rows > 16 && rows <= 32) ? 32 : rows <= 16 ? 16 : 64;
     const int an_sm = !mma ? 2 : hd == 32 ? 4 : hd == 64 ? 3 : 2;             // blocks that an SM holds, by their shared memory

@@ -1,0 +1,368 @@
+// Attention of drafted trees on the 5th-generation tensor cores (tcgen05): bfloat16, heads of 64, trees whose rows ((node, query
+// head) pairs of one key/value head) fill tiles of 128.
+//
+// One CTA takes two tiles of 128 rows through blocks of 128 keys: committed ones, a TMA box a page, then the nodes' own, a box a
+// block. Warp 0 brings queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P read from
+// tensor memory and V as its rows lie), warps 4..7 and 8..11 do the softmax of a tile each, a row a thread, so that one tile's products
+// run beside the other's softmax; they take the registers that the first warpgroup gives up. Trees of up to 128 rows have one tile: the same rows then stand in both, and the tiles take the
+// blocks in turn; their two results are two of the pieces that the merge joins.
+//
+// What it costs is exponentials: a block of 128 x 128 scores keeps the four special-function units of an SM 1,024 cycles, its
+// two products the tensor cores 512.
+//
+// Every wait on an mbarrier is bounded: a role that gives up sets CELLM_DEV_WAIT_TIMEOUT and an abort flag; the CTA frees its tensor
+// memory and returns.
+#include "attention_tree.cuh"
+#include "tcgen05_attn.cuh"
+
+namespace {
+
+constexpr int TM = 128, TN = 128, HD = 64;
+constexpr int KV_STAGES = 3;
+constexpr int TMEM_COLUMNS = 512;      // scores of tile 0 and 1 in columns 0 and 128, their outputs in 256 and 320, their weights
+constexpr int O_COL = 256, P_COL = 384;    // (bfloat16, two keys a column) in 384 and 448
+constexpr int THREADS = 384;
+
+struct TreeTcSmem {                    // starts on a 1024-byte boundary (checked in the kernel)
+    uint8_t q[2][TM * HD * 2];
+    uint8_t k[KV_STAGES][TN * HD * 2];
+    uint8_t v[KV_STAGES][TN * HD * 2];
+    TreeShape tree;
+    uint64_t q_full;
+    uint64_t k_full[KV_STAGES], k_empty[KV_STAGES];
+    uint64_t v_full[KV_STAGES], v_empty[KV_STAGES];
+    uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+
+// grid: (request, key/value head, piece, pair of tiles), the last fastest. alternate: one tile of rows, whose blocks the two tiles take
+// in turn; piece 2 * split + tile.
+__global__ void __launch_bounds__(THREADS, 1)
+attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                         const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_vn, const TreeArgs a, const int alternate) {
+    extern __shared__ __align__(1024) uint8_t tc_smem[];
+    TreeTcSmem& sm = *reinterpret_cast<TreeTcSmem*>(tc_smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (smem_u32(tc_smem) & 1023u) {             // the swizzled tiles need 1024-byte alignment
+        if (threadIdx.x == 0) atomicOr(a.err, CELLM_DEV_BAD_LAYOUT);
+        return;
+    }
+    if (threadIdx.x == 0) {
+        mbar_init(&sm.q_full, 1);
+        for (int i = 0; i < KV_STAGES; ++i) {
+            mbar_init(&sm.k_full[i], 1), mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], 1), mbar_init(&sm.v_empty[i], 1);
+        }
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&sm.s_full[t], 1), mbar_init(&sm.s_empty[t], 128);
+            mbar_init(&sm.p_full[t], 128), mbar_init(&sm.pv_done[t], 1);
+        }
+        sm.abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    // Rows of V that are never loaded must not carry NaN bits into P.V (0 * NaN); scores of keys that nobody sees are masked
+    // whatever K holds.
+    for (int i = threadIdx.x; i < (int)sizeof(sm.v) / 16; i += blockDim.x) reinterpret_cast<uint4*>(sm.v)[i] = make_uint4(0, 0, 0, 0);
+    proxy_fence();
+    if (warp == 1) tmem_alloc(&sm.tmem_base, TMEM_COLUMNS);
+    tc_fence_before();
+    pdl_wait();
+    pdl_trigger();
+    const TreeTile t = tree_tile(a);
+    const int G = a.nh / a.nkv, tile_nodes = TM / G, node_first = t.tile * (alternate ? 1 : 2) * tile_nodes;
+    const bool live = t.live && node_first < t.n;
+    if (live) read_tree(sm.tree, a.parents + t.t_base, t.n, a.window, a.err);
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem_base;
+    volatile int* abort_flag = &sm.abort_flag;
+
+    const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
+    const int first = lo / TN, committed = lo < t.ctx ? (t.ctx + TN - 1) / TN - first : 0, blocks = committed + (t.n + TN - 1) / TN;
+    const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), n_blk = live ? min(blocks, begin + per) - begin : 0;
+    const bool two = alternate || node_first + tile_nodes < t.n;
+    auto takes = [&](int tile, int j) { return alternate ? (j & 1) == tile : tile == 0 || two; };
+
+    if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+        if (live) {
+            if (lane == 0) {
+                mbar_expect_tx(&sm.q_full, (two ? 2 : 1) * tile_nodes * G * HD * 2);
+                tma_load_3d(sm.q[0], &map_q, 0, t.kvh * G, t.t_base + node_first, &sm.q_full);
+                if (two) tma_load_3d(sm.q[1], &map_q, 0, t.kvh * G, t.t_base + node_first + (alternate ? 0 : tile_nodes), &sm.q_full);
+            }
+            const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
+            const int pages_per_block = TN / a.page_size;
+            for (int j = 0; j < n_blk; ++j) {
+                const int st = j % KV_STAGES, blk = begin + j;
+                const uint32_t ph = (uint32_t)(j / KV_STAGES) & 1u;
+                const bool paged = blk < committed;
+                // lane i brings page i of a block; lane 0 a block of nodes
+                int row = -1;
+                uint32_t bytes = TN * HD * 2;
+                if (paged) {
+                    const int key0 = (first + blk) * TN + lane * a.page_size;
+                    if (lane < pages_per_block && key0 < t.ctx && key0 + a.page_size > lo) {
+                        const int page = bt[key0 / a.page_size];
+                        if (page < 0 || page >= a.num_pages) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                        else row = (page * a.nkv + t.kvh) * a.page_size;
+                    }
+                    bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, row >= 0)) * (uint32_t)a.page_size * HD * 2;
+                }
+                for (int kv = 0; kv < 2; ++kv) {
+                    uint64_t* full = kv ? &sm.v_full[st] : &sm.k_full[st];
+                    uint8_t* dst = kv ? sm.v[st] : sm.k[st];
+                    bool ok = true;
+                    if (lane == 0) ok = mbar_wait(kv ? &sm.v_empty[st] : &sm.k_empty[st], ph ^ 1u, abort_flag);
+                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                    if (!ok) { if (lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } j = n_blk; break; }
+                    if (lane == 0) mbar_expect_tx(full, bytes);
+                    __syncwarp();
+                    if (paged) { if (row >= 0) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, kv ? &map_v : &map_k, 0, row, full); }
+                    else if (lane == 0) tma_load_3d(dst, kv ? &map_vn : &map_kn, 0, t.kvh, t.t_base + (blk - committed) * TN, full);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (live && lane == 0) {
+            const uint32_t idesc_s = umma_idesc(TM, TN, false);      // S[128 x 128] = Q (K-major) . K^T (K-major)
+            const uint32_t idesc_o = umma_idesc(TM, HD, true);       // O[128 x 64] += P (K-major) . V (MN-major)
+            int n_s[2] = {0, 0}, n_pv[2] = {0, 0};
+            bool ok = mbar_wait(&sm.q_full, 0, abort_flag);
+            auto issue_s = [&](int j) -> bool {
+                const int st = j % KV_STAGES;
+                if (!mbar_wait(&sm.k_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag)) return false;
+                const uint64_t dk = umma_desc(smem_u32(sm.k[st]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (!takes(i, j)) continue;
+                    if (n_s[i] > 0 && !mbar_wait(&sm.s_empty[i], (uint32_t)(n_s[i] - 1) & 1u, abort_flag)) return false;
+                    tc_fence_after();
+                    const uint64_t dq = umma_desc(smem_u32(sm.q[i]));
+#pragma unroll
+                    for (int ks = 0; ks < HD / 16; ++ks)
+                        umma_bf16(tmem + (uint32_t)(i * TN), dq + (uint64_t)(ks * 2), dk + (uint64_t)(ks * 2), idesc_s, ks != 0 ? 1u : 0u);
+                    umma_commit(&sm.s_full[i]);
+                    ++n_s[i];
+                }
+                umma_commit(&sm.k_empty[st]);
+                return true;
+            };
+            if (ok && n_blk > 0) ok = issue_s(0);
+            for (int j = 0; ok && j < n_blk; ++j) {
+                const int st = j % KV_STAGES;
+                if (j + 1 < n_blk) { ok = issue_s(j + 1); if (!ok) break; }
+                ok = mbar_wait(&sm.v_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag);
+                if (!ok) break;
+                const uint64_t dv = umma_desc(smem_u32(sm.v[st]));
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (!takes(i, j)) continue;
+                    ok = mbar_wait(&sm.p_full[i], (uint32_t)n_pv[i] & 1u, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < TN / 16; ++ks) {
+                        const uint32_t pa = tmem + (uint32_t)(P_COL + i * (TN / 2) + ks * 8);     // 16 keys = 8 columns of P
+                        const uint64_t db = dv + (uint64_t)(ks * 16 * HD * 2 / 16);               // 16 keys = 16 rows of V
+                        umma_bf16_ts(tmem + (uint32_t)(O_COL + i * HD), pa, db, idesc_o, (n_pv[i] | ks) != 0 ? 1u : 0u);
+                    }
+                    umma_commit(&sm.pv_done[i]);
+                    ++n_pv[i];
+                }
+                if (!ok) break;
+                umma_commit(&sm.v_empty[st]);
+            }
+            if (!ok) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); }
+        }
+    }
+    } else {
+        // 384 x 168 registers at launch: as many as 128 x 56 and 256 x 224
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+        const int i = (warp >> 2) - 1;                                // which tile
+        if (live && (i == 0 || two)) {
+        const int r = (warp & 3) * 32 + lane;                         // row of the tile = lane of tensor memory
+        const int node = node_first + (alternate ? 0 : i * tile_nodes) + r / G;
+        const bool row_ok = r < tile_nodes * G && node < t.n, seeing = row_ok && sm.tree.depth[node] >= 0;
+        const int open_from = a.window > 0 ? t.ctx + t.n - a.window : 0;      // no row's window starts behind it
+        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_col = (uint32_t)(i * TN), o_col = (uint32_t)(O_COL + i * HD), p_col = (uint32_t)(P_COL + i * (TN / 2));
+        float m = -INFINITY, l = 0.f;
+        bool ok = true;
+        int it = 0;
+        for (int j = alternate ? i : 0; j < n_blk; j += alternate ? 2 : 1, ++it) {
+            ok = mbar_wait(&sm.s_full[i], (uint32_t)it & 1u, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t s[TN];
+#pragma unroll
+            for (int c = 0; c < TN / 32; ++c) tmem_ld32_nowait(lane_base + s_col + (uint32_t)(c * 32), s + c * 32);
+            tmem_ld_wait();
+            tc_fence_before();
+            mbar_arrive(&sm.s_empty[i]);                              // the scores are in registers now
+            const int blk = begin + j, key0 = (first + blk) * TN, node0 = (blk - committed) * TN;
+            const bool paged = blk < committed;
+            if (!paged || key0 + TN > t.ctx || key0 < open_from) {
+#pragma unroll
+                for (int c = 0; c < TN; c += 64) {
+                    const uint64_t seen = seeing && (paged || node0 + c < TREE_MAX) ? seen_bits<64>(sm.tree, node, a.window, t.ctx, key0 + c, paged ? -1 : node0 + c) : 0ull;
+                    const uint32_t half[2] = {(uint32_t)seen, (uint32_t)(seen >> 32)};
+#pragma unroll
+                    for (int k = 0; k < 64; ++k)
+                        if (!(half[k / 32] >> (k % 32) & 1u)) s[c + k] = 0xff800000u;
+                }
+            }
+            float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < TN; k += 4) {
+                mx0 = fmaxf(mx0, __uint_as_float(s[k])), mx1 = fmaxf(mx1, __uint_as_float(s[k + 1]));
+                mx2 = fmaxf(mx2, __uint_as_float(s[k + 2])), mx3 = fmaxf(mx3, __uint_as_float(s[k + 3]));
+            }
+            const float m_new = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2e);
+            // the output is rescaled only when the maximum has grown by more than 2^RESCALE_STEP; a stale one only scales P
+            const bool want = m_new > m + RESCALE_STEP || (m == -INFINITY && m_new != -INFINITY);
+            bool pv_seen = it == 0;
+            if (__any_sync(0xffffffffu, want)) {
+                if (it > 0) {
+                    ok = mbar_wait(&sm.pv_done[i], (uint32_t)(it - 1) & 1u, abort_flag);
+                    if (!ok) break;
+                    pv_seen = true;
+                    tc_fence_after();
+                    const float corr = want ? (m == -INFINITY ? 0.f : fast_exp2(m - m_new)) : 1.0f;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld32(lane_base + o_col + (uint32_t)(c * 32), o);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                        tmem_st32(lane_base + o_col + (uint32_t)(c * 32), o);
+                    }
+                    if (want) l *= corr;
+                }
+                if (want) m = m_new;
+            }
+            const float neg_use = m == -INFINITY ? 0.f : -m;
+#pragma unroll
+            for (int k = 0; k < TN; ++k) s[k] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k]), a.scale_log2e, neg_use)));
+            float sum0 = 0.f, sum1 = 0.f, sum2 = 0.f, sum3 = 0.f;
+#pragma unroll
+            for (int k = 0; k < TN / 2; k += 2) {
+                const float a0 = __uint_as_float(s[2 * k]), a1 = __uint_as_float(s[2 * k + 1]);
+                const float a2 = __uint_as_float(s[2 * k + 2]), a3 = __uint_as_float(s[2 * k + 3]);
+                sum0 += a0, sum1 += a1, sum2 += a2, sum3 += a3;
+                s[k] = pack_bf16(a0, a1);
+                s[k + 1] = pack_bf16(a2, a3);
+            }
+            l += (sum0 + sum1) + (sum2 + sum3);
+            if (!pv_seen) {
+                ok = mbar_wait(&sm.pv_done[i], (uint32_t)(it - 1) & 1u, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+            }
+#pragma unroll
+            for (int c = 0; c < TN / 64; ++c) tmem_st32_nowait(lane_base + p_col + (uint32_t)(c * 32), s + c * 32);
+            // rows of V behind the context (the rest of its last page), of other trees and of padding become zeros before this
+            // block's P.V; tile 0, whose product is issued first, does it where both tiles take the block
+            if ((i == 0 || alternate) && (!paged || key0 + TN > t.ctx)) {
+                const int st = j % KV_STAGES;
+                ok = mbar_wait(&sm.v_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag);
+                if (!ok) break;
+                if (paged ? key0 + r >= t.ctx : node0 + r >= t.n || sm.tree.depth[node0 + r] < 0) {
+#pragma unroll
+                    for (int c = 0; c < HD * 2 / 16; ++c) reinterpret_cast<uint4*>(sm.v[st] + r * HD * 2)[c] = make_uint4(0, 0, 0, 0);
+                }
+                proxy_fence();
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&sm.p_full[i]);
+        }
+        if (ok && it > 0) ok = mbar_wait(&sm.pv_done[i], (uint32_t)(it - 1) & 1u, abort_flag);
+        if (!ok && lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); }
+        if (ok) {
+            tc_fence_after();
+            const long long gr = (long long)(t.t_base + node) * a.nh + t.kvh * G + r % G;
+            const bool parted = alternate || a.nsplit > 1;
+            const long long piece = alternate ? t.split * 2 + i : t.split;
+            const float inv = seeing && l != 0.f ? 1.0f / l : 0.f;
+            if (parted && row_ok)
+                *reinterpret_cast<float2*>(a.part_ml + (piece * a.T * a.nh + gr) * 2) = it > 0 && seeing ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+                uint32_t o[32];
+                if (it > 0) {
+                    tmem_ld32(lane_base + o_col + (uint32_t)(c * 32), o);
+                }
+                if (!(it > 0 && seeing)) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = 0u;
+                }
+                if (parted && row_ok) {
+                    float4* dst = reinterpret_cast<float4*>(a.part_o + (piece * a.T * a.nh + gr) * HD + c * 32);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        dst[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                } else if (row_ok) {
+                    uint4* dst = reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + gr * HD + c * 32);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            w[x] = pack_bf16(__uint_as_float(o[8 * k + 2 * x]) * inv, __uint_as_float(o[8 * k + 2 * x + 1]) * inv);
+                        dst[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+            }
+        }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) tmem_dealloc(tmem, TMEM_COLUMNS);
+}
+
+bool encode(CUtensorMap* out, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+    EncodeTiledFn enc = encode_fn();
+    if (!enc) return false;
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return enc(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// rows of T nodes, `heads` heads of 64 each, `ld` elements between nodes; boxes of box_heads x box_nodes
+bool encode_rows(CUtensorMap* out, const void* base, int T, int heads, long long ld, int box_heads, int box_nodes) {
+    const cuuint64_t dims[3] = {(cuuint64_t)HD, (cuuint64_t)heads, (cuuint64_t)T};
+    const cuuint64_t strides[2] = {(cuuint64_t)HD * 2, (cuuint64_t)ld * 2};
+    const cuuint32_t box[3] = {(cuuint32_t)HD, (cuuint32_t)box_heads, (cuuint32_t)box_nodes};
+    return encode(out, base, 3, dims, strides, box);
+}
+
+}  // namespace
+
+bool attention_tree_tc_takes(const TreeArgs& a) {
+    const int G = a.nh / a.nkv;
+    const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
+    return a.hd == HD && a.scale_log2e > 0.f && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0 && G <= TM && TM / G * G >= 96 &&
+           a.page_size >= 8 && a.page_size <= TN && (a.page_size & (a.page_size - 1)) == 0 && (long long)a.num_pages * a.nkv * a.page_size <= 0x7fffffffLL;
+}
+
+// part_o and part_ml hold a.nsplit pieces, twice as many where the tree's rows are one tile.
+int attention_tree_tc_launch(const TreeArgs& given, cudaStream_t stream) {
+    TreeArgs a = given;
+    const int G = a.nh / a.nkv, tile_nodes = TM / G, alternate = a.most <= tile_nodes;
+    CUtensorMap mq, mk, mv, mkn, mvn;
+    const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)a.num_pages * a.nkv * a.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)HD * 2};
+    const cuuint32_t box[2] = {(cuuint32_t)HD, (cuuint32_t)a.page_size};
+    if (!encode(&mk, a.k_pool, 2, dims, strides, box) || !encode(&mv, a.v_pool, 2, dims, strides, box) || !encode_rows(&mq, a.q, a.T, a.nh, a.q_ld, G, tile_nodes) ||
+        !encode_rows(&mkn, a.k_new, a.T, a.nkv, a.k_ld, 1, TN) || !encode_rows(&mvn, a.v_new, a.T, a.nkv, a.v_ld, 1, TN))
+        return CELLM_ERR_ARG;
+    cudaError_t e = cudaFuncSetAttribute(attention_tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(TreeTcSmem));
+    if (e != cudaSuccess) return (int)e;
+    const int pair = alternate ? tile_nodes : 2 * tile_nodes;
+    a.tiles = (a.most + pair - 1) / pair;
+    CELLM_RUN(attention_tree_tc_kernel, (unsigned)((long long)a.B * a.nkv * a.nsplit * a.tiles), THREADS, sizeof(TreeTcSmem), stream, mq, mk, mv, mkn, mvn, a, alternate);
+    return CELLM_OK;
+}
