@@ -2,7 +2,7 @@
 // head) pairs of one key/value head) fill tiles of 128.
 //
 // One CTA takes two tiles of 128 rows through blocks of 128 keys: committed ones, a TMA box a page, then the nodes' own, a box a
-// block. Warp 0 brings queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P read from
+// block. Warps 0 and 2 bring queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P read from
 // tensor memory and V as its rows lie), warps 4..7 and 8..11 do the softmax of a tile each, a row a thread, so that one tile's products
 // run beside the other's softmax; they take the registers that the first warpgroup gives up. Trees of up to 128 rows have one tile: the same rows then stand in both, and the tiles take the
 // blocks in turn; their two results are two of the pieces that the merge joins.
@@ -18,10 +18,11 @@
 namespace {
 
 constexpr int TM = 128, TN = 128, HD = 64;
-constexpr int KV_STAGES = 3;
+constexpr int KV_STAGES = 5;
 constexpr int TMEM_COLUMNS = 512;      // scores of tile 0 and 1 in columns 0 and 128, their outputs in 256 and 320, their weights
 constexpr int O_COL = 256, P_COL = 384;    // (bfloat16, two keys a column) in 384 and 448
 constexpr int THREADS = 384;
+constexpr int POLY = 2;                // pairs of exponentials of every eight that the multiply-add units form
 
 struct TreeTcSmem {                    // starts on a 1024-byte boundary (checked in the kernel)
     uint8_t q[2][TM * HD * 2];
@@ -35,6 +36,55 @@ struct TreeTcSmem {                    // starts on a 1024-byte boundary (checke
     uint32_t tmem_base;
     int abort_flag;
 };
+
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+    return d;
+}
+// Two floats in a 64-bit register, worked on by one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ float low_of(uint64_t v) {
+    return __uint_as_float((uint32_t)v);
+}
+__device__ __forceinline__ float high_of(uint64_t v) {
+    return __uint_as_float((uint32_t)(v >> 32));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// 2^x of two numbers without the special-function units: x = n + f with |f| <= 1/2, n out of the rounding of an addition, 2^f = 1 + f
+// P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.8e-6 relative, a thousandth of what rounding
+// the weight to bfloat16 costs. What lies below -126, -inf too, gives 2^-126.
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    x = pair_of(fmaxf(low_of(x), -126.f), fmaxf(high_of(x), -126.f));
+    const uint64_t r = add2(x, pair_of(12582912.f, 12582912.f)), n = add2(r, pair_of(-12582912.f, -12582912.f));
+    const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
+    uint64_t p = pair_of(0.00958284828811884f, 0.00958284828811884f);
+    p = fma2(p, f, pair_of(0.05590643361210823f, 0.05590643361210823f));
+    p = fma2(p, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
+    p = fma2(p, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
+    p = fma2(p, f, pair_of(1.f, 1.f));
+    return pair_of(__uint_as_float(__float_as_uint(low_of(p)) + (__float_as_uint(low_of(r)) << 23)),
+                   __uint_as_float(__float_as_uint(high_of(p)) + (__float_as_uint(high_of(r)) << 23)));
+}
+
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+    return is != 0;
+}
 
 // grid: (request, key/value head, piece, pair of tiles), the last fastest. alternate: one tile of rows, whose blocks the two tiles take
 // in turn; piece 2 * split + tile.
@@ -60,11 +110,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         sm.abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        for (const CUtensorMap* map : {&map_q, &map_k, &map_v, &map_kn, &map_vn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
-    // Rows of V that are never loaded must not carry NaN bits into P.V (0 * NaN); scores of keys that nobody sees are masked
-    // whatever K holds.
-    for (int i = threadIdx.x; i < (int)sizeof(sm.v) / 16; i += blockDim.x) reinterpret_cast<uint4*>(sm.v)[i] = make_uint4(0, 0, 0, 0);
-    proxy_fence();
     if (warp == 1) tmem_alloc(&sm.tmem_base, TMEM_COLUMNS);
     tc_fence_before();
     pdl_wait();
@@ -72,7 +119,6 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const TreeTile t = tree_tile(a);
     const int G = a.nh / a.nkv, tile_nodes = TM / G, node_first = t.tile * (alternate ? 1 : 2) * tile_nodes;
     const bool live = t.live && node_first < t.n;
-    if (live) read_tree(sm.tree, a.parents + t.t_base, t.n, a.window, a.err);
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
@@ -86,102 +132,112 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
     if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 0) {
+    if (warp == 0 || warp == 2) {
+        // warp 0 brings the queries and the keys, warp 2 the values: a stage of keys is free a product earlier than one of values
         if (live) {
-            if (lane == 0) {
+            const bool keys = warp == 0;
+            if (keys && lane == 0) {
                 mbar_expect_tx(&sm.q_full, (two ? 2 : 1) * tile_nodes * G * HD * 2);
                 tma_load_3d(sm.q[0], &map_q, 0, t.kvh * G, t.t_base + node_first, &sm.q_full);
                 if (two) tma_load_3d(sm.q[1], &map_q, 0, t.kvh * G, t.t_base + node_first + (alternate ? 0 : tile_nodes), &sm.q_full);
             }
             const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
             const int pages_per_block = TN / a.page_size;
+            const CUtensorMap *paged_map = keys ? &map_k : &map_v, *node_map = keys ? &map_kn : &map_vn;
+            // lane i brings page i of a block; its entry of the table is asked for a block ahead. -2: nothing of it is seen
+            auto entry = [&](int j) {
+                const int key0 = (first + begin + j) * TN + lane * a.page_size;
+                return j < n_blk && begin + j < committed && lane < pages_per_block && key0 < t.ctx && key0 + a.page_size > lo ? bt[key0 / a.page_size] : -2;
+            };
+            int next = entry(0);
             for (int j = 0; j < n_blk; ++j) {
-                const int st = j % KV_STAGES, blk = begin + j;
-                const uint32_t ph = (uint32_t)(j / KV_STAGES) & 1u;
-                const bool paged = blk < committed;
-                // lane i brings page i of a block; lane 0 a block of nodes
-                int row = -1;
-                uint32_t bytes = TN * HD * 2;
-                if (paged) {
-                    const int key0 = (first + blk) * TN + lane * a.page_size;
-                    if (lane < pages_per_block && key0 < t.ctx && key0 + a.page_size > lo) {
-                        const int page = bt[key0 / a.page_size];
-                        if (page < 0 || page >= a.num_pages) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
-                        else row = (page * a.nkv + t.kvh) * a.page_size;
-                    }
-                    bytes = (uint32_t)__popc(__ballot_sync(0xffffffffu, row >= 0)) * (uint32_t)a.page_size * HD * 2;
-                }
-                for (int kv = 0; kv < 2; ++kv) {
-                    uint64_t* full = kv ? &sm.v_full[st] : &sm.k_full[st];
-                    uint8_t* dst = kv ? sm.v[st] : sm.k[st];
-                    bool ok = true;
-                    if (lane == 0) ok = mbar_wait(kv ? &sm.v_empty[st] : &sm.k_empty[st], ph ^ 1u, abort_flag);
-                    ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                    if (!ok) { if (lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } j = n_blk; break; }
-                    if (lane == 0) mbar_expect_tx(full, bytes);
-                    __syncwarp();
-                    if (paged) { if (row >= 0) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, kv ? &map_v : &map_k, 0, row, full); }
-                    else if (lane == 0) tma_load_3d(dst, kv ? &map_vn : &map_kn, 0, t.kvh, t.t_base + (blk - committed) * TN, full);
-                }
+                const int st = j % KV_STAGES, blk = begin + j, page = next;
+                uint64_t* full = keys ? &sm.k_full[st] : &sm.v_full[st];
+                uint8_t* dst = keys ? sm.k[st] : sm.v[st];
+                next = entry(j + 1);
+                const bool paged = blk < committed, have = paged && page >= 0 && page < a.num_pages;
+                if (keys && page != -2 && !have) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                const uint32_t bytes = paged ? (uint32_t)__popc(__ballot_sync(0xffffffffu, have)) * (uint32_t)a.page_size * HD * 2 : TN * HD * 2;
+                bool ok = true;
+                if (lane == 0) ok = mbar_wait(keys ? &sm.k_empty[st] : &sm.v_empty[st], ((uint32_t)(j / KV_STAGES) & 1u) ^ 1u, abort_flag);
+                ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+                if (!ok) { if (lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } break; }
+                if (lane == 0) mbar_expect_tx(full, bytes);
+                __syncwarp();
+                if (have) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, paged_map, 0, (page * a.nkv + t.kvh) * a.page_size, full);
+                else if (!paged && lane == 0) tma_load_3d(dst, node_map, 0, t.kvh, t.t_base + (blk - committed) * TN, full);
             }
         }
     } else if (warp == 1) {
-        if (live && lane == 0) {
+        // The whole warp walks the blocks and one lane of it issues: what the products' descriptors are made of then stays in uniform
+        // registers (with the other lanes branched away, the moves into them took 3,200 cycles a pair of blocks, more than
+        // everything else).
+        if (live) {
             const uint32_t idesc_s = umma_idesc(TM, TN, false);      // S[128 x 128] = Q (K-major) . K^T (K-major)
             const uint32_t idesc_o = umma_idesc(TM, HD, true);       // O[128 x 64] += P (K-major) . V (MN-major)
-            int n_s[2] = {0, 0}, n_pv[2] = {0, 0};
+            const bool leader = elect_one();
             bool ok = mbar_wait(&sm.q_full, 0, abort_flag);
             auto issue_s = [&](int j) -> bool {
-                const int st = j % KV_STAGES;
+                const int st = j % KV_STAGES, n = alternate ? j >> 1 : j;
                 if (!mbar_wait(&sm.k_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag)) return false;
                 const uint64_t dk = umma_desc(smem_u32(sm.k[st]));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (!takes(i, j)) continue;
-                    if (n_s[i] > 0 && !mbar_wait(&sm.s_empty[i], (uint32_t)(n_s[i] - 1) & 1u, abort_flag)) return false;
+                    if (n > 0 && !mbar_wait(&sm.s_empty[i], (uint32_t)(n - 1) & 1u, abort_flag)) return false;
                     tc_fence_after();
-                    const uint64_t dq = umma_desc(smem_u32(sm.q[i]));
+                    if (leader) {
+                        const uint64_t dq = umma_desc(smem_u32(sm.q[i]));
 #pragma unroll
-                    for (int ks = 0; ks < HD / 16; ++ks)
-                        umma_bf16(tmem + (uint32_t)(i * TN), dq + (uint64_t)(ks * 2), dk + (uint64_t)(ks * 2), idesc_s, ks != 0 ? 1u : 0u);
-                    umma_commit(&sm.s_full[i]);
-                    ++n_s[i];
+                        for (int ks = 0; ks < HD / 16; ++ks)
+                            umma_bf16(tmem + (uint32_t)(i * TN), dq + (uint64_t)(ks * 2), dk + (uint64_t)(ks * 2), idesc_s, ks != 0 ? 1u : 0u);
+                        umma_commit(&sm.s_full[i]);
+                    }
+                    __syncwarp();
                 }
-                umma_commit(&sm.k_empty[st]);
+                if (leader) umma_commit(&sm.k_empty[st]);
+                __syncwarp();
                 return true;
             };
-            if (ok && n_blk > 0) ok = issue_s(0);
+            // a tile's next scores are under way while its softmax works: one block ahead, two where the tiles take turns
+            const int ahead = alternate ? 2 : 1;
+            for (int j = 0; ok && j < min(ahead, n_blk); ++j) ok = issue_s(j);
             for (int j = 0; ok && j < n_blk; ++j) {
-                const int st = j % KV_STAGES;
-                if (j + 1 < n_blk) { ok = issue_s(j + 1); if (!ok) break; }
+                const int st = j % KV_STAGES, n = alternate ? j >> 1 : j;
+                if (j + ahead < n_blk) { ok = issue_s(j + ahead); if (!ok) break; }
                 ok = mbar_wait(&sm.v_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag);
                 if (!ok) break;
                 const uint64_t dv = umma_desc(smem_u32(sm.v[st]));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (!takes(i, j)) continue;
-                    ok = mbar_wait(&sm.p_full[i], (uint32_t)n_pv[i] & 1u, abort_flag);
+                    ok = mbar_wait(&sm.p_full[i], (uint32_t)n & 1u, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
+                    if (leader) {
 #pragma unroll
-                    for (int ks = 0; ks < TN / 16; ++ks) {
-                        const uint32_t pa = tmem + (uint32_t)(P_COL + i * (TN / 2) + ks * 8);     // 16 keys = 8 columns of P
-                        const uint64_t db = dv + (uint64_t)(ks * 16 * HD * 2 / 16);               // 16 keys = 16 rows of V
-                        umma_bf16_ts(tmem + (uint32_t)(O_COL + i * HD), pa, db, idesc_o, (n_pv[i] | ks) != 0 ? 1u : 0u);
+                        for (int ks = 0; ks < TN / 16; ++ks) {
+                            const uint32_t pa = tmem + (uint32_t)(P_COL + i * (TN / 2) + ks * 8);     // 16 keys = 8 columns of P
+                            const uint64_t db = dv + (uint64_t)(ks * 16 * HD * 2 / 16);               // 16 keys = 16 rows of V
+                            umma_bf16_ts(tmem + (uint32_t)(O_COL + i * HD), pa, db, idesc_o, (n | ks) != 0 ? 1u : 0u);
+                        }
+                        umma_commit(&sm.pv_done[i]);
                     }
-                    umma_commit(&sm.pv_done[i]);
-                    ++n_pv[i];
+                    __syncwarp();
                 }
                 if (!ok) break;
-                umma_commit(&sm.v_empty[st]);
+                if (leader) umma_commit(&sm.v_empty[st]);
+                __syncwarp();
             }
-            if (!ok) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); }
+            if (!ok && lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); }
         }
     }
     } else {
         // 384 x 168 registers at launch: as many as 128 x 56 and 256 x 224
         asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int i = (warp >> 2) - 1;                                // which tile
+        // the tree's shape: wanted only where the nodes' own keys are read, so the first committed blocks are on their way meanwhile
+        if (live) read_tree(sm.tree, a.parents + t.t_base, t.n, a.window, a.err, (int)threadIdx.x - 128, 256, [] { asm volatile("bar.sync 1, 256;" ::: "memory"); });
         if (live && (i == 0 || two)) {
         const int r = (warp & 3) * 32 + lane;                         // row of the tile = lane of tensor memory
         const int node = node_first + (alternate ? 0 : i * tile_nodes) + r / G;
@@ -216,13 +272,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             float mx0 = -INFINITY, mx1 = -INFINITY, mx2 = -INFINITY, mx3 = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < TN; k += 4) {
-                mx0 = fmaxf(mx0, __uint_as_float(s[k])), mx1 = fmaxf(mx1, __uint_as_float(s[k + 1]));
-                mx2 = fmaxf(mx2, __uint_as_float(s[k + 2])), mx3 = fmaxf(mx3, __uint_as_float(s[k + 3]));
+            for (int k = 0; k < TN; k += 8) {
+                mx0 = max3(mx0, s[k], s[k + 1]), mx1 = max3(mx1, s[k + 2], s[k + 3]);
+                mx2 = max3(mx2, s[k + 4], s[k + 5]), mx3 = max3(mx3, s[k + 6], s[k + 7]);
             }
-            const float m_new = fmaxf(m, fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * a.scale_log2e);
+            mx0 = max3(mx0, __float_as_uint(mx1), __float_as_uint(mx2));
+            const float m_new = max3(m, __float_as_uint(mx0 * a.scale_log2e), __float_as_uint(mx3 * a.scale_log2e));      // NaN stays
             // the output is rescaled only when the maximum has grown by more than 2^RESCALE_STEP; a stale one only scales P
-            const bool want = m_new > m + RESCALE_STEP || (m == -INFINITY && m_new != -INFINITY);
+            const bool want = !(m_new <= m + RESCALE_STEP);
             bool pv_seen = it == 0;
             if (__any_sync(0xffffffffu, want)) {
                 if (it > 0) {
@@ -243,19 +300,21 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 if (want) m = m_new;
             }
+            // P = 2^(s c - m), two at a time; of every eight, POLY pairs come out of the multiply-add units
+            const uint64_t c2 = pair_of(a.scale_log2e, a.scale_log2e);
             const float neg_use = m == -INFINITY ? 0.f : -m;
+            const uint64_t neg2 = pair_of(neg_use, neg_use);
+            uint64_t sum0 = 0ull, sum1 = 0ull;
 #pragma unroll
-            for (int k = 0; k < TN; ++k) s[k] = __float_as_uint(fast_exp2(fmaf(__uint_as_float(s[k]), a.scale_log2e, neg_use)));
-            float sum0 = 0.f, sum1 = 0.f, sum2 = 0.f, sum3 = 0.f;
-#pragma unroll
-            for (int k = 0; k < TN / 2; k += 2) {
-                const float a0 = __uint_as_float(s[2 * k]), a1 = __uint_as_float(s[2 * k + 1]);
-                const float a2 = __uint_as_float(s[2 * k + 2]), a3 = __uint_as_float(s[2 * k + 3]);
-                sum0 += a0, sum1 += a1, sum2 += a2, sum3 += a3;
-                s[k] = pack_bf16(a0, a1);
-                s[k + 1] = pack_bf16(a2, a3);
+            for (int k = 0; k < TN; k += 2) {
+                const uint64_t x = fma2(pair_of(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), c2, neg2);
+                const uint64_t p = (k >> 1) % 8 < POLY ? exp2_poly(x) : pair_of(fast_exp2(low_of(x)), fast_exp2(high_of(x)));
+                if (k & 2) sum1 = add2(sum1, p);
+                else sum0 = add2(sum0, p);
+                s[k >> 1] = pack_bf16(low_of(p), high_of(p));
             }
-            l += (sum0 + sum1) + (sum2 + sum3);
+            sum0 = add2(sum0, sum1);
+            l += low_of(sum0) + high_of(sum0);
             if (!pv_seen) {
                 ok = mbar_wait(&sm.pv_done[i], (uint32_t)(it - 1) & 1u, abort_flag);
                 if (!ok) break;
@@ -263,13 +322,14 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
 #pragma unroll
             for (int c = 0; c < TN / 64; ++c) tmem_st32_nowait(lane_base + p_col + (uint32_t)(c * 32), s + c * 32);
-            // rows of V behind the context (the rest of its last page), of other trees and of padding become zeros before this
-            // block's P.V; tile 0, whose product is issued first, does it where both tiles take the block
-            if ((i == 0 || alternate) && (!paged || key0 + TN > t.ctx)) {
+            // Rows of V that nobody sees must not carry NaN bits into P.V (0 * NaN): those in front of the window and behind the context
+            // (not loaded, or the rest of a page), of other trees and of padding become zeros before this block's P.V. Tile 0, whose
+            // product is issued first, does it where both tiles take the block.
+            if ((i == 0 || alternate) && (!paged || key0 + TN > t.ctx || key0 < lo)) {
                 const int st = j % KV_STAGES;
                 ok = mbar_wait(&sm.v_full[st], (uint32_t)(j / KV_STAGES) & 1u, abort_flag);
                 if (!ok) break;
-                if (paged ? key0 + r >= t.ctx : node0 + r >= t.n || sm.tree.depth[node0 + r] < 0) {
+                if (paged ? key0 + r >= t.ctx || key0 + r < lo : node0 + r >= t.n || sm.tree.depth[node0 + r] < 0) {
 #pragma unroll
                     for (int c = 0; c < HD * 2 / 16; ++c) reinterpret_cast<uint4*>(sm.v[st] + r * HD * 2)[c] = make_uint4(0, 0, 0, 0);
                 }
