@@ -15,7 +15,7 @@
 // matters.
 #include <algorithm>
 
-#include "common.cuh"
+#include "mma_tiles.cuh"
 
 namespace {
 
@@ -36,67 +36,55 @@ struct RowPart {
 };
 constexpr int LARGE = 1 << 30;
 
-// 2^(x log2 e - n0) with n0 a whole number near the largest x log2 e. x log2 e = n + f with |f| <= 1/2 comes out of one rounding
-// (n) and two multiply-adds with log2 e as a float and its remainder; 2^f = 1 + f P(f), P fitted (weighted least squares,
-// reweighted towards the largest error) to 2.0e-9.
-__device__ __forceinline__ float exp_to(float x, int n0) {
-    const float r = fmaf(x, LOG2E, ROUND_MAGIC), n = r - ROUND_MAGIC;
-    const float f = fmaf(x, LOG2E_REST, fmaf(x, LOG2E, -n));
-    float p = 0.00015353357593994588f;
-    p = fmaf(p, f, 0.0013398876180872321f);
-    p = fmaf(p, f, 0.009618437848985195f);
-    p = fmaf(p, f, 0.055503323674201965f);
-    p = fmaf(p, f, 0.24022647738456726f);
-    p = fmaf(p, f, 0.6931471824645996f);
-    p = fmaf(p, f, 1.0f);
-    return __uint_as_float(__float_as_uint(p) + ((__float_as_uint(r) - (uint32_t)n0) << 23));
+// Two floats in a 64-bit register, worked on by one instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
 }
+__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 2^(x log2 e - n0) of two numbers, n0 a whole number near the largest x log2 e. x log2 e = n + f with |f| <= 1/2 comes out of one
+// rounding (n - n0, in the low bits of r) and two multiply-adds with log2 e as a float and its remainder; 2^f = 1 + f P(f), P
+// fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9.
+struct ExpTo {
+    uint64_t shifted;                         // ROUND_MAGIC - n0: adding it rounds and takes n0 off
+    float least;                              // what is smaller adds 2^-125 instead: nothing
+    __device__ __forceinline__ explicit ExpTo(int n0) {
+        const float s = ROUND_MAGIC - (float)n0;
+        shifted = pair_of(s, s), least = (float)(n0 - 125) * 0.6931472f;
+    }
+    __device__ __forceinline__ uint64_t operator()(float a, float b) const {
+        const uint64_t x = pair_of(fmaxf(a, least), fmaxf(b, least)), l2e = pair_of(LOG2E, LOG2E);
+        const uint64_t r = fma2(x, l2e, shifted), minus_n = fma2(r, pair_of(-1.f, -1.f), shifted);
+        const uint64_t f = fma2(x, pair_of(LOG2E_REST, LOG2E_REST), fma2(x, l2e, minus_n));
+        uint64_t p = pair_of(0.00015353357593994588f, 0.00015353357593994588f);
+        p = fma2(p, f, pair_of(0.0013398876180872321f, 0.0013398876180872321f));
+        p = fma2(p, f, pair_of(0.009618437848985195f, 0.009618437848985195f));
+        p = fma2(p, f, pair_of(0.055503323674201965f, 0.055503323674201965f));
+        p = fma2(p, f, pair_of(0.24022647738456726f, 0.24022647738456726f));
+        p = fma2(p, f, pair_of(0.6931471824645996f, 0.6931471824645996f));
+        p = fma2(p, f, pair_of(1.0f, 1.0f));
+        return pair_of(__uint_as_float(__float_as_uint(low_of(p)) + (__float_as_uint(low_of(r)) << 23)),
+                       __uint_as_float(__float_as_uint(high_of(p)) + (__float_as_uint(high_of(r)) << 23)));
+    }
+};
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
-}
-
-// The 16 bytes of a row from its logit `at` on, logits behind the last as -inf. Which logits a lane takes goes by their places in the
-// row alone, so that equal rows have equal sums wherever they lie: a row that does not start on a 16-byte border (`off` bytes behind
-// one) is read in aligned pieces of which each lane joins two (the second is its neighbour's first).
-template <typename T>
-__device__ __forceinline__ void load_logits(float* x, const T* row, int at, int V, int off) {
-    constexpr int N = 16 / sizeof(T);
-    if (at + N <= V) {
-        uint32_t u[8];
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(row + at) - off);
-        const uint4 w = __ldcs(src);
-        u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
-        if (off != 0) {
-            const uint4 z = __ldcs(src + 1);
-            u[4] = z.x, u[5] = z.y, u[6] = z.z, u[7] = z.w;
-            if (off & 8) {
-#pragma unroll
-                for (int i = 0; i < 6; ++i) u[i] = u[i + 2];
-            }
-            if (off & 4) {
-#pragma unroll
-                for (int i = 0; i < 5; ++i) u[i] = u[i + 1];
-            }
-            if (sizeof(T) == 2 && (off & 2)) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) u[i] = __funnelshift_r(u[i], u[i + 1], 16);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 4) {
-                x[i] = __uint_as_float(u[i]);
-            } else {
-                x[2 * i] = __uint_as_float(u[i] << 16), x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = at + i < V ? to_float(row[at + i]) : -INFINITY;
-    }
 }
 
 // The first logit of piece i of lane `lane` of warp part `part` of a row.
@@ -105,54 +93,138 @@ __device__ __forceinline__ int piece_at(int part, int i, int lane) {
     return part * WARP_VALUES + (i * 32 + lane) * (16 / (int)sizeof(T));
 }
 
-// grid (ceil(parts / ROW_WARPS), rows): tops [rows][parts * 32], sums [rows][parts]
+// A warp's ring of parts in shared memory: the aligned 16-byte pieces that a part lies in.
 template <typename T>
-__global__ void __launch_bounds__(ROW_WARPS * 32)
-beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts,
-                 const uint8_t* __restrict__ done) {
-    constexpr int N = 16 / sizeof(T), PIECES = LANE_VALUES / N;
-    pdl_wait();
-    pdl_trigger();
-    const int row = blockIdx.y, part = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    if (part >= parts || (done != nullptr && done[row])) return;
-    const T* src = logits + (long long)row * ld;
-    const int off = (int)(reinterpret_cast<uintptr_t>(src) & 15);
-    float x[LANE_VALUES];
+struct Ring {
+    static constexpr int N = 16 / sizeof(T), PIECES = LANE_VALUES / N, STAGES = sizeof(T) == 4 ? 2 : 3;
+    static constexpr int BLOCKS = sizeof(T) == 4 ? 3 : 4;                 // of ROW_WARPS warps that an SM holds, by this memory
+    uint4 piece[STAGES][PIECES * 32 + 1];
+};
+
+// Which logits a lane takes goes by their places in the row alone, so that equal rows have equal sums wherever they lie: of a row that
+// starts `off` bytes behind a 16-byte border a lane joins its own piece and the next.
+template <typename T>
+__device__ __forceinline__ void ring_load(Ring<T>& ring, int stage, const T* row, int part, int V, int lane) {
+    using R = Ring<T>;
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+    const char* src = reinterpret_cast<const char*>(row + (long long)part * WARP_VALUES) - off;
+    const long long left = (long long)(V - part * WARP_VALUES) * (int)sizeof(T) + off;          // bytes up to the row's end
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i) load_logits<T>(x + i * N, src, piece_at<T>(part, i, lane), V, off);
-    float top = -INFINITY;
+    for (int i = 0; i < R::PIECES; ++i) {
+        const int at = (i * 32 + lane) * 16, n = (int)min(16ll, left - at);
+        if (n > 0) cp_async16(&ring.piece[stage][i * 32 + lane], src + at, n);
+    }
+    if (lane == 0 && off != 0 && left > R::PIECES * 512) cp_async16(&ring.piece[stage][R::PIECES * 32], src + R::PIECES * 512, (int)min(16ll, left - R::PIECES * 512));
+}
+template <typename T>
+__device__ __forceinline__ void ring_read(float (&x)[LANE_VALUES], const Ring<T>& ring, int stage, const T* row, int part, int V, int lane) {
+    using R = Ring<T>;
+    const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
 #pragma unroll
-    for (int i = 0; i < LANE_VALUES; ++i) top = fmaxf(top, x[i]);            // (a NaN is passed over)
-    tops[((long long)row * parts + part) * 32 + lane] = top;
+    for (int i = 0; i < R::PIECES; ++i) {
+        uint32_t u[8];
+        const uint4 w = ring.piece[stage][i * 32 + lane];
+        u[0] = w.x, u[1] = w.y, u[2] = w.z, u[3] = w.w;
+        if (off != 0) {
+            const uint4 z = ring.piece[stage][i * 32 + lane + 1];
+            u[4] = z.x, u[5] = z.y, u[6] = z.z, u[7] = z.w;
+            if (off & 8) {
+#pragma unroll
+                for (int c = 0; c < 6; ++c) u[c] = u[c + 2];
+            }
+            if (off & 4) {
+#pragma unroll
+                for (int c = 0; c < 5; ++c) u[c] = u[c + 1];
+            }
+            if (sizeof(T) == 2 && (off & 2)) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) u[c] = __funnelshift_r(u[c], u[c + 1], 16);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            if constexpr (sizeof(T) == 4) {
+                x[i * R::N + c] = __uint_as_float(u[c]);
+            } else {
+                x[i * R::N + 2 * c] = __uint_as_float(u[c] << 16), x[i * R::N + 2 * c + 1] = __uint_as_float(u[c] & 0xffff0000u);
+            }
+        }
+    }
+    if ((part + 1) * WARP_VALUES > V) {           // a row's last part: what lies behind its last logit is none
+#pragma unroll
+        for (int k = 0; k < LANE_VALUES; ++k)
+            if (piece_at<T>(part, k / R::N, lane) + k % R::N >= V) x[k] = -INFINITY;
+    }
+}
+
+// A part's maxima and sum.
+template <typename T>
+__device__ __forceinline__ void part_sum(const float (&x)[LANE_VALUES], float* top_to, RowPart* sum_to, const T* row, int part, int V, int lane) {
+    float top = -INFINITY, other = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < LANE_VALUES; k += 4)                                  // (a NaN is passed over)
+        top = fmaxf(fmaxf(top, x[k]), x[k + 1]), other = fmaxf(fmaxf(other, x[k + 2]), x[k + 3]);
+    top = fmaxf(top, other);
+    top_to[lane] = top;
     const float best = warp_max(top);
     double sum = 0.0;
     int power = LARGE;
     if (fabsf(best) < FAST_LIMIT) {
-        const int n0 = (int)rintf(best * LOG2E);
-        const float least = (float)(n0 - 125) * 0.6931472f;                   // what is smaller adds 2^-125 instead: nothing
-        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        power = (int)rintf(best * LOG2E);
+        const ExpTo e(power);
+        uint64_t s0 = 0ull, s1 = 0ull;
 #pragma unroll
-        for (int i = 0; i < LANE_VALUES; i += 4) {
-            s0 += exp_to(fmaxf(x[i], least), n0), s1 += exp_to(fmaxf(x[i + 1], least), n0);
-            s2 += exp_to(fmaxf(x[i + 2], least), n0), s3 += exp_to(fmaxf(x[i + 3], least), n0);
-        }
-        power = n0, sum = warp_sum_d((double)(s0 + s1) + (double)(s2 + s3));
+        for (int k = 0; k < LANE_VALUES; k += 4) s0 = add2(s0, e(x[k], x[k + 1])), s1 = add2(s1, e(x[k + 2], x[k + 3]));
+        sum = warp_sum_d(((double)low_of(s0) + (double)high_of(s0)) + ((double)low_of(s1) + (double)high_of(s1)));
     } else {
         if (best > -INFINITY && best < INFINITY) {
-            for (int i = 0; i < PIECES; ++i) {            // (read again: an index known only here would move the 64 out of registers)
+            for (int i = 0; i < Ring<T>::PIECES; ++i) {   // (read again: an index known only here would move the 64 out of registers)
                 const int at = piece_at<T>(part, i, lane);
-                for (int c = at; c < min(at + N, V); ++c) {
-                    const float v = to_float(src[c]);
+                for (int c = at; c < min(at + Ring<T>::N, V); ++c) {
+                    const float v = to_float(row[c]);
                     if (v > -INFINITY) sum += exp((double)v - (double)best);
                 }
             }
         }
         sum = warp_sum_d(sum);
     }
-    if (lane == 0) sums[(long long)row * parts + part] = RowPart{best, power, sum};
+    if (lane == 0) *sum_to = RowPart{best, power, sum};
 }
 
-constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024;
+// tops [rows][parts * 32], sums [rows][parts]. The warps of a grid that fills the SMs take parts in turn, the next ones on their way
+// through a ring of the warp's own while it works on one.
+template <typename T>
+__global__ void __launch_bounds__(ROW_WARPS * 32)
+beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, int all,
+                 const uint8_t* __restrict__ done) {
+    using R = Ring<T>;
+    extern __shared__ __align__(16) uint8_t ring_smem[];
+    Ring<T>& ring = reinterpret_cast<Ring<T>*>(ring_smem)[threadIdx.x >> 5];
+    pdl_wait();
+    pdl_trigger();
+    const int lane = threadIdx.x & 31, stride = gridDim.x * ROW_WARPS;
+    auto row_of = [&](int i) { return logits + (long long)(i / parts) * ld; };
+    // part i into a stage, if there is one and its row is looked at
+    auto fetch = [&](int i, int stage) {
+        if (i < all && !(done != nullptr && done[i / parts])) ring_load<T>(ring, stage, row_of(i), i % parts, V, lane);
+        cp_async_commit();
+    };
+    int i = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+#pragma unroll
+    for (int s = 0; s < R::STAGES; ++s) fetch(i + s * stride, s);
+    for (int stage = 0; i < all; i += stride, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+        cp_async_wait<R::STAGES - 1>();
+        __syncwarp();
+        const bool over = done != nullptr && done[i / parts];
+        float x[LANE_VALUES];
+        if (!over) ring_read<T>(x, ring, stage, row_of(i), i % parts, V, lane);
+        __syncwarp();
+        fetch(i + R::STAGES * stride, stage);
+        if (!over) part_sum<T>(x, tops + (long long)i * 32, sums + i, row_of(i), i % parts, V, lane);
+    }
+}
+
+constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, HOT_ROOM = 4096;
 
 struct Found {
     double score[PICK_ROOM];
@@ -189,19 +261,20 @@ __global__ void __launch_bounds__(PICK_THREADS)
 beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens, const float* __restrict__ tops,
                  const RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, const float* __restrict__ scores,
                  const uint8_t* __restrict__ done, int beams, int keep, int pad) {
-    constexpr int N = 16 / sizeof(T);
+    constexpr int N = 16 / sizeof(T), WARPS = PICK_THREADS / 32;
     __shared__ Found found;
-    __shared__ double base_s[MAX_BEAMS], best_s[MAX_BEAMS], log_s[MAX_BEAMS], set_top[PICK_SETS];
-    __shared__ double least_s;
+    __shared__ double base_s[MAX_BEAMS], best_s[MAX_BEAMS], log_s[MAX_BEAMS];
+    __shared__ float set_top[PICK_SETS];
+    __shared__ float least_s;
     __shared__ int n_found, n_hot;
-    __shared__ uint32_t hot[PICK_THREADS];
+    __shared__ uint32_t hot[HOT_ROOM];
     const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) n_found = 0, n_hot = 0, least_s = -INFINITY;
     pdl_wait();
     pdl_trigger();
     __syncthreads();
     // ---- the rows' log-sums; a finished beam offers itself alone
-    for (int k = warp; k < beams; k += PICK_THREADS / 32) {
+    for (int k = warp; k < beams; k += WARPS) {
         const int row = r * beams + k;
         const double s = (double)scores[row];
         const bool over = done != nullptr && done[row];
@@ -228,63 +301,77 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         }
     }
     __syncthreads();
-    // ---- a lower bound of the keep-th best score
+    // ---- a lower bound of the keep-th best score, in 32 bits: a lane's best score is known to within 2^-21 of what it is made of, and
+    // that margin is taken off here and added where lanes are held against the bound
     const int groups = parts * 32, all = beams * groups;
     const float* my_tops = tops + (long long)r * all;
-    auto group_score = [&](int i) {
-        const int k = i / groups;
-        const double b = base_s[k];
-        if (b == -INFINITY) return -(double)INFINITY;                         // (its maxima may never have been written)
-        return b + (((double)my_tops[i] - best_s[k]) - log_s[k]);
+    auto each_group = [&](int begin, int end, const auto& see) {      // of lanes begin .. end - 1 of the request's: see(lane, its best score, margin)
+        for (int k = begin / groups; k * groups < end; ++k) {
+            if (base_s[k] == -INFINITY) continue;                     // (its maxima may never have been written)
+            const float base = (float)(base_s[k] - log_s[k]), best = (float)best_s[k];
+            for (int i = max(begin, k * groups) + threadIdx.x; i < min(end, (k + 1) * groups); i += PICK_THREADS) {
+                const float top = my_tops[i], d = top - best;
+                if (top > -INFINITY) see(i, base + d, (fabsf(base) + fabsf(d)) * 4.8e-7f);
+            }
+        }
     };
     {
-        double top = -INFINITY;
-        for (int i = threadIdx.x; i < all; i += PICK_THREADS) top = fmax(top, group_score(i));
+        float top = -INFINITY;
+        each_group(0, all, [&](int, float s, float margin) { top = fmaxf(top, s - margin); });
         constexpr int PER_SET = PICK_THREADS / PICK_SETS;
 #pragma unroll
-        for (int o = PER_SET / 2; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int o = PER_SET / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (threadIdx.x % PER_SET == 0) set_top[threadIdx.x / PER_SET] = top;
         __syncthreads();
-        if (threadIdx.x < PICK_SETS) {
-            const double me = set_top[threadIdx.x];
-            int above = 0;
-            for (int j = 0; j < PICK_SETS; ++j) above += better(set_top[j], j, me, threadIdx.x) ? 1 : 0;
-            if (above == keep - 1) least_s = me;
-        }
+        // a set's rank: its threads count a share of the better ones each
+        const int me = threadIdx.x / PER_SET;
+        int above = 0;
+#pragma unroll 8
+        for (int j = threadIdx.x % PER_SET; j < PICK_SETS; j += PER_SET) above += set_top[j] > top || (set_top[j] == top && j < me) ? 1 : 0;
+#pragma unroll
+        for (int o = PER_SET / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+        if (above == keep - 1 && threadIdx.x % PER_SET == 0) least_s = top;
         __syncthreads();
     }
-    // ---- the logits of the groups that reach it, a run of groups after the other; when the room fills up the best so far stay, and
-    // the worst of them is the new bound
-    double least = least_s;
+    // ---- the logits of the lanes that reach it, HOT_ROOM lanes' tops at a time. A find goes into the room, unless that is full: then the best
+    // so far stay, the worst of them is the new bound, and the run of lanes is gone through again with barriers (rows of few
+    // different values come to that)
+    double least = (double)least_s;
     uint32_t least_at = 0xffffffffu;          // a find must be better than (least, least_at), or equal least where that is the first bound
-    for (int from = 0; from < all; from += PICK_THREADS) {
-        const int g = from + threadIdx.x;
-        const double gs = g < all ? group_score(g) : -INFINITY;
-        if (gs >= least && gs > -INFINITY) hot[atomicAdd(&n_hot, 1)] = (uint32_t)g;
+    auto find = [&](int e) {
+        const int group = (int)hot[e / LANE_VALUES], k = group / groups, gi = group % groups, at = e % LANE_VALUES;
+        const int v = piece_at<T>(gi >> 5, at / N, gi & 31) + at % N;
+        if (v >= V) return;
+        const double s = base_s[k] + (((double)to_float(logits[(long long)(r * beams + k) * ld + v]) - best_s[k]) - log_s[k]);
+        const uint32_t id = (uint32_t)k * (uint32_t)V + (uint32_t)v;
+        if (s > -INFINITY && (s > least || (s == least && id <= least_at))) {
+            const int i = atomicAdd(&n_found, 1);
+            if (i < PICK_ROOM) found.score[i] = s, found.at[i] = id;
+        }
+    };
+    for (int from = 0; from < all; from += HOT_ROOM) {
+        each_group(from, min(all, from + HOT_ROOM), [&](int i, float s, float margin) {
+            if ((double)(s + margin) >= least) hot[atomicAdd(&n_hot, 1)] = (uint32_t)i;
+        });
         __syncthreads();
-        const int n = n_hot;
-        for (int first = 0; first < n * LANE_VALUES; first += PICK_THREADS) {
-            const int e = first + threadIdx.x;
-            if (e < n * LANE_VALUES) {
-                const int group = (int)hot[e / LANE_VALUES], k = group / groups, gi = group % groups, at = e % LANE_VALUES;
-                const T* row = logits + (long long)(r * beams + k) * ld;
-                const int v = piece_at<T>(gi >> 5, at / N, gi & 31) + at % N;
-                if (v < V) {
-                    const double s = base_s[k] + (((double)to_float(row[v]) - best_s[k]) - log_s[k]);
-                    const uint32_t id = (uint32_t)k * (uint32_t)V + (uint32_t)v;
-                    if (s > -INFINITY && (s > least || (s == least && id <= least_at))) {
-                        const int i = atomicAdd(&n_found, 1);
-                        found.score[i] = s, found.at[i] = id;
-                    }
-                }
-            }
+        const int n = n_hot * LANE_VALUES, before = n_found;
+        __syncthreads();
+        for (int e = threadIdx.x; e < n; e += PICK_THREADS) find(e);
+        __syncthreads();
+        if (n_found > PICK_ROOM) {
             __syncthreads();
-            const int have = n_found;
-            __syncthreads();                   // (nobody adds to it before all have read it)
-            if (have > PICK_ROOM - PICK_THREADS) {
-                sort_found(found, have, keep);
-                if (threadIdx.x == 0) n_found = keep;
-                least = found.score[keep - 1], least_at = found.at[keep - 1];
+            if (threadIdx.x == 0) n_found = before;
+            __syncthreads();
+            for (int first = 0; first < n; first += PICK_THREADS) {
+                const int have = n_found;
+                __syncthreads();              // (nobody adds to it before all have read it)
+                if (have > PICK_ROOM - PICK_THREADS) {
+                    sort_found(found, have, keep);
+                    if (threadIdx.x == 0) n_found = keep;
+                    least = found.score[keep - 1], least_at = found.at[keep - 1];
+                    __syncthreads();
+                }
+                if (first + threadIdx.x < n) find(first + threadIdx.x);
                 __syncthreads();
             }
         }
@@ -419,9 +506,13 @@ int launch_pages(void* pool, const int* block_table, int bt_stride, const int* s
 
 template <typename T>
 int launch_select(float* out_scores, int* out_parents, int* out_tokens, float* tops, void* sums, const void* logits, long long ld, int V, int requests,
-                  int beams, int keep, const float* scores, const uint8_t* done, int pad, int parts, cudaStream_t stream) {
-    const dim3 grid((unsigned)((parts + ROW_WARPS - 1) / ROW_WARPS), (unsigned)(requests * beams));
-    CELLM_RUN(beam_rows_kernel<T>, grid, ROW_WARPS * 32, 0, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, done);
+                  int beams, int keep, const float* scores, const uint8_t* done, int pad, int parts, int sms, cudaStream_t stream) {
+    const int all = requests * beams * parts;
+    const unsigned blocks = (unsigned)std::min<long long>((all + ROW_WARPS - 1) / ROW_WARPS, (long long)Ring<T>::BLOCKS * sms);
+    const size_t smem = ROW_WARPS * sizeof(Ring<T>);
+    cudaError_t e = cudaFuncSetAttribute(beam_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return (int)e;
+    CELLM_RUN(beam_rows_kernel<T>, blocks, ROW_WARPS * 32, smem, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, all, done);
     CELLM_RUN(beam_pick_kernel<T>, requests, PICK_THREADS, 0, stream, out_scores, out_parents, out_tokens, tops, (const RowPart*)sums, (const T*)logits, ld, V,
               parts, scores, done, beams, keep, pad);
     return CELLM_OK;
@@ -436,16 +527,16 @@ CELLM_API int cellm_beam_parts(int V) { return (V + WARP_VALUES - 1) / WARP_VALU
 // scores: out_* [requests][keep], -1 and -inf where there are fewer. done: null, or a byte a row: such a beam offers (itself, pad) at
 // its score and its logits are not read.
 CELLM_API int cellm_beam_select(float* out_scores, int* out_parents, int* out_tokens, float* tops, void* sums, const void* logits, long long ld, int V,
-                                int requests, int beams, int keep, const float* scores, const uint8_t* done, int pad, int dtype, cudaStream_t stream) {
+                                int requests, int beams, int keep, const float* scores, const uint8_t* done, int pad, int dtype, int sms, cudaStream_t stream) {
     if (requests <= 0) return CELLM_OK;
     if (dtype != CELLM_F32 && dtype != CELLM_BF16) return CELLM_ERR_DTYPE;
-    if (V <= 0 || beams <= 0 || beams > MAX_BEAMS || keep <= 0 || keep > MAX_KEEP || ld < V || pad < 0 || pad >= V) return CELLM_ERR_SIZE;
-    if ((long long)beams * (V + WARP_VALUES) > 0x7fffffffLL || (long long)requests * beams > 65535) return CELLM_ERR_SIZE;
+    if (V <= 0 || beams <= 0 || beams > MAX_BEAMS || keep <= 0 || keep > MAX_KEEP || ld < V || pad < 0 || pad >= V || sms <= 0) return CELLM_ERR_SIZE;
+    if ((long long)beams * (V + WARP_VALUES) > 0x7fffffffLL || (long long)requests * beams * cellm_beam_parts(V) > 0x3fffffffLL) return CELLM_ERR_SIZE;
     if (!out_scores || !out_parents || !out_tokens || !tops || !sums || !logits || !scores) return CELLM_ERR_ARG;
     if ((((uintptr_t)sums) & 15) || (((uintptr_t)logits) & (dtype == CELLM_F32 ? 3 : 1))) return CELLM_ERR_ALIGN;
     const int parts = cellm_beam_parts(V);
-    return dtype == CELLM_F32 ? launch_select<float>(out_scores, out_parents, out_tokens, tops, sums, logits, ld, V, requests, beams, keep, scores, done, pad, parts, stream)
-                              : launch_select<__nv_bfloat16>(out_scores, out_parents, out_tokens, tops, sums, logits, ld, V, requests, beams, keep, scores, done, pad, parts, stream);
+    return dtype == CELLM_F32 ? launch_select<float>(out_scores, out_parents, out_tokens, tops, sums, logits, ld, V, requests, beams, keep, scores, done, pad, parts, sms, stream)
+                              : launch_select<__nv_bfloat16>(out_scores, out_parents, out_tokens, tops, sums, logits, ld, V, requests, beams, keep, scores, done, pad, parts, sms, stream);
 }
 
 // state [items][slots][bytes], in place: the slot of beam k of request r takes what the slot of beam parents[r][k] held.
@@ -481,7 +572,7 @@ CELLM_API int cellm_reorder_pages(void* pool, const int* block_table, int bt_str
 // The same with its arguments in order as 64-bit words (see common.cuh).
 CELLM_API int cellm_beam_select_packed(const long long* a, cudaStream_t stream) {
     return cellm_beam_select((float*)a[0], (int*)a[1], (int*)a[2], (float*)a[3], (void*)a[4], (const void*)a[5], (long long)a[6], (int)a[7],
-        (int)a[8], (int)a[9], (int)a[10], (const float*)a[11], (const uint8_t*)a[12], (int)a[13], (int)a[14], stream);
+        (int)a[8], (int)a[9], (int)a[10], (const float*)a[11], (const uint8_t*)a[12], (int)a[13], (int)a[14], (int)a[15], stream);
 }
 
 // The same with its arguments in order as 64-bit words (see common.cuh).

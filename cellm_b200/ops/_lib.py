@@ -124,7 +124,7 @@ _SIGNATURES = {
     "candidates": {
         "cellm_accept_drafts": [P, P, P, P, P, P, P, I, I, I, P, L, L, I, P, P, L, L, I, P, P, P, I, I, I, I, I, P, P],
         "cellm_beam_parts": [I],
-        "cellm_beam_select": [P, P, P, P, P, P, L, I, I, I, I, P, P, I, I, P],
+        "cellm_beam_select": [P, P, P, P, P, P, L, I, I, I, I, P, P, I, I, I, P],
         "cellm_reorder_states": [P, P, P, I, I, I, I, L, P, P],
         "cellm_reorder_pages": [P, P, I, P, P, P, I, I, I, I, I, I, I, P, P],
     },

@@ -7,9 +7,10 @@ from typing import Optional
 import torch
 
 from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
+from ._state import _SM_COUNT, sm_count
 
 MAX_BEAMS, MAX_KEEP = 32, 64       # (as in beams.cu)
-_SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("15q").pack, Struct("9q").pack, Struct("14q").pack
+_SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("16q").pack, Struct("9q").pack, Struct("14q").pack
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Optional[torch.Tensor] = None, pad: int = 0):
@@ -41,7 +42,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Opt
         at = ws.data_ptr()
         launch_packed("candidates", "beam_select", index,
                       _SELECT_ARGS(best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at + 16 * rows * parts, at, logits.data_ptr(), stride[0] if rows > 1 else V, V,
-                                   R, K, keep, scores.data_ptr(), 0 if done is None else done.data_ptr(), pad, DTYPE_TAG[logits.dtype]), 2)
+                                   R, K, keep, scores.data_ptr(), 0 if done is None else done.data_ptr(), pad, DTYPE_TAG[logits.dtype],
+                                   _SM_COUNT.get(index) or sm_count(index)), 2)
     return best, parents, tokens
 
 

@@ -42,9 +42,9 @@ def test_acceptance():
 
 def test_selection_and_reordering():
     def select(out=A, logits=A, ld=100, V=100, R=2, K=3, keep=4, scores=A, pad=0, dtype=0, sums=A):
-        return call("candidates", "cellm_beam_select", out, A, A, A, sums, logits, ld, V, R, K, keep, scores, None, pad, dtype, None)
+        return call("candidates", "cellm_beam_select", out, A, A, A, sums, logits, ld, V, R, K, keep, scores, None, pad, dtype, 148, None)
     assert select(dtype=2) == DTYPE
-    for bad in (dict(V=0), dict(K=0), dict(K=33), dict(keep=0), dict(keep=65), dict(ld=99), dict(pad=100), dict(pad=-1), dict(R=40000), dict(V=2 ** 30, ld=2 ** 30)):
+    for bad in (dict(V=0), dict(K=0), dict(K=33), dict(keep=0), dict(keep=65), dict(ld=99), dict(pad=100), dict(pad=-1), dict(R=2 ** 29), dict(V=2 ** 30, ld=2 ** 30)):
         assert select(**bad) == SIZE, bad
     assert select(out=None) == ARG and select(scores=None) == ARG and select(sums=A + 8) == ALIGN and select(logits=A + 2) == ALIGN and select(R=0) == 0
 
