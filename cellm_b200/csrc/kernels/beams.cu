@@ -20,21 +20,16 @@
 namespace {
 
 constexpr int LANE_VALUES = 64;                       // logits of a row a lane holds
-constexpr int WARP_VALUES = 32 * LANE_VALUES;
+constexpr int WARP_VALUES = 32 * LANE_VALUES;          // a warp's part of a row, worked on in halves
+constexpr int HALF_VALUES = LANE_VALUES / 2;
 constexpr int ROW_WARPS = 4;
 constexpr int MAX_BEAMS = 32, MAX_KEEP = 64;
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr float LOG2E_REST = (float)(1.4426950408889634074 - (double)1.4426950408889634f);
-constexpr float ROUND_MAGIC = 12582912.f;             // 1.5 * 2^23: adding it rounds to a whole number, held in the low bits
-constexpr float FAST_LIMIT = 2.9e6f;                  // behind it x log2(e) leaves the range of that
 
-// Of one warp's logits: the largest, and the sum of their exponentials over 2^power, or over exp(best) where power is LARGE.
+// Of one half part's logits: the largest, and the sum of exp(x - best).
 struct RowPart {
     float best;
-    int power;
     double sum;
 };
-constexpr int LARGE = 1 << 30;
 
 // Two floats in a 64-bit register, worked on by one instruction.
 __device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
@@ -55,31 +50,24 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-// 2^(x log2 e - n0) of two numbers, n0 a whole number near the largest x log2 e. x log2 e = n + f with |f| <= 1/2 comes out of one
-// rounding (n - n0, in the low bits of r) and two multiply-adds with log2 e as a float and its remainder; 2^f = 1 + f P(f), P
-// fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9.
-struct ExpTo {
-    uint64_t shifted;                         // ROUND_MAGIC - n0: adding it rounds and takes n0 off
-    float least;                              // what is smaller adds 2^-125 instead: nothing
-    __device__ __forceinline__ explicit ExpTo(int n0) {
-        const float s = ROUND_MAGIC - (float)n0;
-        shifted = pair_of(s, s), least = (float)(n0 - 125) * 0.6931472f;
-    }
-    __device__ __forceinline__ uint64_t operator()(float a, float b) const {
-        const uint64_t x = pair_of(fmaxf(a, least), fmaxf(b, least)), l2e = pair_of(LOG2E, LOG2E);
-        const uint64_t r = fma2(x, l2e, shifted), minus_n = fma2(r, pair_of(-1.f, -1.f), shifted);
-        const uint64_t f = fma2(x, pair_of(LOG2E_REST, LOG2E_REST), fma2(x, l2e, minus_n));
-        uint64_t p = pair_of(0.00015353357593994588f, 0.00015353357593994588f);
-        p = fma2(p, f, pair_of(0.0013398876180872321f, 0.0013398876180872321f));
-        p = fma2(p, f, pair_of(0.009618437848985195f, 0.009618437848985195f));
-        p = fma2(p, f, pair_of(0.055503323674201965f, 0.055503323674201965f));
-        p = fma2(p, f, pair_of(0.24022647738456726f, 0.24022647738456726f));
-        p = fma2(p, f, pair_of(0.6931471824645996f, 0.6931471824645996f));
-        p = fma2(p, f, pair_of(1.0f, 1.0f));
-        return pair_of(__uint_as_float(__float_as_uint(low_of(p)) + (__float_as_uint(low_of(r)) << 23)),
-                       __uint_as_float(__float_as_uint(high_of(p)) + (__float_as_uint(high_of(r)) << 23)));
-    }
-};
+// exp(x - best) of two numbers, best the largest. d log2 e = n + f with |f| <= 1/2 comes out of the rounding of one addition and a
+// multiply-add; 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9. What matters lies
+// near the best, where d is exact. What is smaller than exp(-86), or not a number, adds exp(-86): nothing.
+__device__ __forceinline__ uint64_t exp_below(float a, float b, uint64_t minus_best) {
+    const uint64_t raw = add2(pair_of(a, b), minus_best), l2e = pair_of(1.4426950408889634f, 1.4426950408889634f);
+    const uint64_t d = pair_of(fmaxf(low_of(raw), -86.f), fmaxf(high_of(raw), -86.f));
+    const uint64_t magic = pair_of(12582912.f, 12582912.f);                  // 1.5 * 2^23: its sum holds a whole number in the low bits
+    const uint64_t r = fma2(d, l2e, magic), f = fma2(d, l2e, fma2(r, pair_of(-1.f, -1.f), magic));
+    uint64_t p = pair_of(0.00015353357593994588f, 0.00015353357593994588f);
+    p = fma2(p, f, pair_of(0.0013398876180872321f, 0.0013398876180872321f));
+    p = fma2(p, f, pair_of(0.009618437848985195f, 0.009618437848985195f));
+    p = fma2(p, f, pair_of(0.055503323674201965f, 0.055503323674201965f));
+    p = fma2(p, f, pair_of(0.24022647738456726f, 0.24022647738456726f));
+    p = fma2(p, f, pair_of(0.6931471824645996f, 0.6931471824645996f));
+    p = fma2(p, f, pair_of(1.0f, 1.0f));
+    return pair_of(__uint_as_float(__float_as_uint(low_of(p)) + (__float_as_uint(low_of(r)) << 23)),
+                   __uint_as_float(__float_as_uint(high_of(p)) + (__float_as_uint(high_of(r)) << 23)));
+}
 
 __device__ __forceinline__ double warp_sum_d(double v) {
 #pragma unroll
@@ -87,37 +75,41 @@ __device__ __forceinline__ double warp_sum_d(double v) {
     return v;
 }
 
-// The first logit of piece i of lane `lane` of warp part `part` of a row.
+// The first logit of piece i of a lane from logit `from` of a row on.
 template <typename T>
-__device__ __forceinline__ int piece_at(int part, int i, int lane) {
-    return part * WARP_VALUES + (i * 32 + lane) * (16 / (int)sizeof(T));
+__device__ __forceinline__ int piece_at(int from, int i, int lane) {
+    return from + (i * 32 + lane) * (16 / (int)sizeof(T));
 }
 
-// A warp's ring of parts in shared memory: the aligned 16-byte pieces that a part lies in.
+// A warp's ring of half parts in shared memory: the aligned 16-byte pieces that they lie in.
 template <typename T>
 struct Ring {
-    static constexpr int N = 16 / sizeof(T), PIECES = LANE_VALUES / N, STAGES = sizeof(T) == 4 ? 2 : 3;
-    static constexpr int BLOCKS = sizeof(T) == 4 ? 3 : 4;                 // of ROW_WARPS warps that an SM holds, by this memory
+    static constexpr int N = 16 / sizeof(T), PIECES = HALF_VALUES / N, STAGES = sizeof(T) == 4 ? 2 : 3;
+    static constexpr int BLOCKS = 6;                                      // of ROW_WARPS warps that an SM holds
     uint4 piece[STAGES][PIECES * 32 + 1];
 };
 
 // Which logits a lane takes goes by their places in the row alone, so that equal rows have equal sums wherever they lie: of a row that
 // starts `off` bytes behind a 16-byte border a lane joins its own piece and the next.
 template <typename T>
-__device__ __forceinline__ void ring_load(Ring<T>& ring, int stage, const T* row, int part, int V, int lane) {
+__device__ __forceinline__ void ring_load(Ring<T>& ring, int stage, const T* row, int from, int V, int lane) {
     using R = Ring<T>;
     const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
-    const char* src = reinterpret_cast<const char*>(row + (long long)part * WARP_VALUES) - off;
-    const long long left = (long long)(V - part * WARP_VALUES) * (int)sizeof(T) + off;          // bytes up to the row's end
+    const char* src = reinterpret_cast<const char*>(row + from) - off + lane * 16;
+    uint4* dst = &ring.piece[stage][lane];
+    if (from + HALF_VALUES * 32 + R::N <= V) {
 #pragma unroll
-    for (int i = 0; i < R::PIECES; ++i) {
-        const int at = (i * 32 + lane) * 16, n = (int)min(16ll, left - at);
-        if (n > 0) cp_async16(&ring.piece[stage][i * 32 + lane], src + at, n);
+        for (int i = 0; i < R::PIECES; ++i) cp_async16(dst + i * 32, src + i * 512, 16);
+        if (lane == 0) cp_async16(dst + R::PIECES * 32, src + R::PIECES * 512, 16);
+    } else {
+        const long long left = (long long)(V - from) * (int)sizeof(T) + off - lane * 16;       // bytes up to the row's end
+#pragma unroll
+        for (int i = 0; i <= R::PIECES; ++i)
+            if (left > i * 512 && (i < R::PIECES || lane == 0)) cp_async16(dst + i * 32, src + i * 512, (int)min(16ll, left - i * 512));
     }
-    if (lane == 0 && off != 0 && left > R::PIECES * 512) cp_async16(&ring.piece[stage][R::PIECES * 32], src + R::PIECES * 512, (int)min(16ll, left - R::PIECES * 512));
 }
 template <typename T>
-__device__ __forceinline__ void ring_read(float (&x)[LANE_VALUES], const Ring<T>& ring, int stage, const T* row, int part, int V, int lane) {
+__device__ __forceinline__ void ring_read(float (&x)[HALF_VALUES], const Ring<T>& ring, int stage, const T* row, int from, int V, int lane) {
     using R = Ring<T>;
     const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
 #pragma unroll
@@ -150,81 +142,78 @@ __device__ __forceinline__ void ring_read(float (&x)[LANE_VALUES], const Ring<T>
             }
         }
     }
-    if ((part + 1) * WARP_VALUES > V) {           // a row's last part: what lies behind its last logit is none
+    if (from + WARP_VALUES / 2 > V) {             // a row's last logits: what lies behind them is none
 #pragma unroll
-        for (int k = 0; k < LANE_VALUES; ++k)
-            if (piece_at<T>(part, k / R::N, lane) + k % R::N >= V) x[k] = -INFINITY;
+        for (int k = 0; k < HALF_VALUES; ++k)
+            if (piece_at<T>(from, k / R::N, lane) + k % R::N >= V) x[k] = -INFINITY;
     }
 }
 
-// A part's maxima and sum.
+// tops [rows][parts * 32], sums [rows][parts * 2]. The warps of a grid that fills the SMs take parts in turn, the next halves on their
+// way through a ring of the warp's own while it works on one.
 template <typename T>
-__device__ __forceinline__ void part_sum(const float (&x)[LANE_VALUES], float* top_to, RowPart* sum_to, const T* row, int part, int V, int lane) {
-    float top = -INFINITY, other = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < LANE_VALUES; k += 4)                                  // (a NaN is passed over)
-        top = fmaxf(fmaxf(top, x[k]), x[k + 1]), other = fmaxf(fmaxf(other, x[k + 2]), x[k + 3]);
-    top = fmaxf(top, other);
-    top_to[lane] = top;
-    const float best = warp_max(top);
-    double sum = 0.0;
-    int power = LARGE;
-    if (fabsf(best) < FAST_LIMIT) {
-        power = (int)rintf(best * LOG2E);
-        const ExpTo e(power);
-        uint64_t s0 = 0ull, s1 = 0ull;
-#pragma unroll
-        for (int k = 0; k < LANE_VALUES; k += 4) s0 = add2(s0, e(x[k], x[k + 1])), s1 = add2(s1, e(x[k + 2], x[k + 3]));
-        sum = warp_sum_d(((double)low_of(s0) + (double)high_of(s0)) + ((double)low_of(s1) + (double)high_of(s1)));
-    } else {
-        if (best > -INFINITY && best < INFINITY) {
-            for (int i = 0; i < Ring<T>::PIECES; ++i) {   // (read again: an index known only here would move the 64 out of registers)
-                const int at = piece_at<T>(part, i, lane);
-                for (int c = at; c < min(at + Ring<T>::N, V); ++c) {
-                    const float v = to_float(row[c]);
-                    if (v > -INFINITY) sum += exp((double)v - (double)best);
-                }
-            }
-        }
-        sum = warp_sum_d(sum);
-    }
-    if (lane == 0) *sum_to = RowPart{best, power, sum};
-}
-
-// tops [rows][parts * 32], sums [rows][parts]. The warps of a grid that fills the SMs take parts in turn, the next ones on their way
-// through a ring of the warp's own while it works on one.
-template <typename T>
-__global__ void __launch_bounds__(ROW_WARPS * 32)
-beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, int all,
+__global__ void __launch_bounds__(ROW_WARPS * 32, Ring<T>::BLOCKS)
+beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, int rows,
                  const uint8_t* __restrict__ done) {
     using R = Ring<T>;
     extern __shared__ __align__(16) uint8_t ring_smem[];
     Ring<T>& ring = reinterpret_cast<Ring<T>*>(ring_smem)[threadIdx.x >> 5];
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, stride = gridDim.x * ROW_WARPS;
-    auto row_of = [&](int i) { return logits + (long long)(i / parts) * ld; };
-    // part i into a stage, if there is one and its row is looked at
-    auto fetch = [&](int i, int stage) {
-        if (i < all && !(done != nullptr && done[i / parts])) ring_load<T>(ring, stage, row_of(i), i % parts, V, lane);
-        cp_async_commit();
+    const int lane = threadIdx.x & 31, stride = gridDim.x * ROW_WARPS, first = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    const int row_step = stride / parts, part_step = stride % parts;
+    // a place among the warp's halves: one runs ahead to load, one works
+    struct At {
+        int row, part, half;
     };
-    int i = blockIdx.x * ROW_WARPS + (threadIdx.x >> 5);
+    auto advance = [&](At& at) {
+        if ((at.half ^= 1) != 0) return;
+        at.row += row_step, at.part += part_step;
+        if (at.part >= parts) at.part -= parts, ++at.row;
+    };
+    auto looked_at = [&](const At& at) { return at.row < rows && !(done != nullptr && done[at.row]); };
+    At load = {first / parts, first % parts, 0}, at = load;
+    auto fetch = [&](int stage) {
+        if (looked_at(load)) ring_load<T>(ring, stage, logits + load.row * ld, load.part * WARP_VALUES + load.half * (WARP_VALUES / 2), V, lane);
+        cp_async_commit();
+        advance(load);
+    };
 #pragma unroll
-    for (int s = 0; s < R::STAGES; ++s) fetch(i + s * stride, s);
-    for (int stage = 0; i < all; i += stride, stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+    for (int s = 0; s < R::STAGES; ++s) fetch(s);
+    float top = -INFINITY;
+    for (int stage = 0; at.row < rows; advance(at), stage = stage + 1 == R::STAGES ? 0 : stage + 1) {
+        const int from = at.part * WARP_VALUES + at.half * (WARP_VALUES / 2);
+        const bool wanted = looked_at(at);
         cp_async_wait<R::STAGES - 1>();
         __syncwarp();
-        const bool over = done != nullptr && done[i / parts];
-        float x[LANE_VALUES];
-        if (!over) ring_read<T>(x, ring, stage, row_of(i), i % parts, V, lane);
+        float x[HALF_VALUES];
+        if (wanted) ring_read<T>(x, ring, stage, logits + at.row * ld, from, V, lane);
         __syncwarp();
-        fetch(i + R::STAGES * stride, stage);
-        if (!over) part_sum<T>(x, tops + (long long)i * 32, sums + i, row_of(i), i % parts, V, lane);
+        fetch(stage);
+        if (!wanted) continue;
+        float mine = -INFINITY, other = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < HALF_VALUES; k += 4)                              // (a NaN is passed over)
+            mine = fmaxf(fmaxf(mine, x[k]), x[k + 1]), other = fmaxf(fmaxf(other, x[k + 2]), x[k + 3]);
+        mine = fmaxf(mine, other);
+        top = at.half ? fmaxf(top, mine) : mine;
+        const float best = warp_max(mine);
+        double sum = 0.0;
+        if (fabsf(best) < INFINITY) {                                         // (no logit at all, or one that has no meaning: no sum)
+            const uint64_t minus_best = pair_of(-best, -best);
+            uint64_t s0 = 0ull, s1 = 0ull;
+#pragma unroll
+            for (int k = 0; k < HALF_VALUES; k += 4) s0 = add2(s0, exp_below(x[k], x[k + 1], minus_best)), s1 = add2(s1, exp_below(x[k + 2], x[k + 3], minus_best));
+            s0 = add2(s0, s1);
+            sum = warp_sum_d((double)(low_of(s0) + high_of(s0)));
+        }
+        const long long part = (long long)at.row * parts + at.part;
+        if (lane == 0) sums[2 * part + at.half] = RowPart{best, sum};
+        if (at.half) tops[part * 32 + lane] = top;
     }
 }
 
-constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, HOT_ROOM = 4096;
+constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, HELD = 16, HOT_ROOM = HELD * PICK_THREADS;
 
 struct Found {
     double score[PICK_ROOM];
@@ -265,9 +254,9 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     __shared__ Found found;
     __shared__ double base_s[MAX_BEAMS], best_s[MAX_BEAMS], log_s[MAX_BEAMS];
     __shared__ float set_top[PICK_SETS];
-    __shared__ float least_s;
+    __shared__ float least_s, size_s;
     __shared__ int n_found, n_hot;
-    __shared__ uint32_t hot[HOT_ROOM];
+    extern __shared__ uint32_t hot[];          // [HOT_ROOM]
     const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) n_found = 0, n_hot = 0, least_s = -INFINITY;
     pdl_wait();
@@ -278,22 +267,23 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         const int row = r * beams + k;
         const double s = (double)scores[row];
         const bool over = done != nullptr && done[row];
-        double best = -INFINITY, sum = 0.0;
+        float best = -INFINITY;
+        double log_sum = 0.0, sum = 0.0;
         if (!over) {
-            const RowPart* p = sums + (long long)row * parts;
-            for (int i = lane; i < parts; i += 32) best = fmax(best, (double)p[i].best);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) best = fmax(best, __shfl_xor_sync(0xffffffffu, best, o));
-            for (int i = lane; i < parts; i += 32) {
+            const RowPart* p = sums + 2ll * row * parts;
+            for (int i = lane; i < 2 * parts; i += 32) best = fmaxf(best, p[i].best);
+            best = warp_max(best);
+            for (int i = lane; i < 2 * parts; i += 32) {
                 const RowPart w = p[i];
-                if (w.sum > 0.0) sum += w.sum * (w.power == LARGE ? exp((double)w.best - best) : exp2((double)w.power - best * 1.4426950408889634074));
+                if (w.sum > 0.0) sum += w.sum * exp((double)w.best - (double)best);
             }
             sum = warp_sum_d(sum);
+            log_sum = log(sum);
         }
         if (lane == 0) {
             // nothing of a beam with no score, or of a row without a finite logit, is offered
             base_s[k] = over || !(s > -INFINITY) || !(sum > 0.0) ? -INFINITY : s;
-            best_s[k] = best, log_s[k] = log(sum);
+            best_s[k] = (double)best, log_s[k] = log_sum;
             if (over && s > -INFINITY) {
                 const int i = atomicAdd(&n_found, 1);
                 found.score[i] = s, found.at[i] = (uint32_t)k * (uint32_t)V + (uint32_t)pad;
@@ -305,19 +295,38 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     // that margin is taken off here and added where lanes are held against the bound
     const int groups = parts * 32, all = beams * groups;
     const float* my_tops = tops + (long long)r * all;
-    auto each_group = [&](int begin, int end, const auto& see) {      // of lanes begin .. end - 1 of the request's: see(lane, its best score, margin)
-        for (int k = begin / groups; k * groups < end; ++k) {
-            if (base_s[k] == -INFINITY) continue;                     // (its maxima may never have been written)
-            const float base = (float)(base_s[k] - log_s[k]), best = (float)best_s[k];
-            for (int i = max(begin, k * groups) + threadIdx.x; i < min(end, (k + 1) * groups); i += PICK_THREADS) {
-                const float top = my_tops[i], d = top - best;
-                if (top > -INFINITY) see(i, base + d, (fabsf(base) + fabsf(d)) * 4.8e-7f);
-            }
+    if (threadIdx.x < 32) {
+        float size = 0.f;
+        if (lane < beams && base_s[lane] > -INFINITY) size = fabsf((float)base_s[lane]) + fabsf((float)log_s[lane]);
+        size = warp_max(size);
+        if (lane == 0) size_s = size;
+    }
+    __syncthreads();
+    const float size = 2.f * size_s;
+    auto margin = [&](float s) { return (fabsf(s) + size) * 4.8e-7f; };
+    // the best scores of the lanes from + threadIdx.x, from + threadIdx.x + PICK_THREADS, ... of the request
+    float held[HELD];
+    auto hold = [&](int from) {
+#pragma unroll
+        for (int c = 0; c < HELD; ++c) {
+            const int i = from + threadIdx.x + c * PICK_THREADS, k = i / groups;       // (the same of a warp's lanes)
+            held[c] = -INFINITY;
+            if (i < all && base_s[k] > -INFINITY) held[c] = my_tops[i];       // (else they may never have been written)
+        }
+#pragma unroll
+        for (int c = 0; c < HELD; ++c) {
+            const int k = min((from + (int)threadIdx.x + c * PICK_THREADS) / groups, beams - 1);
+            if (held[c] > -INFINITY) held[c] = (float)(base_s[k] - log_s[k]) + (held[c] - (float)best_s[k]);
         }
     };
     {
         float top = -INFINITY;
-        each_group(0, all, [&](int, float s, float margin) { top = fmaxf(top, s - margin); });
+        for (int from = 0; from < all; from += HOT_ROOM) {
+            hold(from);
+#pragma unroll
+            for (int c = 0; c < HELD; ++c)
+                if (held[c] > -INFINITY) top = fmaxf(top, held[c] - margin(held[c]));
+        }
         constexpr int PER_SET = PICK_THREADS / PICK_SETS;
 #pragma unroll
         for (int o = PER_SET / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -338,25 +347,39 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     // different values come to that)
     double least = (double)least_s;
     uint32_t least_at = 0xffffffffu;          // a find must be better than (least, least_at), or equal least where that is the first bound
-    auto find = [&](int e) {
-        const int group = (int)hot[e / LANE_VALUES], k = group / groups, gi = group % groups, at = e % LANE_VALUES;
-        const int v = piece_at<T>(gi >> 5, at / N, gi & 31) + at % N;
-        if (v >= V) return;
-        const double s = base_s[k] + (((double)to_float(logits[(long long)(r * beams + k) * ld + v]) - best_s[k]) - log_s[k]);
-        const uint32_t id = (uint32_t)k * (uint32_t)V + (uint32_t)v;
+    struct Place {
+        int k, v;
+    };
+    auto place = [&](int e) {                 // e counts the hot lanes' logits
+        const int group = (int)hot[e / LANE_VALUES], gi = group % groups, at = e % LANE_VALUES;
+        return Place{group / groups, piece_at<T>((gi >> 5) * WARP_VALUES, at / N, gi & 31) + at % N};
+    };
+    auto logit = [&](const Place& p) { return p.v < V ? to_float(logits[(long long)(r * beams + p.k) * ld + p.v]) : -INFINITY; };
+    auto find = [&](const Place& p, float x) {
+        const double s = base_s[p.k] + (((double)x - best_s[p.k]) - log_s[p.k]);
+        const uint32_t id = (uint32_t)p.k * (uint32_t)V + (uint32_t)p.v;
         if (s > -INFINITY && (s > least || (s == least && id <= least_at))) {
             const int i = atomicAdd(&n_found, 1);
             if (i < PICK_ROOM) found.score[i] = s, found.at[i] = id;
         }
     };
     for (int from = 0; from < all; from += HOT_ROOM) {
-        each_group(from, min(all, from + HOT_ROOM), [&](int i, float s, float margin) {
-            if ((double)(s + margin) >= least) hot[atomicAdd(&n_hot, 1)] = (uint32_t)i;
-        });
+        if (all > HOT_ROOM) hold(from);
+#pragma unroll
+        for (int c = 0; c < HELD; ++c)
+            if (held[c] > -INFINITY && (double)(held[c] + margin(held[c])) >= least) hot[atomicAdd(&n_hot, 1)] = (uint32_t)(from + threadIdx.x + c * PICK_THREADS);
         __syncthreads();
         const int n = n_hot * LANE_VALUES, before = n_found;
         __syncthreads();
-        for (int e = threadIdx.x; e < n; e += PICK_THREADS) find(e);
+        for (int e = threadIdx.x; e < n; e += 4 * PICK_THREADS) {             // four logits under way at once
+            Place p[4];
+            float x[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[c] = place(min(e + c * PICK_THREADS, n - 1)), x[c] = e + c * PICK_THREADS < n ? logit(p[c]) : -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                if (x[c] > -INFINITY) find(p[c], x[c]);
+        }
         __syncthreads();
         if (n_found > PICK_ROOM) {
             __syncthreads();
@@ -371,7 +394,11 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
                     least = found.score[keep - 1], least_at = found.at[keep - 1];
                     __syncthreads();
                 }
-                if (first + threadIdx.x < n) find(first + threadIdx.x);
+                if (first + threadIdx.x < n) {
+                    const Place p = place(first + threadIdx.x);
+                    const float x = logit(p);
+                    if (x > -INFINITY) find(p, x);
+                }
                 __syncthreads();
             }
         }
@@ -507,20 +534,20 @@ int launch_pages(void* pool, const int* block_table, int bt_stride, const int* s
 template <typename T>
 int launch_select(float* out_scores, int* out_parents, int* out_tokens, float* tops, void* sums, const void* logits, long long ld, int V, int requests,
                   int beams, int keep, const float* scores, const uint8_t* done, int pad, int parts, int sms, cudaStream_t stream) {
-    const int all = requests * beams * parts;
+    const long long all = (long long)requests * beams * parts;
     const unsigned blocks = (unsigned)std::min<long long>((all + ROW_WARPS - 1) / ROW_WARPS, (long long)Ring<T>::BLOCKS * sms);
     const size_t smem = ROW_WARPS * sizeof(Ring<T>);
     cudaError_t e = cudaFuncSetAttribute(beam_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return (int)e;
-    CELLM_RUN(beam_rows_kernel<T>, blocks, ROW_WARPS * 32, smem, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, all, done);
-    CELLM_RUN(beam_pick_kernel<T>, requests, PICK_THREADS, 0, stream, out_scores, out_parents, out_tokens, tops, (const RowPart*)sums, (const T*)logits, ld, V,
+    CELLM_RUN(beam_rows_kernel<T>, blocks, ROW_WARPS * 32, smem, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, requests * beams, done);
+    CELLM_RUN(beam_pick_kernel<T>, requests, PICK_THREADS, HOT_ROOM * sizeof(uint32_t), stream, out_scores, out_parents, out_tokens, tops, (const RowPart*)sums, (const T*)logits, ld, V,
               parts, scores, done, beams, keep, pad);
     return CELLM_OK;
 }
 
 }  // namespace
 
-// Warp parts of a row of V logits: the workspace holds 32 floats (tops) and 16 bytes (sums) for each part of every row.
+// Warp parts of a row of V logits: the workspace holds 32 floats (tops) and 32 bytes (sums of its halves) for each part of every row.
 CELLM_API int cellm_beam_parts(int V) { return (V + WARP_VALUES - 1) / WARP_VALUES; }
 
 // The `keep` best continuations of each request's `beams` rows of logits [requests * beams][V] (rows ld apart) under the beams'

@@ -37,11 +37,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Opt
     tokens = torch.empty_like(parents)
     if R:
         parts = fn("candidates", "cellm_beam_parts")(V)
-        # the rows' sums (16 bytes a part), then their lanes' maxima (32 floats a part)
-        ws = scores.new_empty(rows * parts * 36)
+        # the rows' sums (32 bytes a part), then their lanes' maxima (32 floats a part)
+        ws = scores.new_empty(rows * parts * 40)
         at = ws.data_ptr()
         launch_packed("candidates", "beam_select", index,
-                      _SELECT_ARGS(best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at + 16 * rows * parts, at, logits.data_ptr(), stride[0] if rows > 1 else V, V,
+                      _SELECT_ARGS(best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), at + 32 * rows * parts, at, logits.data_ptr(), stride[0] if rows > 1 else V, V,
                                    R, K, keep, scores.data_ptr(), 0 if done is None else done.data_ptr(), pad, DTYPE_TAG[logits.dtype],
                                    _SM_COUNT.get(index) or sm_count(index)), 2)
     return best, parents, tokens
