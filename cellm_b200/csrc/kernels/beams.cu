@@ -23,7 +23,7 @@ constexpr int LANE_VALUES = 64;                       // logits of a row a lane 
 constexpr int WARP_VALUES = 32 * LANE_VALUES;          // a warp's part of a row, worked on in halves
 constexpr int HALF_VALUES = LANE_VALUES / 2;
 constexpr int ROW_WARPS = 4;
-constexpr int MAX_BEAMS = 32, MAX_KEEP = 64;
+constexpr int MAX_BEAMS = 32, MAX_KEEP = 64, MAX_VOCAB = 1 << 24;
 
 // Of one half part's logits: the largest, and the sum of exp(x - best).
 struct RowPart {
@@ -213,35 +213,52 @@ beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* 
     }
 }
 
+// exp(d) for d <= 0 in 64 bits, to 2.0e-9: as exp_below. The picking block runs its code once, so what it calls is short.
+__device__ __forceinline__ double exp_short(double d) {
+    d = fmax(d, -600.0) * 1.4426950408889634074;
+    const double n = rint(d), f = d - n;
+    double p = 0.00015353357593994588;
+    p = fma(p, f, 0.0013398876180872321);
+    p = fma(p, f, 0.009618437848985195);
+    p = fma(p, f, 0.055503323674201965);
+    p = fma(p, f, 0.24022647738456726);
+    p = fma(p, f, 0.6931471824645996);
+    return fma(p, f, 1.0) * __hiloint2double((1023 + (int)n) << 20, 0);
+}
+// log(s) for s >= 1/2: the 32-bit logarithm and one step of Newton's method
+__device__ __forceinline__ double log_short(double s) {
+    const double y = (double)logf((float)s);
+    return y + (s * exp_short(-y) - 1.0);
+}
+
 constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, HELD = 16, HOT_ROOM = HELD * PICK_THREADS;
 
 struct Found {
     double score[PICK_ROOM];
     uint32_t at[PICK_ROOM];           // k * V + v
 };
+struct Best {
+    double score[MAX_KEEP];
+    uint32_t at[MAX_KEEP];
+};
 __device__ __forceinline__ bool better(double a, uint32_t ai, double b, uint32_t bi) { return a > b || (a == b && ai < bi); }
 
-// The `keep` best of the n found, in order, to the front. All threads; ends with a barrier. A find's rank is the number of better ones.
-__device__ void sort_found(Found& f, int n, int keep) {
-    constexpr int PER = PICK_ROOM / PICK_THREADS;
-    double s[PER];
-    uint32_t at[PER];
-    int rank[PER];
+// The `keep` best of the n found, in order, to the front of `to`. All threads; ends with a barrier. A find's rank is the number of better
+// ones, which eight threads count together.
+__device__ void sort_found(const Found& f, Best& to, int n, int keep) {
+    const int part = threadIdx.x & 7;
     __syncthreads();
+    for (int base = 0; base < n; base += PICK_THREADS / 8) {
+        const int me = min(base + (int)(threadIdx.x >> 3), n - 1);
+        const double s = f.score[me];
+        const uint32_t at = f.at[me];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = part; j < n; j += 8) rank += better(f.score[j], f.at[j], s, at) ? 1 : 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        const int me = threadIdx.x + i * PICK_THREADS;
-        rank[i] = keep;
-        if (me >= n) continue;
-        s[i] = f.score[me], at[i] = f.at[me];
-        int r = 0;
-        for (int j = 0; j < n; ++j) r += better(f.score[j], f.at[j], s[i], at[i]) ? 1 : 0;
-        rank[i] = r;
+        for (int o = 4; o > 0; o >>= 1) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+        if (part == 0 && rank < keep) to.score[rank] = s, to.at[rank] = at;       // (equal places hold equal values)
     }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < PER; ++i)
-        if (rank[i] < keep) f.score[rank[i]] = s[i], f.at[rank[i]] = at[i];
     __syncthreads();
 }
 
@@ -249,9 +266,10 @@ template <typename T>
 __global__ void __launch_bounds__(PICK_THREADS)
 beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens, const float* __restrict__ tops,
                  const RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, const float* __restrict__ scores,
-                 const uint8_t* __restrict__ done, int beams, int keep, int pad) {
+                 const uint8_t* __restrict__ done, int beams, int keep, int pad, unsigned long long per_part) {
     constexpr int N = 16 / sizeof(T), WARPS = PICK_THREADS / 32;
     __shared__ Found found;
+    __shared__ Best kept;
     __shared__ double base_s[MAX_BEAMS], best_s[MAX_BEAMS], log_s[MAX_BEAMS];
     __shared__ float set_top[PICK_SETS];
     __shared__ float least_s, size_s;
@@ -275,10 +293,10 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
             best = warp_max(best);
             for (int i = lane; i < 2 * parts; i += 32) {
                 const RowPart w = p[i];
-                if (w.sum > 0.0) sum += w.sum * exp((double)w.best - (double)best);
+                if (w.sum > 0.0) sum += w.sum * exp_short((double)w.best - (double)best);
             }
             sum = warp_sum_d(sum);
-            log_sum = log(sum);
+            log_sum = log_short(sum);
         }
         if (lane == 0) {
             // nothing of a beam with no score, or of a row without a finite logit, is offered
@@ -294,6 +312,7 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     // ---- a lower bound of the keep-th best score, in 32 bits: a lane's best score is known to within 2^-21 of what it is made of, and
     // that margin is taken off here and added where lanes are held against the bound
     const int groups = parts * 32, all = beams * groups;
+    auto beam_of = [&](int i) { return (int)((((uint32_t)i >> 5) * per_part) >> 32); };  // i / groups: per_part is 2^32 / parts, rounded up
     const float* my_tops = tops + (long long)r * all;
     if (threadIdx.x < 32) {
         float size = 0.f;
@@ -309,13 +328,13 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     auto hold = [&](int from) {
 #pragma unroll
         for (int c = 0; c < HELD; ++c) {
-            const int i = from + threadIdx.x + c * PICK_THREADS, k = i / groups;       // (the same of a warp's lanes)
+            const int i = from + threadIdx.x + c * PICK_THREADS, k = beam_of(i);       // (the same of a warp's lanes)
             held[c] = -INFINITY;
             if (i < all && base_s[k] > -INFINITY) held[c] = my_tops[i];       // (else they may never have been written)
         }
 #pragma unroll
         for (int c = 0; c < HELD; ++c) {
-            const int k = min((from + (int)threadIdx.x + c * PICK_THREADS) / groups, beams - 1);
+            const int k = min(beam_of(from + (int)threadIdx.x + c * PICK_THREADS), beams - 1);
             if (held[c] > -INFINITY) held[c] = (float)(base_s[k] - log_s[k]) + (held[c] - (float)best_s[k]);
         }
     };
@@ -351,8 +370,8 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         int k, v;
     };
     auto place = [&](int e) {                 // e counts the hot lanes' logits
-        const int group = (int)hot[e / LANE_VALUES], gi = group % groups, at = e % LANE_VALUES;
-        return Place{group / groups, piece_at<T>((gi >> 5) * WARP_VALUES, at / N, gi & 31) + at % N};
+        const int group = (int)hot[e / LANE_VALUES], k = beam_of(group), gi = group - k * groups, at = e % LANE_VALUES;
+        return Place{k, piece_at<T>((gi >> 5) * WARP_VALUES, at / N, gi & 31) + at % N};
     };
     auto logit = [&](const Place& p) { return p.v < V ? to_float(logits[(long long)(r * beams + p.k) * ld + p.v]) : -INFINITY; };
     auto find = [&](const Place& p, float x) {
@@ -389,9 +408,10 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
                 const int have = n_found;
                 __syncthreads();              // (nobody adds to it before all have read it)
                 if (have > PICK_ROOM - PICK_THREADS) {
-                    sort_found(found, have, keep);
+                    sort_found(found, kept, have, keep);
                     if (threadIdx.x == 0) n_found = keep;
-                    least = found.score[keep - 1], least_at = found.at[keep - 1];
+                    if (threadIdx.x < keep) found.score[threadIdx.x] = kept.score[threadIdx.x], found.at[threadIdx.x] = kept.at[threadIdx.x];
+                    least = kept.score[keep - 1], least_at = kept.at[keep - 1];
                     __syncthreads();
                 }
                 if (first + threadIdx.x < n) {
@@ -407,12 +427,12 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         __syncthreads();
     }
     const int have = n_found;
-    sort_found(found, have, keep);
+    sort_found(found, kept, have, keep);
     for (int i = threadIdx.x; i < keep; i += PICK_THREADS) {
         const bool fine = i < have;
-        out_scores[r * keep + i] = fine ? (float)found.score[i] : -INFINITY;
-        out_parents[r * keep + i] = fine ? (int)(found.at[i] / (uint32_t)V) : -1;
-        out_tokens[r * keep + i] = fine ? (int)(found.at[i] % (uint32_t)V) : -1;
+        out_scores[r * keep + i] = fine ? (float)kept.score[i] : -INFINITY;
+        out_parents[r * keep + i] = fine ? (int)(kept.at[i] / (uint32_t)V) : -1;
+        out_tokens[r * keep + i] = fine ? (int)(kept.at[i] % (uint32_t)V) : -1;
     }
 }
 
@@ -541,7 +561,7 @@ int launch_select(float* out_scores, int* out_parents, int* out_tokens, float* t
     if (e != cudaSuccess) return (int)e;
     CELLM_RUN(beam_rows_kernel<T>, blocks, ROW_WARPS * 32, smem, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, requests * beams, done);
     CELLM_RUN(beam_pick_kernel<T>, requests, PICK_THREADS, HOT_ROOM * sizeof(uint32_t), stream, out_scores, out_parents, out_tokens, tops, (const RowPart*)sums, (const T*)logits, ld, V,
-              parts, scores, done, beams, keep, pad);
+              parts, scores, done, beams, keep, pad, ((1ull << 32) + parts - 1) / parts);
     return CELLM_OK;
 }
 
@@ -557,7 +577,7 @@ CELLM_API int cellm_beam_select(float* out_scores, int* out_parents, int* out_to
                                 int requests, int beams, int keep, const float* scores, const uint8_t* done, int pad, int dtype, int sms, cudaStream_t stream) {
     if (requests <= 0) return CELLM_OK;
     if (dtype != CELLM_F32 && dtype != CELLM_BF16) return CELLM_ERR_DTYPE;
-    if (V <= 0 || beams <= 0 || beams > MAX_BEAMS || keep <= 0 || keep > MAX_KEEP || ld < V || pad < 0 || pad >= V || sms <= 0) return CELLM_ERR_SIZE;
+    if (V <= 0 || V > MAX_VOCAB || beams <= 0 || beams > MAX_BEAMS || keep <= 0 || keep > MAX_KEEP || ld < V || pad < 0 || pad >= V || sms <= 0) return CELLM_ERR_SIZE;
     if ((long long)beams * (V + WARP_VALUES) > 0x7fffffffLL || (long long)requests * beams * cellm_beam_parts(V) > 0x3fffffffLL) return CELLM_ERR_SIZE;
     if (!out_scores || !out_parents || !out_tokens || !tops || !sums || !logits || !scores) return CELLM_ERR_ARG;
     if ((((uintptr_t)sums) & 15) || (((uintptr_t)logits) & (dtype == CELLM_F32 ? 3 : 1))) return CELLM_ERR_ALIGN;

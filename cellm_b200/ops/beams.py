@@ -9,14 +9,14 @@ import torch
 from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
 from ._state import _SM_COUNT, sm_count
 
-MAX_BEAMS, MAX_KEEP = 32, 64       # (as in beams.cu)
+MAX_BEAMS, MAX_KEEP, MAX_VOCAB = 32, 64, 1 << 24       # (as in beams.cu)
 _SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("16q").pack, Struct("9q").pack, Struct("14q").pack
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Optional[torch.Tensor] = None, pad: int = 0):
     """The `keep` best continuations (beam k, token v) of each request, by scores[r, k] + log softmax(logits[r * K + k])[v], best first
-    and equal ones by (k, v). logits [R * K, V] float32 or bfloat16 (rows may be strided), scores float32 [R, K], K and `keep` up to 32
-    and 64. done [R, K] bool: a finished beam offers itself alone, with token `pad`, at its score (its logits are not looked at).
+    and equal ones by (k, v). logits [R * K, V] float32 or bfloat16 (rows may be strided; V up to 2^24), scores float32 [R, K], K and `keep` up
+    to 32 and 64. done [R, K] bool: a finished beam offers itself alone, with token `pad`, at its score (its logits are not looked at).
     A beam with score -inf and a token with logit -inf (a NaN counts as one) are never chosen; logits of +inf have no meaning here.
     Scores are compared in 64 bits; the sums behind them carry about 2^-25.
 
@@ -28,7 +28,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Opt
     if len(pair) != 2 or pair[0] * pair[1] != rows or scores.dtype is not torch.float32 or scores.get_device() != index or not scores.is_contiguous():
         raise ValueError(f"beam_select: dense float32 scores [requests, beams] for {rows} rows of logits on {logits.device} (got {tuple(pair)} {scores.dtype})")
     R, K = pair
-    if not 0 < K <= MAX_BEAMS or not 0 < keep <= MAX_KEEP or V < 1 or not 0 <= pad < V:
+    if not 0 < K <= MAX_BEAMS or not 0 < keep <= MAX_KEEP or not 0 < V <= MAX_VOCAB or not 0 <= pad < V:
         raise ValueError(f"beam_select: up to {MAX_BEAMS} beams, up to {MAX_KEEP} kept and a padding token of the vocabulary (got {K}, {keep}, {pad} of {V})")
     if done is not None and (done.dtype is not torch.bool or done.get_device() != index or done.shape != pair or not done.is_contiguous()):
         raise ValueError(f"beam_select: done must be dense bool {tuple(pair)} on {logits.device}")
