@@ -231,7 +231,7 @@ __device__ __forceinline__ double log_short(double s) {
     return y + (s * exp_short(-y) - 1.0);
 }
 
-constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, HELD = 16, HOT_ROOM = HELD * PICK_THREADS;
+constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, SUMS_HELD = 4, HELD = 16, HOT_ROOM = HELD * PICK_THREADS;
 
 struct Found {
     double score[PICK_ROOM];
@@ -271,8 +271,8 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     __shared__ Found found;
     __shared__ Best kept;
     __shared__ double base_s[MAX_BEAMS], best_s[MAX_BEAMS], log_s[MAX_BEAMS];
-    __shared__ float set_top[PICK_SETS];
-    __shared__ float least_s, size_s;
+    __shared__ __align__(16) float set_top[PICK_SETS + 16];
+    __shared__ float least_s, base_f[MAX_BEAMS], best_f[MAX_BEAMS], size_f[MAX_BEAMS];
     __shared__ int n_found, n_hot;
     extern __shared__ uint32_t hot[];          // [HOT_ROOM]
     const int r = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -283,25 +283,35 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     // ---- the rows' log-sums; a finished beam offers itself alone
     for (int k = warp; k < beams; k += WARPS) {
         const int row = r * beams + k;
-        const double s = (double)scores[row];
-        const bool over = done != nullptr && done[row];
-        float best = -INFINITY;
-        double log_sum = 0.0, sum = 0.0;
-        if (!over) {
-            const RowPart* p = sums + 2ll * row * parts;
-            for (int i = lane; i < 2 * parts; i += 32) best = fmaxf(best, p[i].best);
-            best = warp_max(best);
-            for (int i = lane; i < 2 * parts; i += 32) {
-                const RowPart w = p[i];
-                if (w.sum > 0.0) sum += w.sum * exp_short((double)w.best - (double)best);
-            }
-            sum = warp_sum_d(sum);
-            log_sum = log_short(sum);
+        // all that is read of a beam is asked for before any of it is used
+        const RowPart* p = sums + 2ll * row * parts;
+        RowPart w[SUMS_HELD];
+#pragma unroll
+        for (int c = 0; c < SUMS_HELD; ++c) {
+            w[c] = RowPart{-INFINITY, 0.0};
+            if (lane + c * 32 < 2 * parts) w[c] = p[lane + c * 32];
         }
+        const double s = (double)scores[row];
+        const bool over = done != nullptr && done[row];           // (its sums were never written, and are not used)
+        float best = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < SUMS_HELD; ++c) best = fmaxf(best, w[c].best);
+        for (int i = lane + SUMS_HELD * 32; i < 2 * parts; i += 32) best = fmaxf(best, p[i].best);
+        best = warp_max(best);
+        double sum = 0.0;
+#pragma unroll
+        for (int c = 0; c < SUMS_HELD; ++c)
+            if (w[c].sum > 0.0) sum += w[c].sum * exp_short((double)w[c].best - (double)best);
+        for (int i = lane + SUMS_HELD * 32; i < 2 * parts; i += 32)
+            if (p[i].sum > 0.0) sum += p[i].sum * exp_short((double)p[i].best - (double)best);
+        sum = warp_sum_d(sum);
         if (lane == 0) {
             // nothing of a beam with no score, or of a row without a finite logit, is offered
-            base_s[k] = over || !(s > -INFINITY) || !(sum > 0.0) ? -INFINITY : s;
-            best_s[k] = (double)best, log_s[k] = log_sum;
+            const bool offers = !over && s > -INFINITY && sum > 0.0;
+            const double log_sum = offers ? log_short(sum) : 0.0;
+            base_s[k] = offers ? s : -INFINITY, best_s[k] = (double)best, log_s[k] = log_sum;
+            base_f[k] = offers ? (float)(s - log_sum) : -INFINITY, best_f[k] = best;
+            size_f[k] = offers ? fabsf((float)s) + fabsf((float)log_sum) : 0.f;
             if (over && s > -INFINITY) {
                 const int i = atomicAdd(&n_found, 1);
                 found.score[i] = s, found.at[i] = (uint32_t)k * (uint32_t)V + (uint32_t)pad;
@@ -314,28 +324,21 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
     const int groups = parts * 32, all = beams * groups;
     auto beam_of = [&](int i) { return (int)((((uint32_t)i >> 5) * per_part) >> 32); };  // i / groups: per_part is 2^32 / parts, rounded up
     const float* my_tops = tops + (long long)r * all;
-    if (threadIdx.x < 32) {
-        float size = 0.f;
-        if (lane < beams && base_s[lane] > -INFINITY) size = fabsf((float)base_s[lane]) + fabsf((float)log_s[lane]);
-        size = warp_max(size);
-        if (lane == 0) size_s = size;
-    }
-    __syncthreads();
-    const float size = 2.f * size_s;
+    float size = lane < beams ? size_f[lane] : 0.f;
+    size = 2.f * warp_max(size);
     auto margin = [&](float s) { return (fabsf(s) + size) * 4.8e-7f; };
     // the best scores of the lanes from + threadIdx.x, from + threadIdx.x + PICK_THREADS, ... of the request
     float held[HELD];
     auto hold = [&](int from) {
 #pragma unroll
         for (int c = 0; c < HELD; ++c) {
-            const int i = from + threadIdx.x + c * PICK_THREADS, k = beam_of(i);       // (the same of a warp's lanes)
-            held[c] = -INFINITY;
-            if (i < all && base_s[k] > -INFINITY) held[c] = my_tops[i];       // (else they may never have been written)
+            const int i = from + threadIdx.x + c * PICK_THREADS;
+            held[c] = i < all ? my_tops[i] : -INFINITY;                       // (a finished beam's were never written, and are not used)
         }
 #pragma unroll
         for (int c = 0; c < HELD; ++c) {
-            const int k = min(beam_of(from + (int)threadIdx.x + c * PICK_THREADS), beams - 1);
-            if (held[c] > -INFINITY) held[c] = (float)(base_s[k] - log_s[k]) + (held[c] - (float)best_s[k]);
+            const int k = min(beam_of(from + (int)threadIdx.x + c * PICK_THREADS), beams - 1);         // (the same of a warp's lanes)
+            held[c] = base_f[k] > -INFINITY && held[c] > -INFINITY ? base_f[k] + (held[c] - best_f[k]) : -INFINITY;
         }
     };
     {
@@ -349,22 +352,30 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         constexpr int PER_SET = PICK_THREADS / PICK_SETS;
 #pragma unroll
         for (int o = PER_SET / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (threadIdx.x % PER_SET == 0) set_top[threadIdx.x / PER_SET] = top;
+        // a set's rank: its four threads count the better ones among a quarter of the sets each (quarters lie four floats further than
+        // the banks are wide, so that the four read side by side)
+        constexpr int QUARTER = PICK_SETS / PER_SET;
+        const int me = threadIdx.x / PER_SET, q = threadIdx.x % PER_SET;
+        if (q == 0) set_top[me / QUARTER * (QUARTER + 4) + me % QUARTER] = top;
         __syncthreads();
-        // a set's rank: its threads count a share of the better ones each
-        const int me = threadIdx.x / PER_SET;
         int above = 0;
-#pragma unroll 8
-        for (int j = threadIdx.x % PER_SET; j < PICK_SETS; j += PER_SET) above += set_top[j] > top || (set_top[j] == top && j < me) ? 1 : 0;
+#pragma unroll
+        for (int j = 0; j < QUARTER; j += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(set_top + q * (QUARTER + 4) + j);
+            const int at = q * QUARTER + j;
+            above += (v.x > top || (v.x == top && at < me)) + (v.y > top || (v.y == top && at + 1 < me)) + (v.z > top || (v.z == top && at + 2 < me)) +
+                     (v.w > top || (v.w == top && at + 3 < me));
+        }
 #pragma unroll
         for (int o = PER_SET / 2; o > 0; o >>= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
-        if (above == keep - 1 && threadIdx.x % PER_SET == 0) least_s = top;
+        if (above == keep - 1 && q == 0) least_s = top;
         __syncthreads();
     }
     // ---- the logits of the lanes that reach it, HOT_ROOM lanes' tops at a time. A find goes into the room, unless that is full: then the best
     // so far stay, the worst of them is the new bound, and the run of lanes is gone through again with barriers (rows of few
     // different values come to that)
-    double least = (double)least_s;
+    float least_f = least_s;
+    double least = (double)least_f;
     uint32_t least_at = 0xffffffffu;          // a find must be better than (least, least_at), or equal least where that is the first bound
     struct Place {
         int k, v;
@@ -386,7 +397,7 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         if (all > HOT_ROOM) hold(from);
 #pragma unroll
         for (int c = 0; c < HELD; ++c)
-            if (held[c] > -INFINITY && (double)(held[c] + margin(held[c])) >= least) hot[atomicAdd(&n_hot, 1)] = (uint32_t)(from + threadIdx.x + c * PICK_THREADS);
+            if (held[c] > -INFINITY && held[c] + margin(held[c]) >= least_f) hot[atomicAdd(&n_hot, 1)] = (uint32_t)(from + threadIdx.x + c * PICK_THREADS);
         __syncthreads();
         const int n = n_hot * LANE_VALUES, before = n_found;
         __syncthreads();
@@ -411,7 +422,7 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
                     sort_found(found, kept, have, keep);
                     if (threadIdx.x == 0) n_found = keep;
                     if (threadIdx.x < keep) found.score[threadIdx.x] = kept.score[threadIdx.x], found.at[threadIdx.x] = kept.at[threadIdx.x];
-                    least = kept.score[keep - 1], least_at = kept.at[keep - 1];
+                    least = kept.score[keep - 1], least_at = kept.at[keep - 1], least_f = __double2float_rd(least);
                     __syncthreads();
                 }
                 if (first + threadIdx.x < n) {
