@@ -492,42 +492,54 @@ reorder_states_kernel(W* state, const int* __restrict__ slot_ids, const int* __r
         reorder_unit<KMAX, W>(beams, from, [&](int k) { return item + slot_at[k] + u; });
 }
 
-// grid (blocks over rows, items, requests); pool [items][pages][nkv][page_size][units] of W; a beam's row of the block table names
-// the pages of its rows. Rows starts[r] .. ends[r] - 1 of every beam of request r take those of its parent. An entry of -1 is a
-// page that was given back: its rows are passed over.
+// What reorder_pages works on: up to two pools [items][pages][nkv][page_size][units] of W that share their pages.
+struct PagedPools {
+    void* pool[2];
+    int units[2], pools;
+};
+constexpr int PAGE_ROWS = 8;                  // rows of a beam that a block looks up and moves at a time
+
+// grid (blocks over rows, items * pools, requests); a beam's row of the block table names the pages of its rows. Rows starts[r] ..
+// ends[r] - 1 of every beam of request r take those of its parent. An entry of -1 is a page that was given back: its rows are passed
+// over. The places of PAGE_ROWS rows of all beams are looked up once, into shared memory.
 template <int KMAX, typename W>
 __global__ void __launch_bounds__(256)
-reorder_pages_kernel(W* pool, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ starts, const int* __restrict__ ends,
-                     const int* __restrict__ parents, int beams, int pages, int nkv, int page_size, int units, int* __restrict__ err) {
+reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ starts, const int* __restrict__ ends,
+                     const int* __restrict__ parents, int beams, int pages, int nkv, int page_size, int* __restrict__ err) {
     __shared__ int from[MAX_BEAMS];
+    __shared__ long long row_at[KMAX][PAGE_ROWS];        // a row's place in its item, in units; -1: it has none
     pdl_wait();
-    const int r = blockIdx.z;
+    const int r = blockIdx.z, which = blockIdx.y % p.pools;
+    const unsigned units = (unsigned)(which ? p.units[1] : p.units[0]);
     read_parents(from, parents, r, beams, err);
-    __syncthreads();
     const int begin = max(0, starts[r]), end = (int)min((long long)ends[r], (long long)bt_stride * page_size);
     if (end < ends[r] && threadIdx.x == 0) atomicOr(err, CELLM_DEV_BAD_PAGE);
-    const int per_row = nkv * units;
-    W* item = pool + (size_t)blockIdx.y * pages * per_row * page_size;
-    const long long total = (long long)max(0, end - begin) * per_row;
-    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < total; u += (long long)gridDim.x * 256) {
-        const int at = begin + (int)(u / per_row), rest = (int)(u % per_row), h = rest / units, x = rest % units;
-        const int* entry = block_table + (long long)r * beams * bt_stride + at / page_size;
-        const size_t in_page = ((size_t)h * page_size + at % page_size) * units + x;
-        W held[KMAX];
-        int to[KMAX];
-#pragma unroll
-        for (int k = 0; k < KMAX; ++k) {
-            to[k] = -1;
-            if (k >= beams || from[k] < 0) continue;
-            const int p = entry[(long long)k * bt_stride], src = entry[(long long)from[k] * bt_stride];
-            if (p >= pages || src >= pages) { atomicOr(err, CELLM_DEV_BAD_PAGE); continue; }
-            if (p < 0 || src < 0) continue;
-            to[k] = p;
-            held[k] = item[(size_t)src * per_row * page_size + in_page];
+    const unsigned per_row = (unsigned)nkv * units, head = (unsigned)page_size * units;
+    W* item = static_cast<W*>(which ? p.pool[1] : p.pool[0]) + (size_t)(blockIdx.y / p.pools) * pages * per_row * page_size;
+    for (int at = begin + blockIdx.x * PAGE_ROWS; at < end; at += gridDim.x * PAGE_ROWS) {
+        const unsigned rows = min(PAGE_ROWS, end - at);
+        __syncthreads();
+        for (int i = threadIdx.x; i < beams * PAGE_ROWS; i += 256) {
+            const int k = i / PAGE_ROWS, j = i % PAGE_ROWS;
+            if (j >= (int)rows) continue;
+            const int page = block_table[((long long)r * beams + k) * bt_stride + (at + j) / page_size];
+            if (page >= pages) atomicOr(err, CELLM_DEV_BAD_PAGE);
+            row_at[k][j] = page < 0 || page >= pages ? -1 : ((long long)page * nkv * page_size + (at + j) % page_size) * units;
         }
+        __syncthreads();
+        // neighbouring threads take a head's rows one behind the other, which lie so on their page
+        for (unsigned u = threadIdx.x; u < PAGE_ROWS * per_row; u += 256) {
+            const unsigned x = u % units, j = u / units % PAGE_ROWS, h = u / units / PAGE_ROWS;
+            if (j >= rows) continue;
+            W* place = item + (size_t)h * head + x;
+            W held[KMAX];
 #pragma unroll
-        for (int k = 0; k < KMAX; ++k)
-            if (to[k] >= 0) item[(size_t)to[k] * per_row * page_size + in_page] = held[k];
+            for (int k = 0; k < KMAX; ++k)
+                if (k < beams && from[k] >= 0 && row_at[from[k]][j] >= 0 && row_at[k][j] >= 0) held[k] = place[row_at[from[k]][j]];
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k)
+                if (k < beams && from[k] >= 0 && row_at[from[k]][j] >= 0 && row_at[k][j] >= 0) place[row_at[k][j]] = held[k];
+        }
     }
 }
 
@@ -547,13 +559,13 @@ int launch_states(void* state, const int* slot_ids, const int* parents, int requ
 }
 
 template <typename W>
-int launch_pages(void* pool, const int* block_table, int bt_stride, const int* starts, const int* ends, const int* parents, int requests, int beams,
-                 int items, int pages, int nkv, int page_size, int row_bytes, int* err, cudaStream_t stream) {
-    const int units = row_bytes / (int)sizeof(W);
-    const long long most = (long long)bt_stride * page_size * nkv * units;
-    const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>((most + 255) / 256, 512));
-    const dim3 grid(blocks, (unsigned)items, (unsigned)requests);
-#define GO(K_) CELLM_RUN((reorder_pages_kernel<K_, W>), grid, 256, 0, stream, (W*)pool, block_table, bt_stride, starts, ends, parents, beams, pages, nkv, page_size, units, err)
+int launch_pages(PagedPools p, const int* block_table, int bt_stride, const int* starts, const int* ends, const int* parents, int requests, int beams,
+                 int items, int pages, int nkv, int page_size, int sms, int* err, cudaStream_t stream) {
+    for (int i = 0; i < p.pools; ++i) p.units[i] /= (int)sizeof(W);
+    const long long most = ((long long)bt_stride * page_size + PAGE_ROWS - 1) / PAGE_ROWS, rest = (long long)items * p.pools * requests;
+    const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>(most, 64ll * sms / rest));
+    const dim3 grid(blocks, (unsigned)(items * p.pools), (unsigned)requests);
+#define GO(K_) CELLM_RUN((reorder_pages_kernel<K_, W>), grid, 256, 0, stream, p, block_table, bt_stride, starts, ends, parents, beams, pages, nkv, page_size, err)
     if (beams <= 4) GO(4);
     else if (beams <= 8) GO(8);
     else if (beams <= 16) GO(16);
@@ -612,14 +624,17 @@ CELLM_API int cellm_reorder_states(void* state, const int* slot_ids, const int* 
     return CELLM_ERR_ALIGN;
 }
 
-// pool [items][pages][nkv][page_size][row_bytes], in place; block_table [requests * beams][bt_stride].
-CELLM_API int cellm_reorder_pages(void* pool, const int* block_table, int bt_stride, const int* starts, const int* ends, const int* parents, int requests,
-                                  int beams, int items, int pages, int nkv, int page_size, int row_bytes, int* err, cudaStream_t stream) {
-    if (requests <= 0 || items <= 0 || row_bytes <= 0) return CELLM_OK;
-    if (beams <= 0 || beams > MAX_BEAMS || pages <= 0 || nkv <= 0 || page_size <= 0 || bt_stride <= 0 || items > 65535 || requests > 65535) return CELLM_ERR_SIZE;
-    if (!pool || !block_table || !starts || !ends || !parents || !err) return CELLM_ERR_ARG;
-    const uintptr_t at = (uintptr_t)pool | (uintptr_t)row_bytes;
-#define GO(W_) return launch_pages<W_>(pool, block_table, bt_stride, starts, ends, parents, requests, beams, items, pages, nkv, page_size, row_bytes, err, stream)
+// k_pool [items][pages][nkv][page_size][k_bytes] and (or null) v_pool likewise, in place; block_table [requests * beams][bt_stride].
+CELLM_API int cellm_reorder_pages(void* k_pool, int k_bytes, void* v_pool, int v_bytes, const int* block_table, int bt_stride, const int* starts, const int* ends,
+                                  const int* parents, int requests, int beams, int items, int pages, int nkv, int page_size, int sms, int* err, cudaStream_t stream) {
+    if (requests <= 0 || items <= 0) return CELLM_OK;
+    if (beams <= 0 || beams > MAX_BEAMS || pages <= 0 || nkv <= 0 || page_size <= 0 || bt_stride <= 0 || items > 32767 || requests > 65535 || sms <= 0 || k_bytes <= 0 ||
+        (v_pool && v_bytes <= 0) || (long long)nkv * page_size * std::max(k_bytes, v_bytes) > 0x7fffffffLL)
+        return CELLM_ERR_SIZE;
+    if (!k_pool || !block_table || !starts || !ends || !parents || !err) return CELLM_ERR_ARG;
+    const PagedPools p = {{k_pool, v_pool}, {k_bytes, v_bytes}, v_pool ? 2 : 1};
+    const uintptr_t at = (uintptr_t)k_pool | (uintptr_t)k_bytes | (v_pool ? (uintptr_t)v_pool | (uintptr_t)v_bytes : 0);
+#define GO(W_) return launch_pages<W_>(p, block_table, bt_stride, starts, ends, parents, requests, beams, items, pages, nkv, page_size, sms, err, stream)
     if (at % 16 == 0) GO(uint4);
     if (at % 4 == 0) GO(uint32_t);
     if (at % 2 == 0) GO(uint16_t);
@@ -641,6 +656,6 @@ CELLM_API int cellm_reorder_states_packed(const long long* a, cudaStream_t strea
 
 // The same with its arguments in order as 64-bit words (see common.cuh).
 CELLM_API int cellm_reorder_pages_packed(const long long* a, cudaStream_t stream) {
-    return cellm_reorder_pages((void*)a[0], (const int*)a[1], (int)a[2], (const int*)a[3], (const int*)a[4], (const int*)a[5], (int)a[6], (int)a[7],
-        (int)a[8], (int)a[9], (int)a[10], (int)a[11], (int)a[12], (int*)a[13], stream);
+    return cellm_reorder_pages((void*)a[0], (int)a[1], (void*)a[2], (int)a[3], (const int*)a[4], (int)a[5], (const int*)a[6], (const int*)a[7], (const int*)a[8], (int)a[9],
+        (int)a[10], (int)a[11], (int)a[12], (int)a[13], (int)a[14], (int)a[15], (int*)a[16], stream);
 }

@@ -21,71 +21,61 @@ struct DraftRows {             // keys or values: [items][T] rows beside the cac
 };
 
 template <typename W>
-__device__ __forceinline__ void copy_rows(const DraftRows& d, int items, int nkv, int pages, int page_size, const int* path, const int* place_page,
-                                          int count, int t_base, int ctx) {
-    const int units = d.row_bytes / (int)sizeof(W), per_node = nkv * units;
-    const long long total = (long long)items * count * per_node;
-    const char* rows = static_cast<const char*>(d.rows);
-    W* pool = static_cast<W*>(d.pool);
-    for (long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x; u < total; u += (long long)gridDim.x * blockDim.x) {
-        const int item = (int)(u / ((long long)count * per_node)), rest = (int)(u % ((long long)count * per_node));
-        const int j = rest / per_node, hx = rest % per_node, h = hx / units, x = hx % units;
-        const int page = place_page[j];
-        if (page < 0) continue;
-        const W v = *reinterpret_cast<const W*>(rows + item * d.item_ld + (long long)(t_base + path[j]) * d.row_ld + (long long)hx * sizeof(W));
-        pool[((((size_t)item * pages + page) * nkv + h) * page_size + (ctx + j) % page_size) * units + x] = v;
-    }
-}
-
-template <typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(TREE_MAX)
 accept_drafts_kernel(int* __restrict__ out_count, int* __restrict__ out_path, int* __restrict__ out_next, const int* __restrict__ tokens,
                      const int* __restrict__ parents, const int* __restrict__ choices, const int* __restrict__ cu_seqlens, int T, int longest,
                      const DraftRows k, const DraftRows v, const int* __restrict__ ctx_lens, const int* __restrict__ block_table, int bt_stride,
                      int items, int nkv, int pages, int page_size, int* __restrict__ err) {
-    __shared__ int child[TREE_MAX], path[TREE_MAX], place_page[TREE_MAX];
+    __shared__ int child[TREE_MAX], choice[TREE_MAX], path[TREE_MAX], place_page[TREE_MAX];
     __shared__ int count_s;
     pdl_wait();
-    const int b = blockIdx.y, t_base = cu_seqlens[b];
+    // what does not depend on the walk is asked for before it
+    const int b = blockIdx.y, t_base = cu_seqlens[b], ctx = items > 0 ? ctx_lens[b] : 0;
     int n = cu_seqlens[b + 1] - t_base;
     if (n > TREE_MAX || n < 0 || t_base < 0 || t_base + n > T) {
         if (threadIdx.x == 0) atomicOr(err, CELLM_DEV_BAD_TREE);
         n = 0;
     }
-    for (int i = threadIdx.x; i < n; i += blockDim.x) child[i] = TREE_MAX;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int p = parents[t_base + i];
-        if (p >= i) atomicOr(err, CELLM_DEV_BAD_TREE);
-        else if (p >= 0 && tokens[t_base + i] == choices[t_base + p]) atomicMin(&child[p], i);
+    const int me = threadIdx.x, node_parent = me < n ? parents[t_base + me] : -1, node_token = me < n ? tokens[t_base + me] : 0;
+    if (me < n) child[me] = TREE_MAX, choice[me] = choices[t_base + me];
+    if (items > 0 && me < min(longest, n)) {
+        const long long at = ((long long)ctx + me) / page_size;
+        const int page = ctx >= 0 && at < bt_stride ? block_table[(long long)b * bt_stride + at] : -1;
+        place_page[me] = page < 0 || page >= pages ? -1 : page;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (me < n) {
+        if (node_parent >= me) atomicOr(err, CELLM_DEV_BAD_TREE);
+        else if (node_parent >= 0 && node_token == choice[node_parent]) atomicMin(&child[node_parent], me);
+    }
+    __syncthreads();
+    if (me == 0) {
         int c = 0;
         // (a tree whose first node is padding keeps nothing)
-        for (int at = n > 0 && parents[t_base] == -1 ? 0 : n; at < n && c < longest && c < TREE_MAX; at = child[at]) path[c++] = at;
+        for (int at = n > 0 && node_parent == -1 ? 0 : n; at < n && c < longest; at = child[at]) path[c++] = at;
         count_s = c;
     }
     __syncthreads();
     const int count = count_s;
     if (blockIdx.x == 0) {
-        for (int j = threadIdx.x; j < longest; j += blockDim.x) out_path[(long long)b * longest + j] = j < count ? path[j] : -1;
-        if (threadIdx.x == 0) out_count[b] = count, out_next[b] = count > 0 ? choices[t_base + path[count - 1]] : -1;
+        for (int j = me; j < longest; j += TREE_MAX) out_path[(long long)b * longest + j] = j < count ? path[j] : -1;
+        if (me == 0) out_count[b] = count, out_next[b] = count > 0 ? choice[path[count - 1]] : -1;
+        if (items > 0 && me < count && place_page[me] < 0) atomicOr(err, CELLM_DEV_BAD_PAGE);
     }
-    if (items == 0) return;
-    const int ctx = ctx_lens[b];
-    for (int j = threadIdx.x; j < count; j += blockDim.x) {
-        const long long at = ((long long)ctx + j) / page_size;
-        int page = ctx >= 0 && at < bt_stride ? block_table[(long long)b * bt_stride + at] : -1;
-        if (page < 0 || page >= pages) {
-            atomicOr(err, CELLM_DEV_BAD_PAGE);
-            page = -1;
-        }
-        place_page[j] = page;
+    // the kept rows: neighbouring threads take a head's pieces, then the kept nodes, whose rows lie one behind the other on a page
+    const unsigned k_units = (unsigned)k.row_bytes / sizeof(W), v_units = (unsigned)v.row_bytes / sizeof(W);
+    const unsigned k_item = (unsigned)(count * nkv) * k_units, per_item = k_item + (unsigned)(count * nkv) * v_units;
+    for (unsigned long long u = (unsigned long long)blockIdx.x * TREE_MAX + me; u < (unsigned long long)items * per_item; u += (unsigned long long)gridDim.x * TREE_MAX) {
+        const unsigned item = (unsigned)(u / per_item), in_item = (unsigned)(u - (unsigned long long)item * per_item);
+        const bool value = in_item >= k_item;
+        const DraftRows& d = value ? v : k;
+        const unsigned units = value ? v_units : k_units, rest = value ? in_item - k_item : in_item;
+        const unsigned x = rest % units, j = rest / units % count, h = rest / units / count;
+        const int page = place_page[j];
+        if (page < 0) continue;
+        const W* src = reinterpret_cast<const W*>(static_cast<const char*>(d.rows) + item * d.item_ld + (long long)(t_base + path[j]) * d.row_ld) + h * units + x;
+        static_cast<W*>(d.pool)[((((size_t)item * pages + page) * nkv + h) * page_size + (ctx + j) % page_size) * units + x] = *src;
     }
-    __syncthreads();
-    copy_rows<W>(k, items, nkv, pages, page_size, path, place_page, count, t_base, ctx);
-    if (v.rows != nullptr) copy_rows<W>(v, items, nkv, pages, page_size, path, place_page, count, t_base, ctx);
 }
 
 }  // namespace
@@ -101,16 +91,17 @@ CELLM_API int cellm_accept_drafts(int* out_count, int* out_path, int* out_next, 
     if (B > 65535 || T < 0 || longest <= 0 || items < 0 || (items > 0 && (nkv <= 0 || pages <= 0 || page_size <= 0 || k_bytes <= 0 || bt_stride < 0))) return CELLM_ERR_SIZE;
     if (!out_count || !out_path || !out_next || !tokens || !parents || !choices || !cu_seqlens || !err) return CELLM_ERR_ARG;
     if (items > 0 && (!k_new || !k_pool || !ctx_lens || !block_table || (v_new && (!v_pool || v_bytes <= 0)))) return CELLM_ERR_ARG;
-    const DraftRows k = {items > 0 ? k_new : nullptr, k_pool, k_item, k_row, k_bytes}, v = {items > 0 ? v_new : nullptr, v_pool, v_item, v_row, v_bytes};
+    const DraftRows k = {items > 0 ? k_new : nullptr, k_pool, k_item, k_row, items > 0 ? k_bytes : 0},
+                    v = {items > 0 ? v_new : nullptr, v_pool, v_item, v_row, items > 0 && v_new ? v_bytes : 0};
     uintptr_t at = 0;
     if (k.rows) at |= (uintptr_t)k.rows | (uintptr_t)k.pool | (uintptr_t)k_item | (uintptr_t)k_row | (uintptr_t)k_bytes;
     if (v.rows) at |= (uintptr_t)v.rows | (uintptr_t)v.pool | (uintptr_t)v_item | (uintptr_t)v_row | (uintptr_t)v_bytes;
     const int width = at % 16 == 0 ? 16 : at % 4 == 0 ? 4 : 2;
     if (at % 2) return CELLM_ERR_ALIGN;
     // blocks for three kept nodes of every request; more nodes take a block's threads round again
-    const long long units = items > 0 ? (long long)items * nkv * (k_bytes / width) * std::min(longest, 3) : 1;
-    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>((units + 255) / 256, 256)), (unsigned)B);
-#define GO(W_) CELLM_RUN(accept_drafts_kernel<W_>, grid, 256, 0, stream, out_count, out_path, out_next, tokens, parents, choices, cu_seqlens, T, longest, k, v, \
+    const long long units = items > 0 ? (long long)items * nkv * ((k.row_bytes + v.row_bytes) / width) * std::min(longest, 3) : 1;
+    const dim3 grid((unsigned)std::max<long long>(1, std::min<long long>((units + TREE_MAX - 1) / TREE_MAX, 256)), (unsigned)B);
+#define GO(W_) CELLM_RUN(accept_drafts_kernel<W_>, grid, TREE_MAX, 0, stream, out_count, out_path, out_next, tokens, parents, choices, cu_seqlens, T, longest, k, v, \
                          ctx_lens, block_table, bt_stride, items, nkv, pages, page_size, err)
     if (width == 16) GO(uint4);
     else if (width == 4) GO(uint32_t);

@@ -126,7 +126,7 @@ _SIGNATURES = {
         "cellm_beam_parts": [I],
         "cellm_beam_select": [P, P, P, P, P, P, L, I, I, I, I, P, P, I, I, I, P],
         "cellm_reorder_states": [P, P, P, I, I, I, I, L, P, P],
-        "cellm_reorder_pages": [P, P, I, P, P, P, I, I, I, I, I, I, I, P, P],
+        "cellm_reorder_pages": [P, I, P, I, P, I, P, P, P, I, I, I, I, I, I, I, P, P],
     },
     "attention_expanded": {
         "cellm_latent_rows": [P, P, P, P, P, I, I, I, I, I, I, I, P, P],

@@ -10,7 +10,7 @@ from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
 from ._state import _SM_COUNT, sm_count
 
 MAX_BEAMS, MAX_KEEP, MAX_VOCAB = 32, 64, 1 << 24       # (as in beams.cu)
-_SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("16q").pack, Struct("9q").pack, Struct("14q").pack
+_SELECT_ARGS, _STATES_ARGS, _PAGES_ARGS = Struct("16q").pack, Struct("9q").pack, Struct("17q").pack
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Optional[torch.Tensor] = None, pad: int = 0):
@@ -84,10 +84,10 @@ def reorder_pages(k_pool: torch.Tensor, v_pool: Optional[torch.Tensor], block_ta
         if len(own) not in (3, 4) or p.shape[:-1] != own or p.get_device() != index or not p.is_contiguous() or p.element_size() % 2:
             raise ValueError("reorder_pages: dense pools [items, pages, kv heads, page size, head size] of elements of 2, 4 or 8 bytes, alike but for the head size, "
                              f"on {parents.device}")
-    if R == 0 or table[1] == 0:
+    if R == 0 or table[1] == 0 or k_pool.numel() == 0:
         return
-    for p in pools:
-        if p.numel():
-            launch_packed("candidates", "reorder_pages", index,
-                          _PAGES_ARGS(p.data_ptr(), block_table.data_ptr(), table[1], starts.data_ptr(), ends.data_ptr(), parents.data_ptr(), R, K,
-                                      own[0] if len(own) == 4 else 1, own[-3], own[-2], own[-1], p.shape[-1] * p.element_size(), err.data_ptr()))
+    k, v = k_pool.data_ptr(), 0 if v_pool is None else v_pool.data_ptr()
+    launch_packed("candidates", "reorder_pages", index,
+                  _PAGES_ARGS(k, k_pool.shape[-1] * k_pool.element_size(), v, v_pool.shape[-1] * v_pool.element_size() if v else 0, block_table.data_ptr(), table[1],
+                              starts.data_ptr(), ends.data_ptr(), parents.data_ptr(), R, K, own[0] if len(own) == 4 else 1, own[-3], own[-2], own[-1],
+                              _SM_COUNT.get(index) or sm_count(index), err.data_ptr()))

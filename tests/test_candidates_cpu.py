@@ -55,11 +55,12 @@ def test_selection_and_reordering():
     assert states(state=None) == ARG and states(slots=None) == ARG and states(size=63) == ALIGN and states(state=A + 1) == ALIGN
     assert states(R=0) == 0 and states(items=0) == 0 and states(size=0) == 0
 
-    def pages(pool=A, table=A, stride=4, R=2, K=3, items=1, n=8, nkv=2, page=16, row=64):
-        return call("candidates", "cellm_reorder_pages", pool, table, stride, A, A, A, R, K, items, n, nkv, page, row, A, None)
-    for bad in (dict(K=0), dict(K=33), dict(n=0), dict(nkv=0), dict(page=0), dict(stride=0), dict(items=65536), dict(R=65536)):
+    def pages(pool=A, table=A, stride=4, R=2, K=3, items=1, n=8, nkv=2, page=16, row=64, v=None, v_row=0):
+        return call("candidates", "cellm_reorder_pages", pool, row, v, v_row, table, stride, A, A, A, R, K, items, n, nkv, page, 148, A, None)
+    for bad in (dict(K=0), dict(K=33), dict(n=0), dict(nkv=0), dict(page=0), dict(stride=0), dict(items=65536), dict(R=65536), dict(row=0), dict(v=A), dict(page=2 ** 30)):
         assert pages(**bad) == SIZE, bad
-    assert pages(pool=None) == ARG and pages(table=None) == ARG and pages(row=63) == ALIGN and pages(R=0) == 0 and pages(row=0) == 0
+    assert pages(pool=None) == ARG and pages(table=None) == ARG and pages(row=63) == ALIGN and pages(v=A, v_row=63) == ALIGN and pages(v=A + 1, v_row=64) == ALIGN
+    assert pages(R=0) == 0 and pages(items=0) == 0
 
 
 def test_tensors_on_the_host_are_refused():
