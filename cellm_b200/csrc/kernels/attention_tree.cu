@@ -6,8 +6,9 @@
 // position, then the nodes by their place in the tree, each with a mask of one bit a key.
 //
 // Sums, maxima and the output's accumulators are 32-bit; a row is rounded once, when it is written (the tensor-core kernel
-// rounds the weights too). Where the keys are cut into pieces (few rows, long contexts), a piece leaves its maximum, sum and
-// unnormalised output in a workspace, and a second kernel merges them in their order.
+// rounds the weights too). Where the keys are cut into pieces (few rows, long contexts), up to eight pieces are one thread-block cluster:
+// each keeps its maximum, sum and unnormalised output in its shared memory, and every CTA merges a share of the rows out of its
+// peers' memory. More pieces leave them in a workspace, and a second kernel merges. Either way in the pieces' order.
 #include <algorithm>
 #include <climits>
 
@@ -16,11 +17,101 @@
 
 namespace {
 
+// ---------------------------------------------------------------- a tile's results
+__device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// What lies at `local` in the shared memory of CTA `rank` of this cluster.
+__device__ __forceinline__ float2 peer_pair(const float* local, uint32_t rank) {
+    uint32_t addr;
+    float2 v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(rank));
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void write_pair(T* out, float2 v, bool both) {
+    if constexpr (sizeof(T) == 2) {
+        if (both) *reinterpret_cast<uint32_t*>(out) = pack_bf16(v.x, v.y);
+        else out[0] = from_float<T>(v.x);
+    } else {
+        if (both) *reinterpret_cast<float2*>(out) = v;
+        else out[0] = v.x;
+    }
+}
+
+// The block's rows, row0 .. row0 + RT - 1 of the tree's (node, head) pairs: o [RT][LD] and ml [RT][2] (maximum and sum) in shared
+// memory, written before a barrier. 16 of the 128 threads take a row. Rows of padding become zeros.
+template <typename T, bool CL>
+__device__ __forceinline__ void finish_rows(const TreeArgs& a, const TreeTile& t, const TreeShape& tree, const float* o, int LD, const float* ml, int RT, int row0) {
+    const int G = a.nh / a.nkv, rows = t.n * G, hd = a.hd, c = threadIdx.x & 15;
+    const bool even = hd % 2 == 0;
+    if constexpr (CL) cluster_meet();                   // every piece of the rows is there
+    const int first = CL ? t.split : 0, step = CL ? a.nsplit : 1;
+    for (int r = first + (threadIdx.x >> 4) * step; r < RT && row0 + r < rows; r += 8 * step) {
+        const int node = (row0 + r) / G;
+        const bool seen = tree.depth[node] >= 0;
+        const long long gr = (long long)(t.t_base + node) * a.nh + t.kvh * G + (row0 + r) % G;
+        if (!CL && a.nsplit > 1) {
+            if (c == 0) *reinterpret_cast<float2*>(a.part_ml + ((long long)t.split * a.T * a.nh + gr) * 2) = seen ? make_float2(ml[r * 2], ml[r * 2 + 1]) : make_float2(-INFINITY, 0.f);
+            float* dst = a.part_o + ((long long)t.split * a.T * a.nh + gr) * hd;
+            for (int d = c; d < hd; d += 16) dst[d] = seen ? o[r * LD + d] : 0.f;
+            continue;
+        }
+        float weight[CL ? 8 : 1], l = 0.f;
+        if constexpr (CL) {
+            float2 all[8];
+            float M = -INFINITY;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) {
+                all[s] = s < a.nsplit ? peer_pair(ml + r * 2, s) : make_float2(-INFINITY, 0.f);
+                M = fmaxf(M, all[s].x);
+            }
+            const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int s = 0; s < 8; ++s) weight[s] = exp2f(all[s].x - use), l = fmaf(weight[s], all[s].y, l);
+        } else {
+            weight[0] = 1.f, l = ml[r * 2 + 1];
+        }
+        const float inv = l != 0.f ? 1.f / l : 0.f;                            // 0 where nothing is seen; NaN stays
+        for (int d = c * 2; d < hd; d += 32) {
+            float2 v = make_float2(0.f, 0.f);
+            if constexpr (CL) {
+                float2 p[8];
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < a.nsplit) p[s] = peer_pair(o + r * LD + d, s);
+#pragma unroll
+                for (int s = 0; s < 8; ++s)
+                    if (s < a.nsplit && weight[s] != 0.f) v.x = fmaf(weight[s], p[s].x, v.x), v.y = fmaf(weight[s], p[s].y, v.y);
+            } else {
+                v = make_float2(o[r * LD + d], o[r * LD + d + 1]);
+            }
+            v = seen ? make_float2(v.x * inv, v.y * inv) : make_float2(0.f, 0.f);
+            T* dst = static_cast<T*>(a.out) + gr * hd + d;
+            if (even) {
+                write_pair<T>(dst, v, true);
+            } else {
+                write_pair<T>(dst, v, false);
+                if (d + 1 < hd) write_pair<T>(dst + 1, make_float2(v.y, 0.f), false);
+            }
+        }
+    }
+    if constexpr (CL) cluster_meet();                   // nobody leaves while its memory is read
+}
+
 // ---------------------------------------------------------------- any type, any head size up to 256
-// 128 threads take 32 rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit arithmetic: a
-// thread forms 4 x KT/16 scores out of shared memory, a row's maximum and sum go over half a warp, and the thread then owns 4 x
-// HDP/16 entries of the output.
-template <int HDP> struct PlainTile { static constexpr int KEYS = HDP <= 128 ? 64 : 32; };
+// 128 threads take 8 R rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit multiply-adds: a
+// thread forms R x KT/16 scores out of shared memory, a row's maximum and sum go over half a warp, and the thread then owns R x HDP/16
+// entries of the output. 32-bit rows on 16-byte borders (FAST) come in by cp.async, the next block while one is worked on; others
+// element by element.
+template <int HDP, int R, bool FAST>
+struct PlainTile {
+    static constexpr int RT = 8 * R, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
+    static constexpr int KV = KT * LD;                                   // floats of a block's keys, and of its values
+    static constexpr size_t bytes = sizeof(TreeShape) + (size_t)(RT * LD + ST * 2 * KV + KT * (RT + 4)) * 4;
+};
 
 template <typename T>
 __device__ __forceinline__ void row_to_floats(float* dst, const T* src, int hd, int padded, int lane, int lanes, bool quads) {
@@ -42,117 +133,177 @@ __device__ __forceinline__ void row_to_floats(float* dst, const T* src, int hd, 
     }
 }
 
-template <typename T, int HDP>
+template <typename T, int HDP, int R, bool FAST, bool CL>
 __global__ void __launch_bounds__(128)
 attention_tree_plain_kernel(const TreeArgs a, int quads) {
-    constexpr int RT = 32, KT = PlainTile<HDP>::KEYS, LD = HDP + 4, KC = KT / 16;
-    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC);
+    using L = PlainTile<HDP, R, FAST>;
+    constexpr int RT = L::RT, KT = L::KT, LD = L::LD, KC = KT / 16;
+    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC), CHUNKS = HDP / 4, ITERS = KT * CHUNKS / 128;
     extern __shared__ __align__(16) uint8_t plain_smem[];
     TreeShape& tree = *reinterpret_cast<TreeShape*>(plain_smem);
     float* qs = reinterpret_cast<float*>(plain_smem + sizeof(TreeShape));     // [RT][LD]
-    float* ks = qs + RT * LD;                                          // [KT][LD]
-    float* vs = ks + KT * LD;                                          // [KT][LD]
-    float* ps = vs + KT * LD;                                          // [KT][RT + 4]
+    float* kv = qs + RT * LD;                                                 // [ST][keys | values][KT][LD]
+    float* ps = kv + L::ST * 2 * L::KV;                                       // [KT][RT + 4]
     pdl_wait();
     pdl_trigger();
     const TreeTile t = tree_tile(a);
-    const int G = a.nh / a.nkv, rows = t.n * G;
-    if (!t.live || t.tile * RT >= rows) return;
-    read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
+    const int G = a.nh / a.nkv, rows = t.n * G, row0 = t.tile * RT;
+    if (!t.live || row0 >= rows) return;
 
     const int hd = a.hd, rg = threadIdx.x >> 4, c = threadIdx.x & 15;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
+    const int first = lo / KT, committed = lo < t.ctx ? (t.ctx + KT - 1) / KT - first : 0, blocks = committed + (t.n + KT - 1) / KT;
+    const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), n_blk = min(blocks, begin + per) - begin;
+    const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
+    // FAST: as in the tensor-core kernel below; an entry of the table is asked for a block before its rows are
+    int entry[FAST ? ITERS : 1];
+    auto look_up = [&](int i) {
+#pragma unroll
+        for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
+            const int blk = begin + i, j = (first + blk) * KT + (threadIdx.x + it * 128) / CHUNKS;
+            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[j / a.page_size] : -2;
+        }
+    };
+    auto load = [&](int i) {
+        if (i < n_blk) {
+            float* ks = kv + (i & 1) * 2 * L::KV;
+            const int blk = begin + i;
+#pragma unroll
+            for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
+                const int row = (threadIdx.x + it * 128) / CHUNKS, chunk = (threadIdx.x + it * 128) % CHUNKS;
+                const float *k = static_cast<const float*>(a.k_pool), *v = static_cast<const float*>(a.v_pool);
+                bool have = chunk * 4 < hd;
+                if (blk < committed) {
+                    const int page = entry[it];
+                    if (page >= 0 && page < a.num_pages) {
+                        const size_t off = (((size_t)page * a.nkv + t.kvh) * a.page_size + ((first + blk) * KT + row) % a.page_size) * hd + chunk * 4;
+                        if (have) k += off, v += off;
+                    } else {
+                        if (page != -2) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                        have = false;
+                    }
+                } else {
+                    const int node = (blk - committed) * KT + row;
+                    have = have && node < t.n && tree.depth[node] >= 0;
+                    if (have) {
+                        k = static_cast<const float*>(a.k_new) + (t.t_base + node) * a.k_ld + t.kvh * hd + chunk * 4;
+                        v = static_cast<const float*>(a.v_new) + (t.t_base + node) * a.v_ld + t.kvh * hd + chunk * 4;
+                    }
+                }
+                cp_async16(ks + row * LD + chunk * 4, k, have ? 16 : 0);
+                cp_async16(ks + L::KV + row * LD + chunk * 4, v, have ? 16 : 0);
+            }
+        }
+        cp_async_commit();
+    };
+    look_up(0);
+    const bool early = FAST && begin < committed;          // the first block needs nothing of the tree's shape
+    if (early) load(0);
     for (int r = warp; r < RT; r += 4) {
-        const int row = t.tile * RT + r;
+        const int row = row0 + r;
         const T* src = row < rows ? static_cast<const T*>(a.q) + (long long)(t.t_base + row / G) * a.q_ld + (long long)(t.kvh * G + row % G) * hd : nullptr;
         row_to_floats(qs + r * LD, src, hd, HDP, lane, 32, quads);
     }
-    // a thread's rows are rg, rg + 8, rg + 16, rg + 24 of the tile
-    int node[4];
-    float m[4], l[4], o[4][NV * VEC];
+    read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
+    if (FAST && !early) load(0);
+    look_up(1);
+    // a thread's rows are rg, rg + 8, rg + 16, ... of the tile
+    int node[R];
+    float m[R], l[R], o[R][NV * VEC];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = t.tile * RT + rg + i * 8;
+    for (int i = 0; i < R; ++i) {
+        const int row = row0 + rg + i * 8;
         node[i] = row < rows && tree.depth[row / G] >= 0 ? row / G : -1;
         m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
         for (int d = 0; d < NV * VEC; ++d) o[i][d] = 0.f;
     }
-    const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
-    const int first = lo / KT, committed = lo < t.ctx ? (t.ctx + KT - 1) / KT - first : 0, blocks = committed + (t.n + KT - 1) / KT;
-    const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), end = min(blocks, begin + per);
-    const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
-    for (int blk = begin; blk < end; ++blk) {
+    for (int i = 0; i < n_blk; ++i) {
+        const int blk = begin + i;
         const bool paged = blk < committed;
         const int key0 = (first + blk) * KT, node0 = paged ? -1 : (blk - committed) * KT;
-        __syncthreads();
-        for (int r = warp; r < KT; r += 4) {
-            const T *k = nullptr, *v = nullptr;
-            if (paged) {
-                const int j = key0 + r;
-                if (j >= lo && j < t.ctx) {
-                    const int page = bt[j / a.page_size];
-                    if (page < 0 || page >= a.num_pages) {
-                        if (lane == 0) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
-                    } else {
-                        const size_t off = (((size_t)page * a.nkv + t.kvh) * a.page_size + j % a.page_size) * hd;
-                        k = static_cast<const T*>(a.k_pool) + off, v = static_cast<const T*>(a.v_pool) + off;
+        float *ks = kv + (FAST ? (i & 1) * 2 * L::KV : 0), *vs = ks + L::KV;
+        if constexpr (FAST) {
+            cp_async_wait<0>();
+            __syncthreads();
+            load(i + 1);                       // into the stage that everybody left before the barrier
+            look_up(i + 2);
+        } else {
+            __syncthreads();
+            for (int r = warp; r < KT; r += 4) {
+                const T *k = nullptr, *v = nullptr;
+                if (paged) {
+                    const int j = key0 + r;
+                    if (j >= lo && j < t.ctx) {
+                        const int page = bt[j / a.page_size];
+                        if (page < 0 || page >= a.num_pages) {
+                            if (lane == 0) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                        } else {
+                            const size_t off = (((size_t)page * a.nkv + t.kvh) * a.page_size + j % a.page_size) * hd;
+                            k = static_cast<const T*>(a.k_pool) + off, v = static_cast<const T*>(a.v_pool) + off;
+                        }
                     }
+                } else if (node0 + r < t.n && tree.depth[node0 + r] >= 0) {
+                    k = static_cast<const T*>(a.k_new) + (long long)(t.t_base + node0 + r) * a.k_ld + (long long)t.kvh * hd;
+                    v = static_cast<const T*>(a.v_new) + (long long)(t.t_base + node0 + r) * a.v_ld + (long long)t.kvh * hd;
                 }
-            } else if (node0 + r < t.n && tree.depth[node0 + r] >= 0) {
-                k = static_cast<const T*>(a.k_new) + (long long)(t.t_base + node0 + r) * a.k_ld + (long long)t.kvh * hd;
-                v = static_cast<const T*>(a.v_new) + (long long)(t.t_base + node0 + r) * a.v_ld + (long long)t.kvh * hd;
+                row_to_floats(ks + r * LD, k, hd, HDP, lane, 32, quads);
+                row_to_floats(vs + r * LD, v, hd, HDP, lane, 32, quads);
             }
-            row_to_floats(ks + r * LD, k, hd, HDP, lane, 32, quads);
-            row_to_floats(vs + r * LD, v, hd, HDP, lane, 32, quads);
+            __syncthreads();
         }
-        __syncthreads();
-        float s[4][KC];
+        float s[R][KC];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int x = 0; x < R; ++x)
 #pragma unroll
-            for (int k = 0; k < KC; ++k) s[i][k] = 0.f;
+            for (int k = 0; k < KC; ++k) s[x][k] = 0.f;
 #pragma unroll 2
         for (int d = 0; d < HDP; d += 4) {
-            float4 q4[4], k4[KC];
+            float4 q4[R], k4[KC];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(qs + (rg + i * 8) * LD + d);
+            for (int x = 0; x < R; ++x) q4[x] = *reinterpret_cast<const float4*>(qs + (rg + x * 8) * LD + d);
 #pragma unroll
             for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const float4*>(ks + (c + k * 16) * LD + d);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int x = 0; x < R; ++x)
 #pragma unroll
                 for (int k = 0; k < KC; ++k)
-                    s[i][k] = fmaf(q4[i].w, k4[k].w, fmaf(q4[i].z, k4[k].z, fmaf(q4[i].y, k4[k].y, fmaf(q4[i].x, k4[k].x, s[i][k]))));
+                    s[x][k] = fmaf(q4[x].w, k4[k].w, fmaf(q4[x].z, k4[k].z, fmaf(q4[x].y, k4[k].y, fmaf(q4[x].x, k4[k].x, s[x][k]))));
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint64_t seen = node[i] >= 0 ? seen_bits<KT>(tree, node[i], a.window, t.ctx, key0, node0) : 0ull;
+        for (int x = 0; x < R; ++x) {
+            const uint64_t seen = node[x] >= 0 ? seen_bits<KT>(tree, node[x], a.window, t.ctx, key0, node0) : 0ull;
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
-                s[i][k] = (seen >> (c + k * 16) & 1ull) ? s[i][k] * a.scale_log2e : -INFINITY;
-                top = fmaxf(top, s[i][k]);
+                s[x][k] = (seen >> (c + k * 16) & 1ull) ? s[x][k] * a.scale_log2e : -INFINITY;
+                top = fmaxf(top, s[x][k]);
             }
 #pragma unroll
-            for (int x = 8; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float now = fmaxf(m[i], top), use = now == -INFINITY ? 0.f : now, corr = exp2f(m[i] - use);
-            m[i] = now;
+            for (int y = 8; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            const float now = fmaxf(m[x], top), use = now == -INFINITY ? 0.f : now, corr = exp2f(m[x] - use);
+            m[x] = now;
             float sum = 0.f;
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
-                const float p = exp2f(s[i][k] - use);
+                const float p = exp2f(s[x][k] - use);
                 sum += p;
-                ps[(c + k * 16) * (RT + 4) + rg * 4 + i] = p;
+                ps[(c + k * 16) * (RT + 4) + rg * R + x] = p;
             }
-            l[i] = l[i] * corr + sum;
+            l[x] = l[x] * corr + sum;
 #pragma unroll
-            for (int d = 0; d < NV * VEC; ++d) o[i][d] *= corr;
+            for (int d = 0; d < NV * VEC; ++d) o[x][d] *= corr;
         }
         __syncwarp();                          // a half-warp writes and reads the columns of its own rows alone
 #pragma unroll 4
         for (int k = 0; k < KT; ++k) {
-            const float4 p = *reinterpret_cast<const float4*>(ps + k * (RT + 4) + rg * 4);
+            float p[R];
+#pragma unroll
+            for (int x = 0; x < R; x += 2) {
+                const float2 w = *reinterpret_cast<const float2*>(ps + k * (RT + 4) + rg * R + x);
+                p[x] = w.x, p[x + 1] = w.y;
+            }
 #pragma unroll
             for (int g = 0; g < NV; ++g) {
                 float v[VEC];
@@ -165,43 +316,27 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
                     v[0] = w.x, v[1] = w.y;
                 }
 #pragma unroll
-                for (int x = 0; x < VEC; ++x) {
-                    o[0][g * VEC + x] = fmaf(p.x, v[x], o[0][g * VEC + x]);
-                    o[1][g * VEC + x] = fmaf(p.y, v[x], o[1][g * VEC + x]);
-                    o[2][g * VEC + x] = fmaf(p.z, v[x], o[2][g * VEC + x]);
-                    o[3][g * VEC + x] = fmaf(p.w, v[x], o[3][g * VEC + x]);
-                }
+                for (int x = 0; x < R; ++x)
+#pragma unroll
+                    for (int y = 0; y < VEC; ++y) o[x][g * VEC + y] = fmaf(p[x], v[y], o[x][g * VEC + y]);
             }
         }
     }
+    if constexpr (FAST) cp_async_wait<0>();
+    __syncthreads();                           // the queries' and the weights' places are free
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int x = 0; x < R; ++x) {
 #pragma unroll
-        for (int x = 8; x > 0; x >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
-        const int row = t.tile * RT + rg + i * 8;
-        if (row >= rows) continue;
-        const long long gr = (long long)(t.t_base + row / G) * a.nh + t.kvh * G + row % G;
-        if (a.nsplit > 1) {
-            float* dst = a.part_o + ((long long)t.split * a.T * a.nh + gr) * hd;
+        for (int y = 8; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
+        const int r = rg + x * 8;
 #pragma unroll
-            for (int g = 0; g < NV; ++g)
+        for (int g = 0; g < NV; ++g)
 #pragma unroll
-                for (int x = 0; x < VEC; ++x)
-                    if ((g * 16 + c) * VEC + x < hd) dst[(g * 16 + c) * VEC + x] = o[i][g * VEC + x];
-            if (c == 0) {
-                float* ml = a.part_ml + ((long long)t.split * a.T * a.nh + gr) * 2;
-                ml[0] = m[i], ml[1] = l[i];
-            }
-        } else {
-            const float inv = l[i] > 0.f ? 1.f / l[i] : l[i];          // 0 where nothing is seen; NaN stays
-            T* dst = static_cast<T*>(a.out) + gr * hd;
-#pragma unroll
-            for (int g = 0; g < NV; ++g)
-#pragma unroll
-                for (int x = 0; x < VEC; ++x)
-                    if ((g * 16 + c) * VEC + x < hd) dst[(g * 16 + c) * VEC + x] = from_float<T>(o[i][g * VEC + x] * inv);
-        }
+            for (int y = 0; y < VEC; ++y) qs[r * LD + (g * 16 + c) * VEC + y] = o[x][g * VEC + y];
+        if (c == 0) ps[r * 2] = m[x], ps[r * 2 + 1] = l[x];
     }
+    __syncthreads();
+    finish_rows<T, CL>(a, t, tree, qs, LD, ps, RT, row0);
 }
 
 // ---------------------------------------------------------------- bfloat16, head sizes 32, 64, 96, 128: mma.sync
@@ -217,7 +352,7 @@ struct MmaTile {
     static_assert(4 * 16 * (HD + 2) * 4 <= ST * 2 * KV, "the warps' outputs must fit the ring");
 };
 
-template <int HD, int RG>
+template <int HD, int RG, bool CL>
 __global__ void __launch_bounds__(128)
 attention_tree_mma_kernel(const TreeArgs a) {
     using L = MmaTile<HD, RG>;
@@ -390,7 +525,7 @@ attention_tree_mma_kernel(const TreeArgs a) {
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 1);
     l_b += __shfl_xor_sync(0xffffffffu, l_b, 2);
 
-    // the warps' results meet in shared memory, where the ring was; 16 lanes of a warp then write a row together
+    // the warps' results meet in shared memory, where the ring was
     __syncthreads();
     float* o_s = reinterpret_cast<float*>(kv_s);                                       // [4][16][HD]
     float* ml_s = o_s + 4 * 16 * HD;                                                   // [4][16][2]
@@ -408,37 +543,35 @@ attention_tree_mma_kernel(const TreeArgs a) {
         }
     }
     __syncthreads();
-    for (int r = threadIdx.x >> 4; r < L::RT; r += 8) {
-        const int row = row0 + r, c = threadIdx.x & 15;
-        if (row >= rows) break;
-        const bool seen = tree.depth[row / G] >= 0;
-        float M = -INFINITY;
-#pragma unroll
-        for (int g = 0; g < KG; ++g) M = fmaxf(M, ml_s[((g * RG + r / 16) * 16 + r % 16) * 2]);
-        const float use = M == -INFINITY ? 0.f : M;
-        float f[KG], l = 0.f;
-#pragma unroll
-        for (int g = 0; g < KG; ++g) {
-            const float* ml = ml_s + ((g * RG + r / 16) * 16 + r % 16) * 2;
-            f[g] = exp2f(ml[0] - use);
-            l += f[g] * ml[1];
-        }
-        const long long gr = (long long)(t.t_base + row / G) * a.nh + t.kvh * G + row % G;
-        const float inv = !seen || l == 0.f ? 0.f : 1.f / l;
-        if (a.nsplit > 1 && c == 0)
-            *reinterpret_cast<float2*>(a.part_ml + ((long long)t.split * a.T * a.nh + gr) * 2) = seen ? make_float2(M, l) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-        for (int d = c * 2; d < HD; d += 32) {
-            float2 acc = make_float2(0.f, 0.f);
+    if constexpr (KG > 1) {
+        // the warps that took the same rows, into the place of the first of them: [RT][HD]
+        for (int r = threadIdx.x >> 4; r < L::RT; r += 8) {
+            float2 ml[KG];
+            float M = -INFINITY, f[KG], l = 0.f;
 #pragma unroll
             for (int g = 0; g < KG; ++g) {
-                const float2 v = *reinterpret_cast<const float2*>(o_s + ((g * RG + r / 16) * 16 + r % 16) * HD + d);
-                acc.x = fmaf(f[g], v.x, acc.x), acc.y = fmaf(f[g], v.y, acc.y);
+                ml[g] = *reinterpret_cast<const float2*>(ml_s + (g * L::RT + r) * 2);
+                M = fmaxf(M, ml[g].x);
             }
-            if (a.nsplit > 1) *reinterpret_cast<float2*>(a.part_o + ((long long)t.split * a.T * a.nh + gr) * HD + d) = seen ? acc : make_float2(0.f, 0.f);
-            else *reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(a.out) + gr * HD + d) = seen ? pack_bf16(acc.x * inv, acc.y * inv) : 0u;
+            const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int g = 0; g < KG; ++g) f[g] = exp2f(ml[g].x - use), l += f[g] * ml[g].y;
+            __syncwarp();
+            if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(ml_s + r * 2) = make_float2(M, l);
+#pragma unroll
+            for (int d = (threadIdx.x & 15) * 2; d < HD; d += 32) {
+                float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int g = 0; g < KG; ++g) {
+                    const float2 v = *reinterpret_cast<const float2*>(o_s + (g * L::RT + r) * HD + d);
+                    acc.x = fmaf(f[g], v.x, acc.x), acc.y = fmaf(f[g], v.y, acc.y);
+                }
+                *reinterpret_cast<float2*>(o_s + r * HD + d) = acc;
+            }
         }
+        __syncthreads();
     }
+    finish_rows<__nv_bfloat16, CL>(a, t, tree, o_s, HD, ml_s, L::RT, row0);
 }
 
 // The pieces of a row merged in their order: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A warp takes a row.
@@ -467,16 +600,52 @@ attention_tree_merge_kernel(T* __restrict__ out, const float* __restrict__ part_
     }
 }
 
+// A grid of 128 threads a block; in_cluster: the pieces of a tile are one cluster (they are neighbours in the grid).
+template <typename... KArgs, typename... Args>
+int launch_tiles(std::atomic<unsigned long long>& allowed, void (*kernel)(KArgs...), const TreeArgs& a, bool in_cluster, size_t smem, cudaStream_t stream, Args... args) {
+    cudaError_t e = cellm_allow_smem(allowed, (const void*)kernel, smem);
+    if (e != cudaSuccess) return (int)e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)a.B * a.nkv * a.tiles * a.nsplit));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.nsplit;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = in_cluster ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, kernel, a, args...);
+    return e == cudaSuccess ? CELLM_OK : (int)e;
+}
+// Up to this many pieces meet in a cluster.
+constexpr int CLUSTER_MAX = 8;
+
+template <typename T, int HDP, int R, bool FAST>
+int launch_plain_rows(TreeArgs a, int quads, cudaStream_t stream) {
+    using L = PlainTile<HDP, R, FAST>;
+    static std::atomic<unsigned long long> allowed[2];
+    a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
+    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_plain_kernel<T, HDP, R, FAST, true>, a, true, L::bytes, stream, quads)
+                                                   : launch_tiles(allowed[0], attention_tree_plain_kernel<T, HDP, R, FAST, false>, a, false, L::bytes, stream, quads);
+}
+// Rows of 32-bit tiles: 48 where that leaves the last tile fuller than 32 would, 16 for the smallest trees.
+int plain_rows(int rows) { return rows <= 16 ? 16 : rows % 32 == 0 || rows <= 32 || (rows + 47) / 48 * 48 > (rows + 31) / 32 * 32 ? 32 : 48; }
 template <typename T, int HDP>
 int launch_plain(const TreeArgs& a, cudaStream_t stream) {
-    constexpr int KT = PlainTile<HDP>::KEYS, LD = HDP + 4;
-    const size_t smem = sizeof(TreeShape) + (size_t)((32 + 2 * KT) * LD + KT * 36) * 4;
-    cudaError_t e = cudaFuncSetAttribute(attention_tree_plain_kernel<T, HDP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool;
     const int quads = a.hd % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && at % (4 * sizeof(T)) == 0;
-    CELLM_RUN((attention_tree_plain_kernel<T, HDP>), (unsigned)((long long)a.B * a.nkv * a.nsplit * a.tiles), 128, smem, stream, a, quads);
-    return CELLM_OK;
+    if constexpr (sizeof(T) == 4) {
+        if (quads) {
+            const int rows = plain_rows(a.most * (a.nh / a.nkv));
+            return rows == 16 ? launch_plain_rows<T, HDP, 2, true>(a, 1, stream) : rows == 32 ? launch_plain_rows<T, HDP, 4, true>(a, 1, stream)
+                                                                                              : launch_plain_rows<T, HDP, 6, true>(a, 1, stream);
+        }
+    }
+    return launch_plain_rows<T, HDP, 4, false>(a, quads, stream);
 }
 
 template <typename T>
@@ -491,11 +660,10 @@ int launch_plain_sized(const TreeArgs& a, cudaStream_t stream) {
 template <int HD, int RG>
 int launch_mma(TreeArgs a, cudaStream_t stream) {
     using L = MmaTile<HD, RG>;
-    cudaError_t e = cudaFuncSetAttribute(attention_tree_mma_kernel<HD, RG>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::bytes);
-    if (e != cudaSuccess) return (int)e;
+    static std::atomic<unsigned long long> allowed[2];
     a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
-    CELLM_RUN((attention_tree_mma_kernel<HD, RG>), (unsigned)((long long)a.B * a.nkv * a.nsplit * a.tiles), 128, L::bytes, stream, a);
-    return CELLM_OK;
+    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_mma_kernel<HD, RG, true>, a, true, L::bytes, stream)
+                                                   : launch_tiles(allowed[0], attention_tree_mma_kernel<HD, RG, false>, a, false, L::bytes, stream);
 }
 template <int HD>
 int launch_mma_rows(const TreeArgs& a, cudaStream_t stream) {
@@ -507,16 +675,7 @@ bool mma_takes(const TreeArgs& a) {
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
     return (a.hd == 32 || a.hd == 64 || a.hd == 96 || a.hd == 128) && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0;
 }
-// Trees that fill tiles of 128 rows go to the tcgen05 kernel.
-bool tc_rows(int rows) { return rows > 64; }
-int launch_bf16(const TreeArgs& a, cudaStream_t stream) {
-    const int G = a.nh / a.nkv;
-    if (tc_rows(a.most * G) && attention_tree_tc_takes(a) && (a.most > 128 / G || a.nsplit % 2 == 0)) {
-        TreeArgs b = a;
-        if (a.most <= 128 / G) b.nsplit /= 2;               // its two tiles leave a piece each
-        return attention_tree_tc_launch(b, stream);
-    }
-    if (!mma_takes(a)) return launch_plain_sized<__nv_bfloat16>(a, stream);
+int launch_mma_sized(const TreeArgs& a, cudaStream_t stream) {
     if (a.hd == 32) return launch_mma_rows<32>(a, stream);
     if (a.hd == 64) return launch_mma_rows<64>(a, stream);
     if (a.hd == 96) return launch_mma_rows<96>(a, stream);
@@ -524,64 +683,90 @@ int launch_bf16(const TreeArgs& a, cudaStream_t stream) {
 }
 
 // How many pieces the keys of a tile of rows are cut into: of all counts the one whose rounds of blocks, each as long as its keys
-// and a few blocks' worth of start and merge, take the least time.
-int pieces(long long tiles, int key_blocks, long long at_once) {
+// and a few blocks' worth of start and merge, take the least time. Up to CLUSTER_MAX pieces merge at the cost of one block (where they
+// may be a cluster), more at that of a launch.
+int pieces(long long tiles, int key_blocks, long long at_once, bool clusters) {
     constexpr int START = 3;
     int best = 1;
     long long least = LLONG_MAX;
     for (int n = 1; n <= 64 && n <= std::max(1, key_blocks); ++n) {
-        const long long cost = (tiles * n + at_once - 1) / at_once * ((key_blocks + n - 1) / n + START) + (n > 1 ? START : 0);
+        const long long cost = (tiles * n + at_once - 1) / at_once * ((key_blocks + n - 1) / n + START) + (n == 1 ? 0 : clusters && n <= CLUSTER_MAX ? 1 : START);
         if (cost < least) least = cost, best = n;
     }
     return best;
 }
 
+// Trees of more rows than this fill tiles of 128 rows well enough for the tcgen05 kernel.
+constexpr int TC_ROWS = 64;
+
+struct TreePlan {
+    bool tc;            // for the tcgen05 kernel, if it takes the call
+    int nsplit;         // pieces a tile's keys are cut into
+    int parts;          // pieces that meet in the workspace (a tree of one tcgen05 tile leaves two a CTA); 0: none do
+};
+TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
+    const int G = nh / nkv, rows = most * G;
+    if (dtype == CELLM_BF16 && hd == 64 && rows > TC_ROWS && G <= 128 && 128 / G * G >= 96) {
+        const int tile = 128 / G, two = most > tile;
+        const int n = pieces((long long)B * nkv * ((most + (1 + two) * tile - 1) / ((1 + two) * tile)), ((keys + 127) / 128 + 1 - two) / (2 - two), sms, false);
+        return {true, n, two ? (n > 1 ? n : 0) : 2 * n};
+    }
+    const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
+    const int tile = mma ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : dtype == CELLM_F32 ? plain_rows(rows) : 32;
+    const int an_sm = hd <= 32 ? (mma ? 4 : 3) : mma && hd == 64 ? 3 : 2;     // blocks that an SM holds, by their shared memory
+    const int block = mma || hd <= 64 ? 64 : hd <= 128 ? 32 : 16;
+    const int n = pieces((long long)B * nkv * ((rows + tile - 1) / tile), (keys + block - 1) / block, (long long)an_sm * sms, true);
+    return {false, n, n > CLUSTER_MAX ? n : 0};
+}
+
 template <typename T>
-int launch_merge(const TreeArgs& a, cudaStream_t stream) {
+int launch_merge(const TreeArgs& a, int parts, cudaStream_t stream) {
     const long long rows = (long long)a.T * a.nh;
-    CELLM_RUN(attention_tree_merge_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, stream, (T*)a.out, a.part_o, a.part_ml, rows, a.hd, a.nsplit);
+    CELLM_RUN(attention_tree_merge_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, stream, (T*)a.out, a.part_o, a.part_ml, rows, a.hd, parts);
     return CELLM_OK;
 }
 
 }  // namespace
 
-// The pieces the keys are best cut into: B trees of up to `most` nodes, `keys` the most that a node sees.
-CELLM_API int cellm_attention_tree_pieces(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
+// How a call of these sizes is best run (`keys`: the most that a node sees): the pieces that a tile's keys are cut into, and 65,536 times
+// the pieces that meet in the workspace.
+CELLM_API int cellm_attention_tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
     if (B <= 0 || most <= 0 || nkv <= 0 || nh < nkv) return 1;
-    const int G = nh / nkv, rows = most * G;
-    if (dtype == CELLM_BF16 && hd == 64 && tc_rows(rows) && G <= 128 && 128 / G * G >= 96) {
-        const int tile = 128 / G, two = most > tile;
-        const int n = pieces((long long)B * nkv * ((most + (1 + two) * tile - 1) / ((1 + two) * tile)), ((keys + 127) / 128 + 1 - two) / (2 - two), sms);
-        return two ? n : 2 * n;
-    }
-    const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
-    const int tile = !mma || (rows > 16 && rows <= 32) ? 32 : rows <= 16 ? 16 : 64;
-    const int an_sm = !mma ? 2 : hd == 32 ? 4 : hd == 64 ? 3 : 2;             // blocks that an SM holds, by their shared memory
-    return pieces((long long)B * nkv * ((rows + tile - 1) / tile), (keys + 63) / 64, (long long)an_sm * sms);
+    const TreePlan p = tree_plan(B, most, nh, nkv, hd, keys, dtype, sms);
+    return p.nsplit | p.parts << 16;
 }
 
 // out [T, nh * hd], q rows q_ld elements apart, the nodes' keys and values in rows k_ld and v_ld apart ([nkv * hd] each), parents
 // [T]; request b owns the nodes cu_seqlens[b] .. cu_seqlens[b + 1] (at most 256, `most` of them in the largest tree) behind
-// ctx_lens[b] committed tokens in the pages of its row of the block table. nsplit pieces of the keys need part_o [nsplit, T * nh,
-// hd] and part_ml [nsplit, T * nh, 2] floats.
+// ctx_lens[b] committed tokens in the pages of its row of the block table. nsplit and parts as planned: part_o [parts, T * nh, hd]
+// and part_ml [parts, T * nh, 2] floats.
 CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, const void* q, long long q_ld, const void* k_new, long long k_ld,
                                    const void* v_new, long long v_ld, const int* parents, const void* k_pool, const void* v_pool,
                                    const int* cu_seqlens, const int* ctx_lens, const int* block_table, int bt_stride, int B, int T, int most,
-                                   int num_pages, int page_size, int nh, int nkv, int hd, float scale, int window, int nsplit, int dtype, int* err,
+                                   int num_pages, int page_size, int nh, int nkv, int hd, float scale, int window, int nsplit, int parts, int dtype, int* err,
                                    cudaStream_t stream) {
     if (T <= 0 || B <= 0 || most <= 0) return CELLM_OK;
     if (dtype != CELLM_F32 && dtype != CELLM_BF16) return CELLM_ERR_DTYPE;
     if (nkv <= 0 || nh <= 0 || nh % nkv || hd <= 0 || hd > 256 || page_size <= 0 || most > TREE_MAX || bt_stride < 0 || window < 0) return CELLM_ERR_SIZE;
-    if (nsplit < 1 || nsplit > 128) return CELLM_ERR_SIZE;
-    if (nsplit > 1 && (!part_o || !part_ml)) return CELLM_ERR_ARG;
+    if (nsplit < 1 || nsplit > 64 || parts < 0) return CELLM_ERR_SIZE;
+    if (parts > 0 && (!part_o || !part_ml)) return CELLM_ERR_ARG;
     if (!out || !q || !k_new || !v_new || !parents || !cu_seqlens || !ctx_lens || !err) return CELLM_ERR_ARG;
+    if ((((uintptr_t)part_o) & 15) || (((uintptr_t)part_ml) & 7)) return CELLM_ERR_ALIGN;
     TreeArgs a = {out, part_o, part_ml, q, k_new, v_new, q_ld, k_ld, v_ld, parents, k_pool, v_pool, cu_seqlens, ctx_lens, block_table,
                   bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, 0, nsplit, window, scale * 1.4426950408889634f, err};
-    a.tiles = (most * (nh / nkv) + 31) / 32;
-    if ((long long)B * nkv * nsplit * a.tiles > 0x7fffffffLL) return CELLM_ERR_SIZE;
-    int rc = dtype == CELLM_F32 ? launch_plain_sized<float>(a, stream) : launch_bf16(a, stream);
-    if (rc != CELLM_OK || nsplit == 1) return rc;
-    return dtype == CELLM_F32 ? launch_merge<float>(a, stream) : launch_merge<__nv_bfloat16>(a, stream);
+    const int G = nh / nkv;
+    if ((long long)B * nkv * 64 * ((most * G + 15) / 16) > 0x7fffffffLL) return CELLM_ERR_SIZE;
+    if (dtype == CELLM_BF16 && most * G > TC_ROWS && attention_tree_tc_takes(a)) {
+        const int need = most <= 128 / G ? 2 * nsplit : nsplit > 1 ? nsplit : 0;
+        if (parts >= need) {
+            const int rc = attention_tree_tc_launch(a, stream);
+            return rc != CELLM_OK || need == 0 ? rc : launch_merge<__nv_bfloat16>(a, need, stream);
+        }
+    }
+    if (nsplit > CLUSTER_MAX && parts < nsplit) a.nsplit = CLUSTER_MAX;
+    const int rc = dtype == CELLM_F32 ? launch_plain_sized<float>(a, stream) : mma_takes(a) ? launch_mma_sized(a, stream) : launch_plain_sized<__nv_bfloat16>(a, stream);
+    if (rc != CELLM_OK || a.nsplit <= CLUSTER_MAX) return rc;
+    return dtype == CELLM_F32 ? launch_merge<float>(a, a.nsplit, stream) : launch_merge<__nv_bfloat16>(a, a.nsplit, stream);
 }
 
 // The same with its arguments in order as 64-bit words (see common.cuh).
@@ -589,5 +774,5 @@ CELLM_API int cellm_attention_tree_packed(const long long* a, cudaStream_t strea
     return cellm_attention_tree((void*)a[0], (float*)a[1], (float*)a[2], (const void*)a[3], (long long)a[4], (const void*)a[5], (long long)a[6],
         (const void*)a[7], (long long)a[8], (const int*)a[9], (const void*)a[10], (const void*)a[11], (const int*)a[12], (const int*)a[13],
         (const int*)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], (int)a[23],
-        (float)cellm_packed_double(a[24]), (int)a[25], (int)a[26], (int)a[27], (int*)a[28], stream);
+        (float)cellm_packed_double(a[24]), (int)a[25], (int)a[26], (int)a[27], (int)a[28], (int*)a[29], stream);
 }

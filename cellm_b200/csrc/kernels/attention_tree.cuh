@@ -30,8 +30,8 @@ struct TreeTile {
 __device__ __forceinline__ TreeTile tree_tile(const TreeArgs& a) {
     TreeTile t;
     int i = blockIdx.x;
-    t.tile = i % a.tiles, i /= a.tiles;
     t.split = i % a.nsplit, i /= a.nsplit;
+    t.tile = i % a.tiles, i /= a.tiles;
     t.kvh = i % a.nkv;
     t.b = i / a.nkv;
     t.t_base = a.cu_seqlens[t.b];
@@ -53,9 +53,10 @@ __device__ __forceinline__ TreeTile tree_tile(const TreeArgs& a) {
 // Which of a block's KT keys a node sees, a bit a key: committed ones from position key0 on, or (node0 >= 0) the nodes from node0 on.
 template <int KT>
 __device__ __forceinline__ uint64_t seen_bits(const TreeShape& tree, int node, int window, int ctx, int key0, int node0) {
-    static_assert(KT == 32 || KT == 64, "");
+    static_assert(KT == 16 || KT == 32 || KT == 64, "a power of two of keys");
     if (node0 >= 0) {
         uint64_t m = tree.line[node][node0 >> 5];
+        if (KT == 16) m >>= node0 & 31;
         if (KT == 64 && (node0 >> 5) + 1 < TREE_WORDS) m |= (uint64_t)tree.line[node][(node0 >> 5) + 1] << 32;
         return m;
     }

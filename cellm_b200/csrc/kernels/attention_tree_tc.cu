@@ -86,7 +86,7 @@ __device__ __forceinline__ bool elect_one() {
     return is != 0;
 }
 
-// grid: (request, key/value head, piece, pair of tiles), the last fastest. alternate: one tile of rows, whose blocks the two tiles take
+// grid: (request, key/value head, pair of tiles, piece), the last fastest. alternate: one tile of rows, whose blocks the two tiles take
 // in turn; piece 2 * split + tile.
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -419,7 +419,8 @@ int attention_tree_tc_launch(const TreeArgs& given, cudaStream_t stream) {
     if (!encode(&mk, a.k_pool, 2, dims, strides, box) || !encode(&mv, a.v_pool, 2, dims, strides, box) || !encode_rows(&mq, a.q, a.T, a.nh, a.q_ld, G, tile_nodes) ||
         !encode_rows(&mkn, a.k_new, a.T, a.nkv, a.k_ld, 1, TN) || !encode_rows(&mvn, a.v_new, a.T, a.nkv, a.v_ld, 1, TN))
         return CELLM_ERR_ARG;
-    cudaError_t e = cudaFuncSetAttribute(attention_tree_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(TreeTcSmem));
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = cellm_allow_smem(allowed, (const void*)attention_tree_tc_kernel, sizeof(TreeTcSmem));
     if (e != cudaSuccess) return (int)e;
     const int pair = alternate ? tile_nodes : 2 * tile_nodes;
     a.tiles = (a.most + pair - 1) / pair;

@@ -580,7 +580,8 @@ int launch_select(float* out_scores, int* out_parents, int* out_tokens, float* t
     const long long all = (long long)requests * beams * parts;
     const unsigned blocks = (unsigned)std::min<long long>((all + ROW_WARPS - 1) / ROW_WARPS, (long long)Ring<T>::BLOCKS * sms);
     const size_t smem = ROW_WARPS * sizeof(Ring<T>);
-    cudaError_t e = cudaFuncSetAttribute(beam_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = cellm_allow_smem(allowed, (const void*)beam_rows_kernel<T>, smem);
     if (e != cudaSuccess) return (int)e;
     CELLM_RUN(beam_rows_kernel<T>, blocks, ROW_WARPS * 32, smem, stream, tops, (RowPart*)sums, (const T*)logits, ld, V, parts, requests * beams, done);
     CELLM_RUN(beam_pick_kernel<T>, requests, PICK_THREADS, HOT_ROOM * sizeof(uint32_t), stream, out_scores, out_parents, out_tokens, tops, (const RowPart*)sums, (const T*)logits, ld, V,

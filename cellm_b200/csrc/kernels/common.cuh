@@ -4,6 +4,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdlib>
 #include <cstring>
 #include <utility>
@@ -215,6 +216,18 @@ template <typename... KArgs, typename... Args>
 inline cudaError_t cellm_launch_serial(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                                        Args&&... args) {
     return cellm_launch_with(0, kernel, grid, block, smem, stream, std::forward<Args>(args)...);
+}
+
+// Lets a kernel use more than 48 KB of shared memory, once a device (the attribute's call costs a microsecond). `done` is a static of
+// the caller's, a bit a device.
+inline cudaError_t cellm_allow_smem(std::atomic<unsigned long long>& done, const void* kernel, size_t bytes) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    if (device < 64 && (done.load(std::memory_order_relaxed) >> device & 1ull)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && device < 64) done.fetch_or(1ull << device, std::memory_order_relaxed);
+    return e;
 }
 
 #define CELLM_RUN(kernel, grid, block, smem, stream, ...)                                   \

@@ -118,8 +118,8 @@ _SIGNATURES = {
         "cellm_decay_chunks_supports": [I, I],
     },
     "attention_tree": {
-        "cellm_attention_tree_pieces": [I, I, I, I, I, I, I, I],
-        "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, P, P],
+        "cellm_attention_tree_plan": [I, I, I, I, I, I, I, I],
+        "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, P, P],
     },
     "candidates": {
         "cellm_accept_drafts": [P, P, P, P, P, P, P, I, I, I, P, L, L, I, P, P, L, L, I, P, P, P, I, I, I, I, I, P, P],

@@ -18,13 +18,13 @@ def call(library, name, *args):
 
 
 def test_attention_of_trees():
-    def tree(out=A, part=None, q=A, parents=A, cu=A, T=8, B=2, most=5, page=16, nh=4, nkv=2, hd=64, window=0, nsplit=1, dtype=1, err=A):
+    def tree(out=A, part=None, q=A, parents=A, cu=A, T=8, B=2, most=5, page=16, nh=4, nkv=2, hd=64, window=0, nsplit=1, parts=0, dtype=1, err=A):
         return call("attention_tree", "cellm_attention_tree", out, part, part, q, nh * hd, A, nkv * hd, A, nkv * hd, parents, A, A, cu, A, A, 4, B, T, most, 8, page, nh, nkv,
-                    hd, 0.125, window, nsplit, dtype, err, None)
+                    hd, 0.125, window, nsplit, parts, dtype, err, None)
     assert tree(dtype=2) == DTYPE and tree(dtype=-1) == DTYPE
-    for bad in (dict(nh=5), dict(nkv=0), dict(nh=0), dict(hd=0), dict(hd=257), dict(page=0), dict(most=257), dict(window=-1), dict(nsplit=0), dict(nsplit=129, part=A)):
+    for bad in (dict(nh=5), dict(nkv=0), dict(nh=0), dict(hd=0), dict(hd=257), dict(page=0), dict(most=257), dict(window=-1), dict(nsplit=0), dict(nsplit=65, part=A), dict(parts=-1)):
         assert tree(**bad) == SIZE, bad
-    assert tree(nsplit=2) == ARG and tree(out=None) == ARG and tree(parents=None) == ARG and tree(err=None) == ARG
+    assert tree(nsplit=2, parts=2) == ARG and tree(parts=2, part=A + 4) == ALIGN and tree(out=None) == ARG and tree(parents=None) == ARG and tree(err=None) == ARG
     assert tree(T=0) == 0 and tree(B=0) == 0 and tree(most=0) == 0
 
 
