@@ -21,6 +21,8 @@ def main(argv=None) -> int:
     ap.add_argument("--repeat-penalty", type=float, default=1.05, help="repetition penalty (1.0 disables)")
     ap.add_argument("--repeat-window", type=int, default=64, help="recent token window for the penalty")
     ap.add_argument("--tokens", help="comma-separated token ids (overrides --seq)")
+    ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams (0: sampling or greedy); prints every beam, best first")
+    ap.add_argument("--length-penalty", type=float, default=1.0, help="beams are ranked by log probability / length ** this")
     ap.add_argument("--stop-eos", type=lambda s: s.lower() not in ("0", "false", "no"), default=True,
                     help="stop when the EOS token is produced")
     args = ap.parse_args(argv)
@@ -39,10 +41,19 @@ def main(argv=None) -> int:
         prompt = parse_tokens(args.tokens)
     else:
         prompt = list(range(args.seq))
-    blocks = args.total_blocks or default_blocks(len(prompt), args.gen, args.tokens_per_block)
-    eng = Engine(folder, dtype=args.dtype, tokens_per_block=args.tokens_per_block, total_blocks=blocks, max_num_seqs=1)
+    blocks = args.total_blocks or default_blocks(len(prompt), args.gen, args.tokens_per_block, max(args.beams, 1))
+    eng = Engine(folder, dtype=args.dtype, tokens_per_block=args.tokens_per_block, total_blocks=blocks, max_num_seqs=max(args.beams, 1))
     eng.max_layers = args.max_layers
     print(f"Startup: {time.time() - t0:.2f}s  KV cache: blocks={blocks} tokens_per_block={args.tokens_per_block}")
+    if args.beams:
+        t1 = time.time()
+        found = eng.beam_search([prompt], args.beams, args.gen, args.length_penalty, args.stop_eos)[0]
+        print(f"Beam search: {len(found)} beams of up to {args.gen} tokens in {time.time() - t1:.2f}s")
+        for b in found:
+            print(f"beam {b.score:.4f}:", ",".join(str(t) for t in b.tokens))
+        if tok is not None:
+            print(tok.decode(found[0].tokens))
+        return 0
     seed = args.seed if args.seed is not None else (time.time_ns() & 0xFFFFFFFFFFFF)   # seed from the clock, as the reference
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, seed=seed,
                             repeat_penalty=args.repeat_penalty, repeat_window=args.repeat_window,

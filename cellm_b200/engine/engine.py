@@ -14,6 +14,7 @@ from ..cache.manager import CacheManager
 from ..config.engine_config import EngineConfig
 from ..models import load_model
 from ..sampling import RequestSampler, SamplingParams, sample_rows, session_seed
+from .beams import BeamOutput, beam_search
 from .scheduler import Scheduler
 from .step import StepRunner
 
@@ -238,6 +239,15 @@ class Engine:
             if o.finish_reason == "out_of_pages":
                 raise RuntimeError(f"request {o.request_id} could not fit the cache pool")
         return [o.tokens for o in outs]
+
+    def beam_search(self, prompts: Sequence[Sequence[int]], beams: int = 4, max_new_tokens: int = 16, length_penalty: float = 1.0,
+                    stop_eos: bool = True) -> list[list[BeamOutput]]:
+        """The best `beams` continuations of each prompt, best first: in every step the beams of a prompt that have the highest sums of log
+        probabilities go on, and one that chose the end-of-sequence token (with `stop_eos`) stands as it is. The final order is by that
+        sum divided by length ** length_penalty. Fewer than `beams` come back where there are no more. Every beam takes a state slot and
+        pages of its own (len(prompts) * beams <= max_num_seqs); OutOfPages where the pool is too small. The engine must have no
+        unfinished requests."""
+        return beam_search(self, prompts, beams, max_new_tokens, length_penalty, stop_eos)
 
     def stats(self) -> dict:
         """crates/cellm-sdk/src/lib.rs:495-502: active sessions and used / free pages."""
