@@ -574,29 +574,51 @@ attention_tree_mma_kernel(const TreeArgs a) {
     finish_rows<__nv_bfloat16, CL>(a, t, tree, o_s, HD, ml_s, L::RT, row0);
 }
 
-// The pieces of a row merged in their order: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. A warp takes a row.
+// The pieces of a row merged in their order: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s. 16 threads a row, which work out the
+// pieces' weights together and take two neighbouring entries (four where the rows allow it) of every piece.
 template <typename T>
 __global__ void __launch_bounds__(256)
 attention_tree_merge_kernel(T* __restrict__ out, const float* __restrict__ part_o, const float* __restrict__ part_ml, long long rows, int hd, int nsplit) {
     pdl_wait();
     pdl_trigger();
-    const long long r = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (r >= rows) return;
-    float M = -INFINITY;
-    for (int s = lane; s < nsplit; s += 32) M = fmaxf(M, part_ml[(s * rows + r) * 2]);
-    M = warp_max(M);
+    const long long r = min((long long)blockIdx.x * 16 + (threadIdx.x >> 4), rows - 1);       // (a row twice is written twice alike)
+    const int c = threadIdx.x & 15, group = threadIdx.x & 16;
+    float2 ml[4];
+    float M = -INFINITY, L = 0.f, w[4];
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        ml[g] = make_float2(-INFINITY, 0.f);
+        if (g * 16 + c < nsplit) ml[g] = *reinterpret_cast<const float2*>(part_ml + ((long long)(g * 16 + c) * rows + r) * 2);
+        M = fmaxf(M, ml[g].x);
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
     const float use = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    for (int s = 0; s < nsplit; ++s) L = fmaf(exp2f(part_ml[(s * rows + r) * 2] - use), part_ml[(s * rows + r) * 2 + 1], L);
-    const float inv = L > 0.f ? 1.f / L : L;
-    for (int d = lane; d < hd; d += 32) {
-        float acc = 0.f;
-        for (int s = 0; s < nsplit; ++s) {
-            const float w = exp2f(part_ml[(s * rows + r) * 2] - use);
-            if (w != 0.f) acc = fmaf(w, part_o[(s * rows + r) * hd + d], acc);       // (a piece that sees nothing holds zeros)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) w[g] = exp2f(ml[g].x - use), L = fmaf(w[g], ml[g].y, L);
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) L += __shfl_xor_sync(0xffffffffu, L, x);
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    const int quad = hd % 4 == 0 ? 4 : 1;
+    for (int d0 = 0; d0 < hd; d0 += 16 * quad) {
+        const int d = d0 + c * quad;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (g * 16 >= nsplit) break;
+#pragma unroll 8
+            for (int s = 0; s < min(16, nsplit - g * 16); ++s) {
+                const float f = __shfl_sync(0xffffffffu, w[g], group + s);
+                if (d >= hd) continue;
+                const float* src = part_o + ((long long)(g * 16 + s) * rows + r) * hd + d;
+                const float4 v = quad == 4 ? *reinterpret_cast<const float4*>(src) : make_float4(*src, 0.f, 0.f, 0.f);
+                if (f != 0.f) acc.x = fmaf(f, v.x, acc.x), acc.y = fmaf(f, v.y, acc.y), acc.z = fmaf(f, v.z, acc.z), acc.w = fmaf(f, v.w, acc.w);
+            }
         }
-        out[r * hd + d] = from_float<T>(acc * inv);
+        if (d >= hd) continue;
+        T* dst = out + r * hd + d;
+        dst[0] = from_float<T>(acc.x * inv);
+        if (quad == 4) dst[1] = from_float<T>(acc.y * inv), dst[2] = from_float<T>(acc.z * inv), dst[3] = from_float<T>(acc.w * inv);
     }
 }
 
@@ -702,14 +724,14 @@ constexpr int TC_ROWS = 64;
 struct TreePlan {
     bool tc;            // for the tcgen05 kernel, if it takes the call
     int nsplit;         // pieces a tile's keys are cut into
-    int parts;          // pieces that meet in the workspace (a tree of one tcgen05 tile leaves two a CTA); 0: none do
+    int parts;          // pieces that meet in the workspace; 0: none do
 };
 TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
     const int G = nh / nkv, rows = most * G;
     if (dtype == CELLM_BF16 && hd == 64 && rows > TC_ROWS && G <= 128 && 128 / G * G >= 96) {
         const int tile = 128 / G, two = most > tile;
         const int n = pieces((long long)B * nkv * ((most + (1 + two) * tile - 1) / ((1 + two) * tile)), ((keys + 127) / 128 + 1 - two) / (2 - two), sms, false);
-        return {true, n, two ? (n > 1 ? n : 0) : 2 * n};
+        return {true, n, n > 1 ? n : 0};
     }
     const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
     const int tile = mma ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : dtype == CELLM_F32 ? plain_rows(rows) : 32;
@@ -722,7 +744,7 @@ TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype
 template <typename T>
 int launch_merge(const TreeArgs& a, int parts, cudaStream_t stream) {
     const long long rows = (long long)a.T * a.nh;
-    CELLM_RUN(attention_tree_merge_kernel<T>, (unsigned)((rows + 7) / 8), 256, 0, stream, (T*)a.out, a.part_o, a.part_ml, rows, a.hd, parts);
+    CELLM_RUN(attention_tree_merge_kernel<T>, (unsigned)((rows + 15) / 16), 256, 0, stream, (T*)a.out, a.part_o, a.part_ml, rows, a.hd, parts);
     return CELLM_OK;
 }
 
@@ -757,7 +779,7 @@ CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, con
     const int G = nh / nkv;
     if ((long long)B * nkv * 64 * ((most * G + 15) / 16) > 0x7fffffffLL) return CELLM_ERR_SIZE;
     if (dtype == CELLM_BF16 && most * G > TC_ROWS && attention_tree_tc_takes(a)) {
-        const int need = most <= 128 / G ? 2 * nsplit : nsplit > 1 ? nsplit : 0;
+        const int need = nsplit > 1 ? nsplit : 0;
         if (parts >= need) {
             const int rc = attention_tree_tc_launch(a, stream);
             return rc != CELLM_OK || need == 0 ? rc : launch_merge<__nv_bfloat16>(a, need, stream);

@@ -5,7 +5,7 @@
 // block. Warps 0 and 2 bring queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P read from
 // tensor memory and V as its rows lie), warps 4..7 and 8..11 do the softmax of a tile each, a row a thread, so that one tile's products
 // run beside the other's softmax; they take the registers that the first warpgroup gives up. Trees of up to 128 rows have one tile: the same rows then stand in both, and the tiles take the
-// blocks in turn; their two results are two of the pieces that the merge joins.
+// blocks in turn; the second tile's result joins the first's through shared memory at the end.
 //
 // What it costs is exponentials: a block of 128 x 128 scores keeps the four special-function units of an SM 1,024 cycles, its
 // two products the tensor cores 512.
@@ -87,7 +87,7 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // grid: (request, key/value head, pair of tiles, piece), the last fastest. alternate: one tile of rows, whose blocks the two tiles take
-// in turn; piece 2 * split + tile.
+// in turn.
 __global__ void __launch_bounds__(THREADS, 1)
 attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                          const __grid_constant__ CUtensorMap map_kn, const __grid_constant__ CUtensorMap map_vn, const TreeArgs a, const int alternate) {
@@ -341,21 +341,53 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (ok && it > 0) ok = mbar_wait(&sm.pv_done[i], (uint32_t)(it - 1) & 1u, abort_flag);
         if (!ok && lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); }
-        if (ok) {
-            tc_fence_after();
+        tc_fence_after();
+        // One tile of rows: the second tile's results go to the first through the place of the keys, a row of 65 floats each (64 and
+        // the banks would be the same for all). Every warp meets at the barriers, whatever became of its waits.
+        float* room = reinterpret_cast<float*>(sm.k[0]);              // [TM][HD + 1], then [TM][2]
+        float w_own = 1.f, w_room = 0.f;
+        if (alternate) {
+            asm volatile("bar.sync 2, 256;" ::: "memory");            // all products are done
+            if (i == 1) {
+#pragma unroll 1
+                for (int c = 0; c < (it > 0 ? HD / 32 : 0); ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(lane_base + o_col + (uint32_t)(c * 32), o);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) room[r * (HD + 1) + c * 32 + k] = __uint_as_float(o[k]);
+                }
+                room[TM * (HD + 1) + r * 2] = it > 0 ? m : -INFINITY, room[TM * (HD + 1) + r * 2 + 1] = l;
+            }
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            if (i == 0) {
+                const float m_room = room[TM * (HD + 1) + r * 2], top = fmaxf(it > 0 ? m : -INFINITY, m_room), use = top == -INFINITY ? 0.f : top;
+                w_own = it > 0 ? exp2f(m - use) : 0.f, w_room = exp2f(m_room - use);
+                l = (it > 0 ? l * w_own : 0.f) + (w_room != 0.f ? room[TM * (HD + 1) + r * 2 + 1] * w_room : 0.f);
+                m = top;
+            }
+        }
+        if (ok && !(alternate && i == 1)) {
             const long long gr = (long long)(t.t_base + node) * a.nh + t.kvh * G + r % G;
-            const bool parted = alternate || a.nsplit > 1;
-            const long long piece = alternate ? t.split * 2 + i : t.split;
+            const bool parted = a.nsplit > 1, any = it > 0 || alternate;
+            const long long piece = t.split;
             const float inv = seeing && l != 0.f ? 1.0f / l : 0.f;
             if (parted && row_ok)
-                *reinterpret_cast<float2*>(a.part_ml + (piece * a.T * a.nh + gr) * 2) = it > 0 && seeing ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
+                *reinterpret_cast<float2*>(a.part_ml + (piece * a.T * a.nh + gr) * 2) = any && seeing ? make_float2(m, l) : make_float2(-INFINITY, 0.f);
 #pragma unroll 1
             for (int c = 0; c < HD / 32; ++c) {
                 uint32_t o[32];
                 if (it > 0) {
                     tmem_ld32(lane_base + o_col + (uint32_t)(c * 32), o);
                 }
-                if (!(it > 0 && seeing)) {
+                if (alternate) {
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        float v = w_own != 0.f ? __uint_as_float(o[k]) * w_own : 0.f;
+                        if (w_room != 0.f) v = fmaf(room[r * (HD + 1) + c * 32 + k], w_room, v);
+                        o[k] = __float_as_uint(v);
+                    }
+                }
+                if (!(any && seeing)) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k) o[k] = 0u;
                 }
@@ -408,7 +440,7 @@ bool attention_tree_tc_takes(const TreeArgs& a) {
            a.page_size >= 8 && a.page_size <= TN && (a.page_size & (a.page_size - 1)) == 0 && (long long)a.num_pages * a.nkv * a.page_size <= 0x7fffffffLL;
 }
 
-// part_o and part_ml hold a.nsplit pieces, twice as many where the tree's rows are one tile.
+// part_o and part_ml hold a.nsplit pieces where there are more than one.
 int attention_tree_tc_launch(const TreeArgs& given, cudaStream_t stream) {
     TreeArgs a = given;
     const int G = a.nh / a.nkv, tile_nodes = TM / G, alternate = a.most <= tile_nodes;
