@@ -718,8 +718,12 @@ int pieces(long long tiles, int key_blocks, long long at_once, bool clusters) {
     return best;
 }
 
-// Trees of more rows than this fill tiles of 128 rows well enough for the tcgen05 kernel.
-constexpr int TC_ROWS = 64;
+// Which trees of heads of 64 go to the tcgen05 kernel, whose tiles have 128 rows: those of more than 64 rows, and behind long contexts those
+// of more than 16. Microseconds of mma.sync and of tcgen05, 32 heads over 8, for 1, 8 and 32 trees:
+//   8 nodes (32 rows)    1,024 keys 10.0 12.0 | 12.7 15.3 | 33.9 30.5     4,096 keys 18.8 16.3 | 24.8 27.0 | 105 77
+//   12 nodes (48 rows)   1,024 keys 10.7 12.5 | 14.2 15.4 | 39.7 30.8     4,096 keys 21.3 17.1 | 30.9 27.3 | 127 77
+//   25 nodes (100 rows)  1,024 keys 12.3 12.9 | 21.8 15.6 | 76.2 31.2     4,096 keys 24.0 18.7 | 54.9 28.2 | 226 77
+bool tc_pays(int rows, int keys) { return rows > 64 || (rows > 16 && keys >= 2048); }
 
 struct TreePlan {
     bool tc;            // for the tcgen05 kernel, if it takes the call
@@ -728,7 +732,7 @@ struct TreePlan {
 };
 TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
     const int G = nh / nkv, rows = most * G;
-    if (dtype == CELLM_BF16 && hd == 64 && rows > TC_ROWS && G <= 128 && 128 / G * G >= 96) {
+    if (dtype == CELLM_BF16 && hd == 64 && tc_pays(rows, keys) && G <= 128 && 128 / G * G >= 96) {
         const int tile = 128 / G, two = most > tile;
         const int n = pieces((long long)B * nkv * ((most + (1 + two) * tile - 1) / ((1 + two) * tile)), ((keys + 127) / 128 + 1 - two) / (2 - two), sms, false);
         return {true, n, n > 1 ? n : 0};
@@ -750,22 +754,22 @@ int launch_merge(const TreeArgs& a, int parts, cudaStream_t stream) {
 
 }  // namespace
 
-// How a call of these sizes is best run (`keys`: the most that a node sees): the pieces that a tile's keys are cut into, and 65,536 times
-// the pieces that meet in the workspace.
+// How a call of these sizes is best run (`keys`: the most that a node sees), in three bytes: the pieces that a tile's keys are cut into, the
+// pieces that meet in the workspace, whether the tcgen05 kernel is to be taken.
 CELLM_API int cellm_attention_tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype, int sms) {
     if (B <= 0 || most <= 0 || nkv <= 0 || nh < nkv) return 1;
     const TreePlan p = tree_plan(B, most, nh, nkv, hd, keys, dtype, sms);
-    return p.nsplit | p.parts << 16;
+    return p.nsplit | p.parts << 8 | (p.tc ? 1 : 0) << 16;
 }
 
 // out [T, nh * hd], q rows q_ld elements apart, the nodes' keys and values in rows k_ld and v_ld apart ([nkv * hd] each), parents
 // [T]; request b owns the nodes cu_seqlens[b] .. cu_seqlens[b + 1] (at most 256, `most` of them in the largest tree) behind
-// ctx_lens[b] committed tokens in the pages of its row of the block table. nsplit and parts as planned: part_o [parts, T * nh, hd]
+// ctx_lens[b] committed tokens in the pages of its row of the block table. nsplit, parts and tc as planned: part_o [parts, T * nh, hd]
 // and part_ml [parts, T * nh, 2] floats.
 CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, const void* q, long long q_ld, const void* k_new, long long k_ld,
                                    const void* v_new, long long v_ld, const int* parents, const void* k_pool, const void* v_pool,
                                    const int* cu_seqlens, const int* ctx_lens, const int* block_table, int bt_stride, int B, int T, int most,
-                                   int num_pages, int page_size, int nh, int nkv, int hd, float scale, int window, int nsplit, int parts, int dtype, int* err,
+                                   int num_pages, int page_size, int nh, int nkv, int hd, float scale, int window, int nsplit, int parts, int tc, int dtype, int* err,
                                    cudaStream_t stream) {
     if (T <= 0 || B <= 0 || most <= 0) return CELLM_OK;
     if (dtype != CELLM_F32 && dtype != CELLM_BF16) return CELLM_ERR_DTYPE;
@@ -778,7 +782,7 @@ CELLM_API int cellm_attention_tree(void* out, float* part_o, float* part_ml, con
                   bt_stride, B, T, most, num_pages, page_size, nh, nkv, hd, 0, nsplit, window, scale * 1.4426950408889634f, err};
     const int G = nh / nkv;
     if ((long long)B * nkv * 64 * ((most * G + 15) / 16) > 0x7fffffffLL) return CELLM_ERR_SIZE;
-    if (dtype == CELLM_BF16 && most * G > TC_ROWS && attention_tree_tc_takes(a)) {
+    if (tc && dtype == CELLM_BF16 && attention_tree_tc_takes(a)) {
         const int need = nsplit > 1 ? nsplit : 0;
         if (parts >= need) {
             const int rc = attention_tree_tc_launch(a, stream);
@@ -796,5 +800,5 @@ CELLM_API int cellm_attention_tree_packed(const long long* a, cudaStream_t strea
     return cellm_attention_tree((void*)a[0], (float*)a[1], (float*)a[2], (const void*)a[3], (long long)a[4], (const void*)a[5], (long long)a[6],
         (const void*)a[7], (long long)a[8], (const int*)a[9], (const void*)a[10], (const void*)a[11], (const int*)a[12], (const int*)a[13],
         (const int*)a[14], (int)a[15], (int)a[16], (int)a[17], (int)a[18], (int)a[19], (int)a[20], (int)a[21], (int)a[22], (int)a[23],
-        (float)cellm_packed_double(a[24]), (int)a[25], (int)a[26], (int)a[27], (int)a[28], (int*)a[29], stream);
+        (float)cellm_packed_double(a[24]), (int)a[25], (int)a[26], (int)a[27], (int)a[28], (int)a[29], (int*)a[30], stream);
 }

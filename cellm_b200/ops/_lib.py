@@ -119,7 +119,7 @@ _SIGNATURES = {
     },
     "attention_tree": {
         "cellm_attention_tree_plan": [I, I, I, I, I, I, I, I],
-        "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, P, P],
+        "cellm_attention_tree": [P, P, P, P, L, P, L, P, L, P, P, P, P, P, P, I, I, I, I, I, I, I, I, I, F, I, I, I, I, I, P, P],
     },
     "candidates": {
         "cellm_accept_drafts": [P, P, P, P, P, P, P, I, I, I, P, L, L, I, P, P, L, L, I, P, P, P, I, I, I, I, I, P, P],

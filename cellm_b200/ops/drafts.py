@@ -16,7 +16,7 @@ from ._lib import DTYPE_TAG, dense_ints, fn, launch_packed
 from ._state import _SM_COUNT, sm_count
 
 MAX_TREE = 256                     # nodes of a tree (TREE_MAX in draft_tree.cuh)
-_TREE_ARGS, _ACCEPT_ARGS = Struct("24qd5q").pack, Struct("28q").pack
+_TREE_ARGS, _ACCEPT_ARGS = Struct("24qd6q").pack, Struct("28q").pack
 
 
 def _plan(*sizes) -> int:
@@ -81,7 +81,7 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     if 0 < window < keys:
         keys = window
     plan = _plan(B, most, nh, nkv, hd, keys + most, tag, _SM_COUNT.get(index) or sm_count(index))
-    nsplit, parts, part_o, part_ml = plan & 0xffff, plan >> 16, 0, 0
+    nsplit, parts, part_o, part_ml = plan & 0xff, plan >> 8 & 0xff, 0, 0
     if parts:
         ws = parents.new_empty(parts * T * nh * (hd + 2))              # of 32-bit words: the pieces' outputs, then maxima and sums
         part_o = ws.data_ptr()
@@ -89,7 +89,7 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     launch_packed("attention_tree", "attention_tree", index,
                   _TREE_ARGS(out.data_ptr(), part_o, part_ml, q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, parents.data_ptr(), k_pool.data_ptr(),
                              v_pool.data_ptr(), cu_seqlens.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), entries, B, T, most, pages, page_size, nh, nkv, hd,
-                             scale, window, nsplit, parts, tag, err.data_ptr()), 2 if parts else 1)
+                             scale, window, nsplit, parts, plan >> 16, tag, err.data_ptr()), 2 if parts else 1)
     return out
 
 

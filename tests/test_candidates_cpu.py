@@ -20,12 +20,31 @@ def call(library, name, *args):
 def test_attention_of_trees():
     def tree(out=A, part=None, q=A, parents=A, cu=A, T=8, B=2, most=5, page=16, nh=4, nkv=2, hd=64, window=0, nsplit=1, parts=0, dtype=1, err=A):
         return call("attention_tree", "cellm_attention_tree", out, part, part, q, nh * hd, A, nkv * hd, A, nkv * hd, parents, A, A, cu, A, A, 4, B, T, most, 8, page, nh, nkv,
-                    hd, 0.125, window, nsplit, parts, dtype, err, None)
+                    hd, 0.125, window, nsplit, parts, 1, dtype, err, None)
     assert tree(dtype=2) == DTYPE and tree(dtype=-1) == DTYPE
     for bad in (dict(nh=5), dict(nkv=0), dict(nh=0), dict(hd=0), dict(hd=257), dict(page=0), dict(most=257), dict(window=-1), dict(nsplit=0), dict(nsplit=65, part=A), dict(parts=-1)):
         assert tree(**bad) == SIZE, bad
     assert tree(nsplit=2, parts=2) == ARG and tree(parts=2, part=A + 4) == ALIGN and tree(out=None) == ARG and tree(parents=None) == ARG and tree(err=None) == ARG
     assert tree(T=0) == 0 and tree(B=0) == 0 and tree(most=0) == 0
+
+
+def test_plans_of_attention_of_trees():
+    """Pieces, pieces in the workspace, tcgen05 or not: by the rows of a tree and the keys before them."""
+    def plan(B, most, keys, nh=32, nkv=8, hd=64, dtype=1):
+        p = call("attention_tree", "cellm_attention_tree_plan", B, most, nh, nkv, hd, keys, dtype, 148)
+        return p & 0xff, p >> 8 & 0xff, p >> 16
+    n, parts, tc = plan(1, 8, 508)
+    assert tc == 0 and 1 < n <= 8 and parts == 0                   # a cluster, no workspace
+    assert plan(16, 25, 4121)[2] == 1 and plan(8, 16, 4096)[2] == 1 and plan(8, 16, 1024)[2] == 0 and plan(8, 4, 30000)[2] == 0
+    assert plan(8, 25, 4121, dtype=0)[2] == 0 and plan(8, 25, 4121, hd=128)[2] == 0 and plan(8, 25, 4121, nh=70, nkv=1)[2] == 0       # (70 of 128 rows)
+    for B in (1, 3, 8, 64):
+        for most in (1, 5, 16, 63, 256):
+            for keys in (1, 100, 5000, 100000):
+                for hd in (32, 64, 96, 128, 200):
+                    for dtype in (0, 1):
+                        n, parts, tc = plan(B, most, keys, hd=hd, dtype=dtype)
+                        assert 1 <= n <= 64 and parts == (n if n > (1 if tc else 8) else 0)
+    assert plan(64, 63, 100)[0] == 1                                # enough blocks without cutting
 
 
 def test_acceptance():

@@ -128,6 +128,17 @@ def test_long_contexts_are_cut_into_pieces(dtype, hd, nodes):
     check(x, run(x, max_ctx=3001))
 
 
+@pytest.mark.parametrize("nodes,nh,nkv", [(9, 8, 2), (16, 4, 1), (33, 4, 2), (7, 12, 4), (32, 32, 8)])
+@pytest.mark.parametrize("window", [0, 2500])
+def test_small_trees_behind_long_contexts(nodes, nh, nkv, window):
+    """Few rows on the wide tiles: both tiles of a CTA hold the same rows and take the blocks of keys in turn, an odd and an even
+    number of them, one alone for a context without keys."""
+    r = np.random.RandomState(nodes)
+    x = make(r, torch.bfloat16, [nodes, nodes, nodes], [2600, 0, 4099], nh, nkv, 64, 16, padding=1)
+    out = run(x, window)
+    check(x, out, window)
+
+
 def test_rows_may_be_dense_or_columns_and_other_trees_do_not_matter():
     r = np.random.RandomState(3)
     x = make(r, torch.bfloat16, [9, 30], [100, 40], 8, 2, 64, 16)
