@@ -14,6 +14,7 @@
 
 #include "attention_tree.cuh"
 #include "mma_tiles.cuh"
+#include "pairs.cuh"
 
 namespace {
 
@@ -42,14 +43,14 @@ __device__ __forceinline__ void write_pair(T* out, float2 v, bool both) {
 }
 
 // The block's rows, row0 .. row0 + RT - 1 of the tree's (node, head) pairs: o [RT][LD] and ml [RT][2] (maximum and sum) in shared
-// memory, written before a barrier. 16 of the 128 threads take a row. Rows of padding become zeros.
+// memory, written before a barrier. 16 threads take a row. Rows of padding become zeros.
 template <typename T, bool CL>
 __device__ __forceinline__ void finish_rows(const TreeArgs& a, const TreeTile& t, const TreeShape& tree, const float* o, int LD, const float* ml, int RT, int row0) {
     const int G = a.nh / a.nkv, rows = t.n * G, hd = a.hd, c = threadIdx.x & 15;
     const bool even = hd % 2 == 0;
     if constexpr (CL) cluster_meet();                   // every piece of the rows is there
     const int first = CL ? t.split : 0, step = CL ? a.nsplit : 1;
-    for (int r = first + (threadIdx.x >> 4) * step; r < RT && row0 + r < rows; r += 8 * step) {
+    for (int r = first + (threadIdx.x >> 4) * step; r < RT && row0 + r < rows; r += (blockDim.x >> 4) * step) {
         const int node = (row0 + r) / G;
         const bool seen = tree.depth[node] >= 0;
         const long long gr = (long long)(t.t_base + node) * a.nh + t.kvh * G + (row0 + r) % G;
@@ -102,13 +103,13 @@ __device__ __forceinline__ void finish_rows(const TreeArgs& a, const TreeTile& t
 }
 
 // ---------------------------------------------------------------- any type, any head size up to 256
-// 128 threads take 8 R rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit multiply-adds: a
+// 256 threads take 16 R rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit multiply-adds: a
 // thread forms R x KT/16 scores out of shared memory, a row's maximum and sum go over half a warp, and the thread then owns R x HDP/16
 // entries of the output. 32-bit rows on 16-byte borders (FAST) come in by cp.async, the next block while one is worked on; others
 // element by element.
 template <int HDP, int R, bool FAST>
 struct PlainTile {
-    static constexpr int RT = 8 * R, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
+    static constexpr int THREADS = 256, RT = 16 * R, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
     static constexpr int KV = KT * LD;                                   // floats of a block's keys, and of its values
     static constexpr size_t bytes = sizeof(TreeShape) + (size_t)(RT * LD + ST * 2 * KV + KT * (RT + 4)) * 4;
 };
@@ -134,11 +135,11 @@ __device__ __forceinline__ void row_to_floats(float* dst, const T* src, int hd, 
 }
 
 template <typename T, int HDP, int R, bool FAST, bool CL>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(256)
 attention_tree_plain_kernel(const TreeArgs a, int quads) {
     using L = PlainTile<HDP, R, FAST>;
     constexpr int RT = L::RT, KT = L::KT, LD = L::LD, KC = KT / 16;
-    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC), CHUNKS = HDP / 4, ITERS = KT * CHUNKS / 128;
+    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC), CHUNKS = HDP / 4, ITERS = KT * CHUNKS / L::THREADS;
     extern __shared__ __align__(16) uint8_t plain_smem[];
     TreeShape& tree = *reinterpret_cast<TreeShape*>(plain_smem);
     float* qs = reinterpret_cast<float*>(plain_smem + sizeof(TreeShape));     // [RT][LD]
@@ -156,13 +157,15 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     const int first = lo / KT, committed = lo < t.ctx ? (t.ctx + KT - 1) / KT - first : 0, blocks = committed + (t.n + KT - 1) / KT;
     const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), n_blk = min(blocks, begin + per) - begin;
     const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
+    const int shift = (a.page_size & (a.page_size - 1)) == 0 ? __ffs(a.page_size) - 1 : -1;
+    const size_t page_elems = (size_t)a.nkv * a.page_size * hd;
     // FAST: as in the tensor-core kernel below; an entry of the table is asked for a block before its rows are
     int entry[FAST ? ITERS : 1];
     auto look_up = [&](int i) {
 #pragma unroll
         for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
-            const int blk = begin + i, j = (first + blk) * KT + (threadIdx.x + it * 128) / CHUNKS;
-            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[j / a.page_size] : -2;
+            const int blk = begin + i, j = (first + blk) * KT + (threadIdx.x + it * L::THREADS) / CHUNKS;
+            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
         }
     };
     auto load = [&](int i) {
@@ -171,13 +174,14 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             const int blk = begin + i;
 #pragma unroll
             for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
-                const int row = (threadIdx.x + it * 128) / CHUNKS, chunk = (threadIdx.x + it * 128) % CHUNKS;
+                const int row = (threadIdx.x + it * L::THREADS) / CHUNKS, chunk = (threadIdx.x + it * L::THREADS) % CHUNKS;
                 const float *k = static_cast<const float*>(a.k_pool), *v = static_cast<const float*>(a.v_pool);
                 bool have = chunk * 4 < hd;
                 if (blk < committed) {
                     const int page = entry[it];
                     if (page >= 0 && page < a.num_pages) {
-                        const size_t off = (((size_t)page * a.nkv + t.kvh) * a.page_size + ((first + blk) * KT + row) % a.page_size) * hd + chunk * 4;
+                        const int j = (first + blk) * KT + row;
+                        const size_t off = (size_t)page * page_elems + (t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * hd + chunk * 4;
                         if (have) k += off, v += off;
                     } else {
                         if (page != -2) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
@@ -200,7 +204,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     look_up(0);
     const bool early = FAST && begin < committed;          // the first block needs nothing of the tree's shape
     if (early) load(0);
-    for (int r = warp; r < RT; r += 4) {
+    for (int r = warp; r < RT; r += 8) {
         const int row = row0 + r;
         const T* src = row < rows ? static_cast<const T*>(a.q) + (long long)(t.t_base + row / G) * a.q_ld + (long long)(t.kvh * G + row % G) * hd : nullptr;
         row_to_floats(qs + r * LD, src, hd, HDP, lane, 32, quads);
@@ -208,16 +212,17 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
     if (FAST && !early) load(0);
     look_up(1);
-    // a thread's rows are rg, rg + 8, rg + 16, ... of the tile
+    // a thread's rows are rg, rg + 16, rg + 32 of the tile
     int node[R];
-    float m[R], l[R], o[R][NV * VEC];
+    float m[R], l[R];
+    uint64_t o[R][NV * VEC / 2];               // in pairs
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-        const int row = row0 + rg + i * 8;
+        const int row = row0 + rg + i * 16;
         node[i] = row < rows && tree.depth[row / G] >= 0 ? row / G : -1;
         m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < NV * VEC; ++d) o[i][d] = 0.f;
+        for (int d = 0; d < NV * VEC / 2; ++d) o[i][d] = 0ull;
     }
     for (int i = 0; i < n_blk; ++i) {
         const int blk = begin + i;
@@ -231,7 +236,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             look_up(i + 2);
         } else {
             __syncthreads();
-            for (int r = warp; r < KT; r += 4) {
+            for (int r = warp; r < KT; r += 8) {
                 const T *k = nullptr, *v = nullptr;
                 if (paged) {
                     const int j = key0 + r;
@@ -253,31 +258,32 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             }
             __syncthreads();
         }
-        float s[R][KC];
+        // a score's products in two sums, of the even and of the odd entries
+        uint64_t s2[R][KC];
 #pragma unroll
         for (int x = 0; x < R; ++x)
 #pragma unroll
-            for (int k = 0; k < KC; ++k) s[x][k] = 0.f;
+            for (int k = 0; k < KC; ++k) s2[x][k] = 0ull;
 #pragma unroll 2
         for (int d = 0; d < HDP; d += 4) {
-            float4 q4[R], k4[KC];
+            ulonglong2 q4[R], k4[KC];
 #pragma unroll
-            for (int x = 0; x < R; ++x) q4[x] = *reinterpret_cast<const float4*>(qs + (rg + x * 8) * LD + d);
+            for (int x = 0; x < R; ++x) q4[x] = *reinterpret_cast<const ulonglong2*>(qs + (rg + x * 16) * LD + d);
 #pragma unroll
-            for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const float4*>(ks + (c + k * 16) * LD + d);
+            for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const ulonglong2*>(ks + (c + k * 16) * LD + d);
 #pragma unroll
             for (int x = 0; x < R; ++x)
 #pragma unroll
-                for (int k = 0; k < KC; ++k)
-                    s[x][k] = fmaf(q4[x].w, k4[k].w, fmaf(q4[x].z, k4[k].z, fmaf(q4[x].y, k4[k].y, fmaf(q4[x].x, k4[k].x, s[x][k]))));
+                for (int k = 0; k < KC; ++k) s2[x][k] = fma2(q4[x].y, k4[k].y, fma2(q4[x].x, k4[k].x, s2[x][k]));
         }
+        float s[R][KC];
 #pragma unroll
         for (int x = 0; x < R; ++x) {
             const uint64_t seen = node[x] >= 0 ? seen_bits<KT>(tree, node[x], a.window, t.ctx, key0, node0) : 0ull;
             float top = -INFINITY;
 #pragma unroll
             for (int k = 0; k < KC; ++k) {
-                s[x][k] = (seen >> (c + k * 16) & 1ull) ? s[x][k] * a.scale_log2e : -INFINITY;
+                s[x][k] = (seen >> (c + k * 16) & 1ull) ? (low_of(s2[x][k]) + high_of(s2[x][k])) * a.scale_log2e : -INFINITY;
                 top = fmaxf(top, s[x][k]);
             }
 #pragma unroll
@@ -293,32 +299,31 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             }
             l[x] = l[x] * corr + sum;
 #pragma unroll
-            for (int d = 0; d < NV * VEC; ++d) o[x][d] *= corr;
+            for (int d = 0; d < NV * VEC / 2; ++d) o[x][d] = fma2(o[x][d], pair_of(corr, corr), 0ull);
         }
         __syncwarp();                          // a half-warp writes and reads the columns of its own rows alone
 #pragma unroll 4
         for (int k = 0; k < KT; ++k) {
-            float p[R];
+            uint64_t p[R];
 #pragma unroll
-            for (int x = 0; x < R; x += 2) {
-                const float2 w = *reinterpret_cast<const float2*>(ps + k * (RT + 4) + rg * R + x);
-                p[x] = w.x, p[x + 1] = w.y;
+            for (int x = 0; x < R; ++x) {
+                const float w = ps[k * (RT + 4) + rg * R + x];
+                p[x] = pair_of(w, w);
             }
 #pragma unroll
             for (int g = 0; g < NV; ++g) {
-                float v[VEC];
                 const float* src = vs + k * LD + (g * 16 + c) * VEC;
+                uint64_t v[VEC / 2];
                 if constexpr (VEC == 4) {
-                    const float4 w = *reinterpret_cast<const float4*>(src);
-                    v[0] = w.x, v[1] = w.y, v[2] = w.z, v[3] = w.w;
-                } else {
-                    const float2 w = *reinterpret_cast<const float2*>(src);
+                    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(src);
                     v[0] = w.x, v[1] = w.y;
+                } else {
+                    v[0] = *reinterpret_cast<const uint64_t*>(src);
                 }
 #pragma unroll
                 for (int x = 0; x < R; ++x)
 #pragma unroll
-                    for (int y = 0; y < VEC; ++y) o[x][g * VEC + y] = fmaf(p[x], v[y], o[x][g * VEC + y]);
+                    for (int y = 0; y < VEC / 2; ++y) o[x][g * (VEC / 2) + y] = fma2(p[x], v[y], o[x][g * (VEC / 2) + y]);
             }
         }
     }
@@ -328,11 +333,11 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     for (int x = 0; x < R; ++x) {
 #pragma unroll
         for (int y = 8; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
-        const int r = rg + x * 8;
+        const int r = rg + x * 16;
 #pragma unroll
         for (int g = 0; g < NV; ++g)
 #pragma unroll
-            for (int y = 0; y < VEC; ++y) qs[r * LD + (g * 16 + c) * VEC + y] = o[x][g * VEC + y];
+            for (int y = 0; y < VEC / 2; ++y) *reinterpret_cast<uint64_t*>(qs + r * LD + (g * 16 + c) * VEC + y * 2) = o[x][g * (VEC / 2) + y];
         if (c == 0) ps[r * 2] = m[x], ps[r * 2 + 1] = l[x];
     }
     __syncthreads();
@@ -622,14 +627,14 @@ attention_tree_merge_kernel(T* __restrict__ out, const float* __restrict__ part_
     }
 }
 
-// A grid of 128 threads a block; in_cluster: the pieces of a tile are one cluster (they are neighbours in the grid).
+// The grid; in_cluster: the pieces of a tile are one cluster (they are neighbours in the grid).
 template <typename... KArgs, typename... Args>
-int launch_tiles(std::atomic<unsigned long long>& allowed, void (*kernel)(KArgs...), const TreeArgs& a, bool in_cluster, size_t smem, cudaStream_t stream, Args... args) {
+int launch_tiles(std::atomic<unsigned long long>& allowed, void (*kernel)(KArgs...), const TreeArgs& a, bool in_cluster, int threads, size_t smem, cudaStream_t stream, Args... args) {
     cudaError_t e = cellm_allow_smem(allowed, (const void*)kernel, smem);
     if (e != cudaSuccess) return (int)e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((long long)a.B * a.nkv * a.tiles * a.nsplit));
-    cfg.blockDim = dim3(128);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -651,8 +656,8 @@ int launch_plain_rows(TreeArgs a, int quads, cudaStream_t stream) {
     using L = PlainTile<HDP, R, FAST>;
     static std::atomic<unsigned long long> allowed[2];
     a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
-    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_plain_kernel<T, HDP, R, FAST, true>, a, true, L::bytes, stream, quads)
-                                                   : launch_tiles(allowed[0], attention_tree_plain_kernel<T, HDP, R, FAST, false>, a, false, L::bytes, stream, quads);
+    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_plain_kernel<T, HDP, R, FAST, true>, a, true, L::THREADS, L::bytes, stream, quads)
+                                                   : launch_tiles(allowed[0], attention_tree_plain_kernel<T, HDP, R, FAST, false>, a, false, L::THREADS, L::bytes, stream, quads);
 }
 // Rows of 32-bit tiles: 48 where that leaves the last tile fuller than 32 would, 16 for the smallest trees.
 int plain_rows(int rows) { return rows <= 16 ? 16 : rows % 32 == 0 || rows <= 32 || (rows + 47) / 48 * 48 > (rows + 31) / 32 * 32 ? 32 : 48; }
@@ -663,11 +668,11 @@ int launch_plain(const TreeArgs& a, cudaStream_t stream) {
     if constexpr (sizeof(T) == 4) {
         if (quads) {
             const int rows = plain_rows(a.most * (a.nh / a.nkv));
-            return rows == 16 ? launch_plain_rows<T, HDP, 2, true>(a, 1, stream) : rows == 32 ? launch_plain_rows<T, HDP, 4, true>(a, 1, stream)
-                                                                                              : launch_plain_rows<T, HDP, 6, true>(a, 1, stream);
+            return rows == 16 ? launch_plain_rows<T, HDP, 1, true>(a, 1, stream) : rows == 32 ? launch_plain_rows<T, HDP, 2, true>(a, 1, stream)
+                                                                                              : launch_plain_rows<T, HDP, 3, true>(a, 1, stream);
         }
     }
-    return launch_plain_rows<T, HDP, 4, false>(a, quads, stream);
+    return launch_plain_rows<T, HDP, 2, false>(a, quads, stream);
 }
 
 template <typename T>
@@ -684,8 +689,8 @@ int launch_mma(TreeArgs a, cudaStream_t stream) {
     using L = MmaTile<HD, RG>;
     static std::atomic<unsigned long long> allowed[2];
     a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
-    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_mma_kernel<HD, RG, true>, a, true, L::bytes, stream)
-                                                   : launch_tiles(allowed[0], attention_tree_mma_kernel<HD, RG, false>, a, false, L::bytes, stream);
+    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_mma_kernel<HD, RG, true>, a, true, 128, L::bytes, stream)
+                                                   : launch_tiles(allowed[0], attention_tree_mma_kernel<HD, RG, false>, a, false, 128, L::bytes, stream);
 }
 template <int HD>
 int launch_mma_rows(const TreeArgs& a, cudaStream_t stream) {
@@ -705,14 +710,17 @@ int launch_mma_sized(const TreeArgs& a, cudaStream_t stream) {
 }
 
 // How many pieces the keys of a tile of rows are cut into: of all counts the one whose rounds of blocks, each as long as its keys
-// and a few blocks' worth of start and merge, take the least time. Up to CLUSTER_MAX pieces merge at the cost of one block (where they
-// may be a cluster), more at that of a launch.
+// and a few blocks' worth of start and merge, take the least time. Up to CLUSTER_MAX pieces merge at the cost of one block where they may be
+// a cluster (clusters leave about an eighth of the blocks' places empty, since a cluster stays within a group of SMs: 280 blocks in clusters
+// of 7 took two rounds on 296 places), more at that of a launch.
 int pieces(long long tiles, int key_blocks, long long at_once, bool clusters) {
     constexpr int START = 3;
     int best = 1;
     long long least = LLONG_MAX;
     for (int n = 1; n <= 64 && n <= std::max(1, key_blocks); ++n) {
-        const long long cost = (tiles * n + at_once - 1) / at_once * ((key_blocks + n - 1) / n + START) + (n == 1 ? 0 : clusters && n <= CLUSTER_MAX ? 1 : START);
+        const bool cluster = clusters && n > 1 && n <= CLUSTER_MAX;
+        const long long room = cluster ? at_once - at_once / 8 : at_once;
+        const long long cost = (tiles * n + room - 1) / room * ((key_blocks + n - 1) / n + START) + (n == 1 ? 0 : cluster ? 1 : START);
         if (cost < least) least = cost, best = n;
     }
     return best;

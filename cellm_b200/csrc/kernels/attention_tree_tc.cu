@@ -13,6 +13,7 @@
 // Every wait on an mbarrier is bounded: a role that gives up sets CELLM_DEV_WAIT_TIMEOUT and an abort flag; the CTA frees its tensor
 // memory and returns.
 #include "attention_tree.cuh"
+#include "pairs.cuh"
 #include "tcgen05_attn.cuh"
 
 namespace {
@@ -40,28 +41,6 @@ struct TreeTcSmem {                    // starts on a 1024-byte boundary (checke
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
     float d;
     asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
-    return d;
-}
-// Two floats in a 64-bit register, worked on by one instruction.
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-    return d;
-}
-__device__ __forceinline__ float low_of(uint64_t v) {
-    return __uint_as_float((uint32_t)v);
-}
-__device__ __forceinline__ float high_of(uint64_t v) {
-    return __uint_as_float((uint32_t)(v >> 32));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 // 2^x of two numbers without the special-function units: x = n + f with |f| <= 1/2, n out of the rounding of an addition, 2^f = 1 + f

@@ -16,6 +16,7 @@
 #include <algorithm>
 
 #include "mma_tiles.cuh"
+#include "pairs.cuh"
 
 namespace {
 
@@ -30,25 +31,6 @@ struct RowPart {
     float best;
     double sum;
 };
-
-// Two floats in a 64-bit register, worked on by one instruction.
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
-    uint64_t d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-    return d;
-}
-__device__ __forceinline__ float low_of(uint64_t v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float high_of(uint64_t v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
 
 // exp(x - best) of two numbers, best the largest. d log2 e = n + f with |f| <= 1/2 comes out of the rounding of one addition and a
 // multiply-add; 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9. What matters lies
