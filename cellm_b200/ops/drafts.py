@@ -137,7 +137,13 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
                 or block_table.shape[0] != B:
             raise ValueError(f"accept_drafts: rows are written behind ctx_lens [{B}] on the pages of block_table [{B}, entries], dense int32 on {tokens.device}")
         k = _layers(k_new, k_pool, T, index)
-        v = (0, 0, 0, None) if v_new is None else _layers(v_new, v_pool, T, index)
+        if v_new is None:
+            v = (0, 0, 0, None)
+        elif (v_new.shape == k_new.shape and v_new.stride() == k_new.stride() and v_pool.shape == k_pool.shape and v_new.dtype is v_pool.dtype is k_pool.dtype
+              and v_new.get_device() == index and v_pool.get_device() == index and v_pool.is_contiguous()):
+            v = k                                                              # laid out alike
+        else:
+            v = _layers(v_new, v_pool, T, index)
         if k is None or v is None or (v_new is not None and v[3][:4] != k[3][:4]):
             raise ValueError("accept_drafts: k_new and v_new [items, T, kv heads, head size], a node's heads side by side, of the type of their dense pools [items, pages, "
                              f"kv heads, page size, head size] (got {[tuple(t.shape) for t in (k_new, v_new, k_pool, v_pool) if t is not None]})")
@@ -145,8 +151,7 @@ def accept_drafts(tokens: torch.Tensor, parents: torch.Tensor, choices: torch.Te
         rows = (k_new.data_ptr(), k[0], k[1], k[2], k_pool.data_ptr()) + ((v_new.data_ptr(), v[0], v[1], v[2], v_pool.data_ptr()) if v_new is not None else (0,) * 5)
         where = (ctx_lens.data_ptr(), block_table.data_ptr(), block_table.shape[1], items, nkv, pages, page_size)
     path = tokens.new_empty((B, longest))
-    count = torch.empty_like(ctx_lens) if ctx_lens is not None and ctx_lens.dim() == 1 and ctx_lens.numel() == B and ctx_lens.dtype is torch.int32 \
-        and ctx_lens.get_device() == index else tokens.new_empty(B)
+    count = tokens.new_empty(B) if k_new is None or ctx_lens.dim() != 1 else torch.empty_like(ctx_lens)
     after = torch.empty_like(count)
     if B:
         launch_packed("candidates", "accept_drafts", index,
