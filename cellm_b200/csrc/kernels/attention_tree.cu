@@ -103,15 +103,21 @@ __device__ __forceinline__ void finish_rows(const TreeArgs& a, const TreeTile& t
 }
 
 // ---------------------------------------------------------------- any type, any head size up to 256
-// 256 threads take 16 R rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit multiply-adds: a
-// thread forms R x KT/16 scores out of shared memory, a row's maximum and sum go over half a warp, and the thread then owns R x HDP/16
-// entries of the output. 32-bit rows on 16-byte borders (FAST) come in by cp.async, the next block while one is worked on; others
-// element by element.
-template <int HDP, int R, bool FAST>
+// A block takes 16 RG rows ((node, query head) pairs of one key/value head) through blocks of KT keys in 32-bit multiply-adds.
+// RG groups of 16 rows times KG equal parts of the keys: a warp each, with a softmax state of its own; the KG warps of a
+// group meet in shared memory at the end. In a warp four lanes stand for four rows each, eight for WK/8 keys each (then for an
+// eighth of the output's columns), so 16 x WK scores are formed out of 16 + WK rows of shared memory (with 6 x 64 scores a
+// warp its bandwidth was at 72 %). 32-bit rows on 16-byte borders (FAST) come in by cp.async, the next block while one is worked on;
+// others element by element. A block of 64 keys for 48 rows of 64 takes 10,000 cycles alone on an SM: 3,400 for the scores and 3,000 for
+// the output (their multiply-adds would be 3,072 of an SM's), 2,200 to issue the copies, 1,100 for the softmax.
+template <int HDP, int RG, bool FAST>
 struct PlainTile {
-    static constexpr int THREADS = 256, RT = 16 * R, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
+    static constexpr int RT = 16 * RG, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
+    static constexpr int KG = RG == 3 || HDP > 128 ? 2 : 4, WK = KT / KG, THREADS = 32 * RG * KG, PLD = 20;
     static constexpr int KV = KT * LD;                                   // floats of a block's keys, and of its values
-    static constexpr size_t bytes = sizeof(TreeShape) + (size_t)(RT * LD + ST * 2 * KV + KT * (RT + 4)) * 4;
+    static constexpr int O_FLOATS = KG * RT * (HDP + 2), RING = ST * 2 * KV > O_FLOATS ? ST * 2 * KV : O_FLOATS;     // the outputs meet where the ring was
+    static constexpr size_t bytes = sizeof(TreeShape) + (size_t)(RT * LD + RING + RG * KG * WK * PLD) * 4;
+    static_assert(WK >= 8, "a key a lane at least");
 };
 
 template <typename T>
@@ -134,25 +140,54 @@ __device__ __forceinline__ void row_to_floats(float* dst, const T* src, int hd, 
     }
 }
 
-template <typename T, int HDP, int R, bool FAST, bool CL>
-__global__ void __launch_bounds__(256)
+// What KG groups of warps found for the same RT rows, into the place of the first of them: o [KG][RT][HD], ml [KG][RT][2]. 16 threads a
+// row; between barriers.
+template <int KG>
+__device__ __forceinline__ void join_groups(float* o, float* ml, int RT, int HD) {
+    for (int r = threadIdx.x >> 4; r < RT; r += blockDim.x >> 4) {
+        float2 w[KG];
+        float M = -INFINITY, f[KG], l = 0.f;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+            w[g] = *reinterpret_cast<const float2*>(ml + (g * RT + r) * 2);
+            M = fmaxf(M, w[g].x);
+        }
+        const float use = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int g = 0; g < KG; ++g) f[g] = exp2f(w[g].x - use), l += f[g] * w[g].y;
+        __syncwarp();
+        if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(M, l);
+        for (int d = (threadIdx.x & 15) * 2; d < HD; d += 32) {
+            float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int g = 0; g < KG; ++g) {
+                const float2 v = *reinterpret_cast<const float2*>(o + (g * RT + r) * HD + d);
+                acc.x = fmaf(f[g], v.x, acc.x), acc.y = fmaf(f[g], v.y, acc.y);
+            }
+            *reinterpret_cast<float2*>(o + r * HD + d) = acc;
+        }
+    }
+}
+
+template <typename T, int HDP, int RG, bool FAST, bool CL>
+__global__ void __launch_bounds__(PlainTile<HDP, RG, FAST>::THREADS)
 attention_tree_plain_kernel(const TreeArgs a, int quads) {
-    using L = PlainTile<HDP, R, FAST>;
-    constexpr int RT = L::RT, KT = L::KT, LD = L::LD, KC = KT / 16;
-    constexpr int VEC = HDP % 64 == 0 ? 4 : 2, NV = HDP / (16 * VEC), CHUNKS = HDP / 4, ITERS = KT * CHUNKS / L::THREADS;
+    using L = PlainTile<HDP, RG, FAST>;
+    constexpr int RT = L::RT, KT = L::KT, LD = L::LD, KG = L::KG, WK = L::WK, KC = WK / 8, WARPS = RG * KG;
+    constexpr int NV = HDP / 32, CHUNKS = HDP / 4, PIECES = KT * CHUNKS, ITERS = (PIECES + L::THREADS - 1) / L::THREADS;
     extern __shared__ __align__(16) uint8_t plain_smem[];
     TreeShape& tree = *reinterpret_cast<TreeShape*>(plain_smem);
     float* qs = reinterpret_cast<float*>(plain_smem + sizeof(TreeShape));     // [RT][LD]
     float* kv = qs + RT * LD;                                                 // [ST][keys | values][KT][LD]
-    float* ps = kv + L::ST * 2 * L::KV;                                       // [KT][RT + 4]
+    float* ps = kv + L::RING + (threadIdx.x >> 5) * WK * L::PLD;              // this warp's weights, [WK][16 rows]
     pdl_wait();
     pdl_trigger();
     const TreeTile t = tree_tile(a);
     const int G = a.nh / a.nkv, rows = t.n * G, row0 = t.tile * RT;
     if (!t.live || row0 >= rows) return;
 
-    const int hd = a.hd, rg = threadIdx.x >> 4, c = threadIdx.x & 15;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int hd = a.hd, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rg = warp % RG, kg = warp / RG;
+    const int rl = lane >> 3, c = lane & 7;            // the lane's rows: rl, rl + 4, ...; its keys and columns
     const int lo = a.window > 0 ? max(0, t.ctx - a.window + 1) : 0;
     const int first = lo / KT, committed = lo < t.ctx ? (t.ctx + KT - 1) / KT - first : 0, blocks = committed + (t.n + KT - 1) / KT;
     const int per = (blocks + a.nsplit - 1) / a.nsplit, begin = min(blocks, t.split * per), n_blk = min(blocks, begin + per) - begin;
@@ -164,8 +199,8 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     auto look_up = [&](int i) {
 #pragma unroll
         for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
-            const int blk = begin + i, j = (first + blk) * KT + (threadIdx.x + it * L::THREADS) / CHUNKS;
-            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
+            const int blk = begin + i, at = threadIdx.x + it * L::THREADS, j = (first + blk) * KT + at / CHUNKS;
+            entry[it] = at < PIECES && i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
         }
     };
     auto load = [&](int i) {
@@ -175,6 +210,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
 #pragma unroll
             for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
                 const int row = (threadIdx.x + it * L::THREADS) / CHUNKS, chunk = (threadIdx.x + it * L::THREADS) % CHUNKS;
+                if (PIECES % L::THREADS && row >= KT) break;
                 const float *k = static_cast<const float*>(a.k_pool), *v = static_cast<const float*>(a.v_pool);
                 bool have = chunk * 4 < hd;
                 if (blk < committed) {
@@ -204,7 +240,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     look_up(0);
     const bool early = FAST && begin < committed;          // the first block needs nothing of the tree's shape
     if (early) load(0);
-    for (int r = warp; r < RT; r += 8) {
+    for (int r = warp; r < RT; r += WARPS) {
         const int row = row0 + r;
         const T* src = row < rows ? static_cast<const T*>(a.q) + (long long)(t.t_base + row / G) * a.q_ld + (long long)(t.kvh * G + row % G) * hd : nullptr;
         row_to_floats(qs + r * LD, src, hd, HDP, lane, 32, quads);
@@ -212,17 +248,17 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
     read_tree(tree, a.parents + t.t_base, t.n, a.window, a.err);
     if (FAST && !early) load(0);
     look_up(1);
-    // a thread's rows are rg, rg + 16, rg + 32 of the tile
-    int node[R];
-    float m[R], l[R];
-    uint64_t o[R][NV * VEC / 2];               // in pairs
+    const int open_from = a.window > 0 ? t.ctx + t.n - a.window : 0;        // no row's window starts behind it
+    int node[4];
+    float m[4], l[4];
+    uint64_t o[4][NV * 2];                     // in pairs of columns
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int row = row0 + rg + i * 16;
+    for (int i = 0; i < 4; ++i) {
+        const int row = row0 + rg * 16 + rl + i * 4;
         node[i] = row < rows && tree.depth[row / G] >= 0 ? row / G : -1;
         m[i] = -INFINITY, l[i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < NV * VEC / 2; ++d) o[i][d] = 0ull;
+        for (int d = 0; d < NV * 2; ++d) o[i][d] = 0ull;
     }
     for (int i = 0; i < n_blk; ++i) {
         const int blk = begin + i;
@@ -236,7 +272,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             look_up(i + 2);
         } else {
             __syncthreads();
-            for (int r = warp; r < KT; r += 8) {
+            for (int r = warp; r < KT; r += WARPS) {
                 const T *k = nullptr, *v = nullptr;
                 if (paged) {
                     const int j = key0 + r;
@@ -258,90 +294,83 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
             }
             __syncthreads();
         }
-        // a score's products in two sums, of the even and of the odd entries
-        uint64_t s2[R][KC];
+        const float *q_row = qs + (rg * 16 + rl) * LD, *k_row = ks + (kg * WK + c) * LD;
+        float s2[4][KC];
 #pragma unroll
-        for (int x = 0; x < R; ++x)
+        for (int x = 0; x < 4; ++x)
 #pragma unroll
-            for (int k = 0; k < KC; ++k) s2[x][k] = 0ull;
+            for (int k = 0; k < KC; ++k) s2[x][k] = 0.f;
 #pragma unroll 2
         for (int d = 0; d < HDP; d += 4) {
-            ulonglong2 q4[R], k4[KC];
+            float4 q4[4], k4[KC];
 #pragma unroll
-            for (int x = 0; x < R; ++x) q4[x] = *reinterpret_cast<const ulonglong2*>(qs + (rg + x * 16) * LD + d);
+            for (int x = 0; x < 4; ++x) q4[x] = *reinterpret_cast<const float4*>(q_row + x * 4 * LD + d);
 #pragma unroll
-            for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const ulonglong2*>(ks + (c + k * 16) * LD + d);
+            for (int k = 0; k < KC; ++k) k4[k] = *reinterpret_cast<const float4*>(k_row + k * 8 * LD + d);
 #pragma unroll
-            for (int x = 0; x < R; ++x)
+            for (int x = 0; x < 4; ++x)
 #pragma unroll
-                for (int k = 0; k < KC; ++k) s2[x][k] = fma2(q4[x].y, k4[k].y, fma2(q4[x].x, k4[k].x, s2[x][k]));
+                for (int k = 0; k < KC; ++k) s2[x][k] = fmaf(q4[x].w, k4[k].w, fmaf(q4[x].z, k4[k].z, fmaf(q4[x].y, k4[k].y, fmaf(q4[x].x, k4[k].x, s2[x][k]))));
         }
-        float s[R][KC];
+        float s[4][KC];
+        const bool open = paged && key0 + KT <= t.ctx && key0 >= open_from;
 #pragma unroll
-        for (int x = 0; x < R; ++x) {
-            const uint64_t seen = node[x] >= 0 ? seen_bits<KT>(tree, node[x], a.window, t.ctx, key0, node0) : 0ull;
+        for (int x = 0; x < 4; ++x) {
             float top = -INFINITY;
 #pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                s[x][k] = (seen >> (c + k * 16) & 1ull) ? (low_of(s2[x][k]) + high_of(s2[x][k])) * a.scale_log2e : -INFINITY;
-                top = fmaxf(top, s[x][k]);
+            for (int k = 0; k < KC; ++k) s[x][k] = s2[x][k] * a.scale_log2e;
+            if (!open) {
+                const uint64_t seen = node[x] >= 0 ? seen_bits<KT>(tree, node[x], a.window, t.ctx, key0, node0) >> (kg * WK + c) : 0ull;
+#pragma unroll
+                for (int k = 0; k < KC; ++k)
+                    if (!(seen >> (k * 8) & 1ull)) s[x][k] = -INFINITY;
             }
 #pragma unroll
-            for (int y = 8; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
-            const float now = fmaxf(m[x], top), use = now == -INFINITY ? 0.f : now, corr = exp2f(m[x] - use);
+            for (int k = 0; k < KC; ++k) top = fmaxf(top, s[x][k]);
+#pragma unroll
+            for (int y = 4; y > 0; y >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, y));
+            const float now = fmaxf(m[x], top), use = now == -INFINITY ? 0.f : now, corr = fast_exp2(m[x] - use);
             m[x] = now;
             float sum = 0.f;
 #pragma unroll
-            for (int k = 0; k < KC; ++k) {
-                const float p = exp2f(s[x][k] - use);
-                sum += p;
-                ps[(c + k * 16) * (RT + 4) + rg * R + x] = p;
-            }
+            for (int k = 0; k < KC; ++k) s[x][k] = fast_exp2(s[x][k] - use), sum += s[x][k];
             l[x] = l[x] * corr + sum;
 #pragma unroll
-            for (int d = 0; d < NV * VEC / 2; ++d) o[x][d] = fma2(o[x][d], pair_of(corr, corr), 0ull);
+            for (int d = 0; d < NV * 2; ++d) o[x][d] = fma2(o[x][d], pair_of(corr, corr), 0ull);
         }
-        __syncwarp();                          // a half-warp writes and reads the columns of its own rows alone
-#pragma unroll 4
-        for (int k = 0; k < KT; ++k) {
-            uint64_t p[R];
 #pragma unroll
-            for (int x = 0; x < R; ++x) {
-                const float w = ps[k * (RT + 4) + rg * R + x];
-                p[x] = pair_of(w, w);
-            }
+        for (int k = 0; k < KC; ++k) *reinterpret_cast<float4*>(ps + (c + k * 8) * L::PLD + rl * 4) = make_float4(s[0][k], s[1][k], s[2][k], s[3][k]);
+        __syncwarp();
+        const float* v_row = vs + kg * WK * LD + c * 4;
+#pragma unroll 4
+        for (int k = 0; k < WK; ++k) {
+            const float4 w = *reinterpret_cast<const float4*>(ps + k * L::PLD + rl * 4);
+            const uint64_t p[4] = {pair_of(w.x, w.x), pair_of(w.y, w.y), pair_of(w.z, w.z), pair_of(w.w, w.w)};
 #pragma unroll
             for (int g = 0; g < NV; ++g) {
-                const float* src = vs + k * LD + (g * 16 + c) * VEC;
-                uint64_t v[VEC / 2];
-                if constexpr (VEC == 4) {
-                    const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(src);
-                    v[0] = w.x, v[1] = w.y;
-                } else {
-                    v[0] = *reinterpret_cast<const uint64_t*>(src);
-                }
+                const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(v_row + k * LD + g * 32);
 #pragma unroll
-                for (int x = 0; x < R; ++x)
-#pragma unroll
-                    for (int y = 0; y < VEC / 2; ++y) o[x][g * (VEC / 2) + y] = fma2(p[x], v[y], o[x][g * (VEC / 2) + y]);
+                for (int x = 0; x < 4; ++x) o[x][2 * g] = fma2(p[x], v.x, o[x][2 * g]), o[x][2 * g + 1] = fma2(p[x], v.y, o[x][2 * g + 1]);
             }
         }
+        __syncwarp();                          // (the weights' place is written again by the next block)
     }
     if constexpr (FAST) cp_async_wait<0>();
-    __syncthreads();                           // the queries' and the weights' places are free
+    __syncthreads();                           // the ring's place is free
+    float *o_s = kv, *ml_s = kv + KG * RT * HDP;             // [KG][RT][HDP], [KG][RT][2]
 #pragma unroll
-    for (int x = 0; x < R; ++x) {
+    for (int x = 0; x < 4; ++x) {
 #pragma unroll
-        for (int y = 8; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
-        const int r = rg + x * 16;
+        for (int y = 4; y > 0; y >>= 1) l[x] += __shfl_xor_sync(0xffffffffu, l[x], y);
+        const int r = kg * RT + rg * 16 + rl + x * 4;
 #pragma unroll
-        for (int g = 0; g < NV; ++g)
-#pragma unroll
-            for (int y = 0; y < VEC / 2; ++y) *reinterpret_cast<uint64_t*>(qs + r * LD + (g * 16 + c) * VEC + y * 2) = o[x][g * (VEC / 2) + y];
-        if (c == 0) ps[r * 2] = m[x], ps[r * 2 + 1] = l[x];
+        for (int g = 0; g < NV; ++g) *reinterpret_cast<ulonglong2*>(o_s + r * HDP + g * 32 + c * 4) = make_ulonglong2(o[x][2 * g], o[x][2 * g + 1]);
+        if (c == 0) ml_s[r * 2] = m[x], ml_s[r * 2 + 1] = l[x];
     }
     __syncthreads();
-    finish_rows<T, CL>(a, t, tree, qs, LD, ps, RT, row0);
+    join_groups<KG>(o_s, ml_s, RT, HDP);
+    __syncthreads();
+    finish_rows<T, CL>(a, t, tree, o_s, HDP, ml_s, RT, row0);
 }
 
 // ---------------------------------------------------------------- bfloat16, head sizes 32, 64, 96, 128: mma.sync
@@ -549,31 +578,7 @@ attention_tree_mma_kernel(const TreeArgs a) {
     }
     __syncthreads();
     if constexpr (KG > 1) {
-        // the warps that took the same rows, into the place of the first of them: [RT][HD]
-        for (int r = threadIdx.x >> 4; r < L::RT; r += 8) {
-            float2 ml[KG];
-            float M = -INFINITY, f[KG], l = 0.f;
-#pragma unroll
-            for (int g = 0; g < KG; ++g) {
-                ml[g] = *reinterpret_cast<const float2*>(ml_s + (g * L::RT + r) * 2);
-                M = fmaxf(M, ml[g].x);
-            }
-            const float use = M == -INFINITY ? 0.f : M;
-#pragma unroll
-            for (int g = 0; g < KG; ++g) f[g] = exp2f(ml[g].x - use), l += f[g] * ml[g].y;
-            __syncwarp();
-            if ((threadIdx.x & 15) == 0) *reinterpret_cast<float2*>(ml_s + r * 2) = make_float2(M, l);
-#pragma unroll
-            for (int d = (threadIdx.x & 15) * 2; d < HD; d += 32) {
-                float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-                for (int g = 0; g < KG; ++g) {
-                    const float2 v = *reinterpret_cast<const float2*>(o_s + (g * L::RT + r) * HD + d);
-                    acc.x = fmaf(f[g], v.x, acc.x), acc.y = fmaf(f[g], v.y, acc.y);
-                }
-                *reinterpret_cast<float2*>(o_s + r * HD + d) = acc;
-            }
-        }
+        join_groups<KG>(o_s, ml_s, L::RT, HD);
         __syncthreads();
     }
     finish_rows<__nv_bfloat16, CL>(a, t, tree, o_s, HD, ml_s, L::RT, row0);
@@ -651,25 +656,29 @@ int launch_tiles(std::atomic<unsigned long long>& allowed, void (*kernel)(KArgs.
 // Up to this many pieces meet in a cluster.
 constexpr int CLUSTER_MAX = 8;
 
-template <typename T, int HDP, int R, bool FAST>
+template <typename T, int HDP, int RG, bool FAST>
 int launch_plain_rows(TreeArgs a, int quads, cudaStream_t stream) {
-    using L = PlainTile<HDP, R, FAST>;
+    using L = PlainTile<HDP, RG, FAST>;
     static std::atomic<unsigned long long> allowed[2];
     a.tiles = (a.most * (a.nh / a.nkv) + L::RT - 1) / L::RT;
-    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_plain_kernel<T, HDP, R, FAST, true>, a, true, L::THREADS, L::bytes, stream, quads)
-                                                   : launch_tiles(allowed[0], attention_tree_plain_kernel<T, HDP, R, FAST, false>, a, false, L::THREADS, L::bytes, stream, quads);
+    return a.nsplit > 1 && a.nsplit <= CLUSTER_MAX ? launch_tiles(allowed[1], attention_tree_plain_kernel<T, HDP, RG, FAST, true>, a, true, L::THREADS, L::bytes, stream, quads)
+                                                   : launch_tiles(allowed[0], attention_tree_plain_kernel<T, HDP, RG, FAST, false>, a, false, L::THREADS, L::bytes, stream, quads);
 }
-// Rows of 32-bit tiles: 48 where that leaves the last tile fuller than 32 would, 16 for the smallest trees.
-int plain_rows(int rows) { return rows <= 16 ? 16 : rows % 32 == 0 || rows <= 32 || (rows + 47) / 48 * 48 > (rows + 31) / 32 * 32 ? 32 : 48; }
+// Rows of 32-bit tiles: 48 where that leaves the last tile fuller than 32 would (not for the widest heads, whose tiles would not fit
+// twice into an SM), 16 for the smallest trees.
+int plain_rows(int rows, int hd) { return rows <= 16 ? 16 : hd > 128 || rows % 32 == 0 || rows <= 32 || (rows + 47) / 48 * 48 > (rows + 31) / 32 * 32 ? 32 : 48; }
 template <typename T, int HDP>
 int launch_plain(const TreeArgs& a, cudaStream_t stream) {
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool;
     const int quads = a.hd % 4 == 0 && a.q_ld % 4 == 0 && a.k_ld % 4 == 0 && a.v_ld % 4 == 0 && at % (4 * sizeof(T)) == 0;
     if constexpr (sizeof(T) == 4) {
         if (quads) {
-            const int rows = plain_rows(a.most * (a.nh / a.nkv));
-            return rows == 16 ? launch_plain_rows<T, HDP, 1, true>(a, 1, stream) : rows == 32 ? launch_plain_rows<T, HDP, 2, true>(a, 1, stream)
-                                                                                              : launch_plain_rows<T, HDP, 3, true>(a, 1, stream);
+            const int rows = plain_rows(a.most * (a.nh / a.nkv), a.hd);
+            if (rows == 16) return launch_plain_rows<T, HDP, 1, true>(a, 1, stream);
+            if constexpr (HDP <= 128) {
+                if (rows == 48) return launch_plain_rows<T, HDP, 3, true>(a, 1, stream);
+            }
+            return launch_plain_rows<T, HDP, 2, true>(a, 1, stream);
         }
     }
     return launch_plain_rows<T, HDP, 2, false>(a, quads, stream);
@@ -746,7 +755,7 @@ TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype
         return {true, n, n > 1 ? n : 0};
     }
     const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
-    const int tile = mma ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : dtype == CELLM_F32 ? plain_rows(rows) : 32;
+    const int tile = mma ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : dtype == CELLM_F32 ? plain_rows(rows, hd) : 32;
     const int an_sm = hd <= 32 ? (mma ? 4 : 3) : mma && hd == 64 ? 3 : 2;     // blocks that an SM holds, by their shared memory
     const int block = mma || hd <= 64 ? 64 : hd <= 128 ? 32 : 16;
     const int n = pieces((long long)B * nkv * ((rows + tile - 1) / tile), (keys + block - 1) / block, (long long)an_sm * sms, true);
