@@ -115,7 +115,8 @@ def _search(engine, group: _Beams, prompts, K: int, max_new_tokens: int, length_
                 group.hold(r * K + k, at + len(part))
         rows.append(logits.clone())
     scores, parents, tokens = ops.beam_select(torch.cat(rows), torch.zeros((R, 1), device=dev), K)
-    group.follow(parents, torch.zeros_like(group.starts))        # all of a prompt's beams start from the first one's cache
+    # all of a prompt's beams start from the first one's cache, those too that find no continuation yet (a vocabulary of fewer tokens)
+    group.follow(torch.zeros_like(parents), torch.zeros_like(group.starts))
     done = tokens == eos if eos is not None else torch.zeros((R, K), dtype=torch.bool, device=dev)
     histories = [[[t] for t in row] for row in tokens.tolist()]
     for _ in range(max_new_tokens - 1):

@@ -86,6 +86,18 @@ def test_a_beam_that_ends_stands(folders):
         assert any(b.finished for b in got)
 
 
+def test_fewer_tokens_than_beams(tmp_path):
+    """A vocabulary of five tokens and eight beams: the first step finds five continuations, and beams that had none follow later."""
+    from cellm_b200 import Engine
+    name = list(CONFIGS)[0]
+    folder = make_model(tmp_path, name, "float32", overrides={"vocab_size": 5, "eos_token_id": 4})
+    cfg, w = plain.load_folder(folder)
+    eng = Engine(folder, dtype="float32", tokens_per_block=4, total_blocks=100, max_num_seqs=8)
+    prompt = [1, 0, 3, 2, 2, 1, 0]
+    check(cfg, w, prompt, eng.beam_search([prompt], beams=8, max_new_tokens=5, stop_eos=False)[0], 8, 5, None)
+    assert len(eng.beam_search([prompt], beams=8, max_new_tokens=1, stop_eos=False)[0]) == 5
+
+
 def test_the_engine_serves_on_after_a_search(folders):
     from cellm_b200 import Engine, SamplingParams
     name = list(CONFIGS)[1]
