@@ -217,7 +217,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
                     const int page = entry[it];
                     if (page >= 0 && page < a.num_pages) {
                         const int j = (first + blk) * KT + row;
-                        const size_t off = (size_t)page * page_elems + (t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * hd + chunk * 4;
+                        const size_t off = (size_t)page * page_elems + ((size_t)t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * hd + chunk * 4;
                         if (have) k += off, v += off;
                     } else {
                         if (page != -2) atomicOr(a.err, CELLM_DEV_BAD_PAGE);

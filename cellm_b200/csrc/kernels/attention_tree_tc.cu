@@ -416,7 +416,7 @@ bool attention_tree_tc_takes(const TreeArgs& a) {
     const int G = a.nh / a.nkv;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
     return a.hd == HD && a.scale_log2e > 0.f && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0 && G <= TM && TM / G * G >= 96 &&
-           a.page_size >= 8 && a.page_size <= TN && (a.page_size & (a.page_size - 1)) == 0 && (long long)a.num_pages * a.nkv * a.page_size <= 0x7fffffffLL;
+           a.num_pages > 0 && a.page_size >= 8 && a.page_size <= TN && (a.page_size & (a.page_size - 1)) == 0 && (long long)a.num_pages * a.nkv * a.page_size <= 0x7fffffffLL;
 }
 
 // part_o and part_ml hold a.nsplit pieces where there are more than one.

@@ -89,7 +89,8 @@ CELLM_API int cellm_accept_drafts(int* out_count, int* out_path, int* out_next, 
                                   int items, int nkv, int pages, int page_size, int* err, cudaStream_t stream) {
     if (B <= 0) return CELLM_OK;
     if (B > 65535 || T < 0 || longest <= 0 || items < 0 || (items > 0 && (nkv <= 0 || pages <= 0 || page_size <= 0 || k_bytes <= 0 || bt_stride < 0))) return CELLM_ERR_SIZE;
-    if (!out_count || !out_path || !out_next || !tokens || !parents || !choices || !cu_seqlens || !err) return CELLM_ERR_ARG;
+    if (!out_count || !out_path || !out_next || !cu_seqlens || !err || (T > 0 && (!tokens || !parents || !choices))) return CELLM_ERR_ARG;
+    if (T == 0) items = 0;                // (trees without nodes: nothing stands)
     if (items > 0 && (!k_new || !k_pool || !ctx_lens || !block_table || (v_new && (!v_pool || v_bytes <= 0)))) return CELLM_ERR_ARG;
     const DraftRows k = {items > 0 ? k_new : nullptr, k_pool, k_item, k_row, items > 0 ? k_bytes : 0},
                     v = {items > 0 ? v_new : nullptr, v_pool, v_item, v_row, items > 0 && v_new ? v_bytes : 0};

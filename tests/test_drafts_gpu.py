@@ -266,6 +266,25 @@ def test_accepted_rows_go_into_the_pages(dtype, items, nkv, hd, vd, page):
     assert e.item() == 0 and all(torch.equal(pool[x], want[x]) for x in "kv" if sizes[x])
 
 
+def test_trees_without_nodes_keep_nothing():
+    from cellm_b200 import ops
+    e, none, pool = err_word(), ints([]), torch.zeros(1, 4, 1, 2, 8, device=DEV)
+    for more in ({}, dict(k_new=pool.new_zeros(1, 0, 1, 8), k_pool=pool, ctx_lens=ints([0, 3]), block_table=ints([[0, 1], [2, 3]]))):
+        count, path, after = ops.accept_drafts(none, none, none, ints([0, 0, 0]), 3, e, **more)
+        assert count.tolist() == [0, 0] and path.tolist() == [[-1] * 3] * 2 and after.tolist() == [-1, -1]
+    count, path, after = ops.accept_drafts(none, none, none, ints([0]), 3, e)
+    assert count.shape == after.shape == (0,) and path.shape == (0, 3) and e.item() == 0
+
+
+def test_an_empty_cache():
+    """Trees of requests without a committed token, over a pool without pages."""
+    r = np.random.RandomState(4)
+    for n in (5, 40):
+        x = make(r, torch.bfloat16, [n], [0], 4, 2, 64, 16)
+        check(x, run(x))
+        check(x, run(dict(x, k=x["k"][:0], v=x["v"][:0], table=np.zeros((1, 0)))))
+
+
 def test_acceptance_of_bad_trees_and_pages():
     from cellm_b200 import ops
     e = err_word()
