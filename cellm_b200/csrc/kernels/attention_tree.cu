@@ -376,7 +376,9 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
 // ---------------------------------------------------------------- bfloat16, head sizes 32, 64, 96, 128: mma.sync
 // Four warps take 16 * RG rows through blocks of 64 keys that all threads bring in with cp.async (a ring of ST stages, one barrier
 // a block). RG groups of 16 rows share a block; the 4 / RG warps of a group take its keys in equal parts, each with a softmax
-// state of its own, and meet in shared memory at the end. Few rows (small trees) so still use every warp.
+// state of its own, and meet in shared memory at the end. Few rows (small trees) so still use every warp. One tree of 8 nodes behind 500
+// keys, 32 heads over 8: 8.9 us in a CUDA graph, bound by latency (the copies' first block, the merge); with many long trees by issue
+// slots (42 %) and waits for shared memory, which is why those go to tcgen05.
 template <int HD, int RG>
 struct MmaTile {
     static constexpr int KG = 4 / RG, RT = 16 * RG;

@@ -2,13 +2,21 @@
 // head) pairs of one key/value head) fill tiles of 128.
 //
 // One CTA takes two tiles of 128 rows through blocks of 128 keys: committed ones, a TMA box a page, then the nodes' own, a box a
-// block. Warps 0 and 2 bring queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P read from
-// tensor memory and V as its rows lie), warps 4..7 and 8..11 do the softmax of a tile each, a row a thread, so that one tile's products
-// run beside the other's softmax; they take the registers that the first warpgroup gives up. Trees of up to 128 rows have one tile: the same rows then stand in both, and the tiles take the
-// blocks in turn; the second tile's result joins the first's through shared memory at the end.
+// block. Warps 0 and 2 bring queries, keys and values in, warp 1 issues the products (S = Q.K^T into tensor memory, O += P.V with P
+// read from tensor memory and V as its rows lie), warps 4..7 and 8..11 do the softmax of a tile each, a row a thread, so that one
+// tile's products run beside the other's softmax; they take the registers that the first warpgroup gives up. Trees of up to 128 rows
+// have one tile: the same rows then stand in both, and the tiles take the blocks in turn; the second tile's result joins the first's
+// through shared memory at the end.
 //
 // What it costs is exponentials: a block of 128 x 128 scores keeps the four special-function units of an SM 1,024 cycles, its
-// two products the tensor cores 512.
+// two products the tensor cores 512. A quarter of the exponentials are formed by multiply-adds (none 240 us, an eighth 241, a quarter
+// 237, three eighths 250 where it was measured).
+//
+// Eight trees of 63 nodes behind 32,768 keys, 32 heads over 8: 233 us, 581 TFLOP/s (the keys and values alone would take 82 us). Half of
+// that is handing over: with the exponentials taken out it still took 134 us, a tile waiting for the other role about as long as it
+// computes, and the two tiles of a CTA cover only part of one another's waits. Two CTAs an SM with blocks of 64 keys (258 us), a product
+// warp a tile (240), the next half block's scores loaded under this half's exponentials (304, more code than the instruction cache
+// holds) and fewer barriers a block (246) were slower.
 //
 // Every wait on an mbarrier is bounded: a role that gives up sets CELLM_DEV_WAIT_TIMEOUT and an abort flag; the CTA frees its tensor
 // memory and returns.
@@ -415,7 +423,8 @@ bool encode_rows(CUtensorMap* out, const void* base, int T, int heads, long long
 bool attention_tree_tc_takes(const TreeArgs& a) {
     const int G = a.nh / a.nkv;
     const uintptr_t at = (uintptr_t)a.q | (uintptr_t)a.k_new | (uintptr_t)a.v_new | (uintptr_t)a.k_pool | (uintptr_t)a.v_pool | (uintptr_t)a.out;
-    return a.hd == HD && a.scale_log2e > 0.f && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0 && G <= TM && TM / G * G >= 96 &&
+    return a.hd == HD && a.scale_log2e > 0.f && at % 16 == 0 && a.q_ld % 8 == 0 && a.k_ld % 8 == 0 && a.v_ld % 8 == 0 &&
+           a.q_ld > 0 && a.k_ld > 0 && a.v_ld > 0 && G <= TM && TM / G * G >= 96 &&
            a.num_pages > 0 && a.page_size >= 8 && a.page_size <= TN && (a.page_size & (a.page_size - 1)) == 0 && (long long)a.num_pages * a.nkv * a.page_size <= 0x7fffffffLL;
 }
 

@@ -132,7 +132,10 @@ __device__ __forceinline__ void ring_read(float (&x)[HALF_VALUES], const Ring<T>
 }
 
 // tops [rows][parts * 32], sums [rows][parts * 2]. The warps of a grid that fills the SMs take parts in turn, the next halves on their
-// way through a ring of the warp's own while it works on one.
+// way through a ring of the warp's own while it works on one. 512 rows of 65,536 32-bit logits (134 MB): 29 us,
+// 4.6 TB/s, with 56 % of the issue slots taken: neither limit is reached, a warp's halves wait in turn for memory and for one another's
+// instructions (pick included, 83 us with the warps loading in step, 51 with the ring and exponentials of any sign, 42 with those below
+// the best alone).
 template <typename T>
 __global__ void __launch_bounds__(ROW_WARPS * 32, Ring<T>::BLOCKS)
 beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* __restrict__ logits, long long ld, int V, int parts, int rows,
@@ -244,6 +247,8 @@ __device__ void sort_found(const Found& f, Best& to, int n, int keep) {
     __syncthreads();
 }
 
+// A block a request, so that no launch comes behind it: 512 rows of 64 requests 10 us, bound by its barriers (a dozen phases of few
+// instructions each) and not by its reads.
 template <typename T>
 __global__ void __launch_bounds__(PICK_THREADS)
 beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, int* __restrict__ out_tokens, const float* __restrict__ tops,
@@ -450,7 +455,8 @@ __device__ __forceinline__ void read_parents(int* to, const int* parents, int r,
     }
 }
 
-// grid (blocks over a slot's units, items, requests); state [items][slots][units] of W
+// grid (blocks over a slot's units, items, requests); state [items][slots][units] of W. Bound by memory: 8 requests of 8 beams that all
+// move, 10 layers of 1 MB a state, 1 GB in all: 177 us, 89 % of a plain copy's rate.
 template <int KMAX, typename W>
 __global__ void __launch_bounds__(256)
 reorder_states_kernel(W* state, const int* __restrict__ slot_ids, const int* __restrict__ parents, int beams, int slots, long long units, int* __restrict__ err) {
@@ -483,7 +489,9 @@ constexpr int PAGE_ROWS = 8;                  // rows of a beam that a block loo
 
 // grid (blocks over rows, items * pools, requests); a beam's row of the block table names the pages of its rows. Rows starts[r] ..
 // ends[r] - 1 of every beam of request r take those of its parent. An entry of -1 is a page that was given back: its rows are passed
-// over. The places of PAGE_ROWS rows of all beams are looked up once, into shared memory.
+// over. The places of PAGE_ROWS rows of all beams are looked up once, into shared memory. Bound by memory: 16 requests of 8 beams, 1 GB
+// read and written: 162 us, 95 % of a plain copy's rate (275 us with neighbouring threads on a position's heads, which lie far apart;
+// 219 us with a launch a pool).
 template <int KMAX, typename W>
 __global__ void __launch_bounds__(256)
 reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ starts, const int* __restrict__ ends,

@@ -6,7 +6,8 @@
 // parent (the smallest stays), and the walk then follows one word a step.
 //
 // The kept rows of all layers are written to places ctx, ctx + 1, ... of the request's pages. Every block repeats the walk
-// (a microsecond at most) and takes its share of the copies, so that one launch does it all.
+// (a microsecond at most) and takes its share of the copies, so that one launch does it all. Bound by latency: one tree of 8 nodes takes
+// 2.8 us in a CUDA graph, 64 trees of 63 nodes with 16 layers' rows 7.4 us (17 MB, 2.6 us at a copy's rate).
 #include <algorithm>
 
 #include "draft_tree.cuh"

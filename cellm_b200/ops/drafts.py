@@ -83,9 +83,10 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     plan = _plan(B, most, nh, nkv, hd, keys + most, tag, _SM_COUNT.get(index) or sm_count(index))
     nsplit, parts, part_o, part_ml = plan & 0xff, plan >> 8 & 0xff, 0, 0
     if parts:
-        ws = parents.new_empty(parts * T * nh * (hd + 2))              # of 32-bit words: the pieces' outputs, then maxima and sums
+        outputs = parts * T * nh * hd + 1 & ~1                         # (what follows them is read in pairs)
+        ws = parents.new_empty(outputs + parts * T * nh * 2)           # of 32-bit words: the pieces' outputs, then maxima and sums
         part_o = ws.data_ptr()
-        part_ml = part_o + 4 * parts * T * nh * hd
+        part_ml = part_o + 4 * outputs
     launch_packed("attention_tree", "attention_tree", index,
                   _TREE_ARGS(out.data_ptr(), part_o, part_ml, q.data_ptr(), q_ld, k_new.data_ptr(), k_ld, v_new.data_ptr(), v_ld, parents.data_ptr(), k_pool.data_ptr(),
                              v_pool.data_ptr(), cu_seqlens.data_ptr(), ctx_lens.data_ptr(), block_table.data_ptr(), entries, B, T, most, pages, page_size, nh, nkv, hd,

@@ -276,6 +276,24 @@ def test_trees_without_nodes_keep_nothing():
     assert count.shape == after.shape == (0,) and path.shape == (0, 3) and e.item() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,ctx", [(33, 4000), (65, 9000), (64, 9000)])
+def test_one_node_behind_a_long_context(dtype, hd, ctx):
+    """One row whose keys are cut into an odd number of pieces, more than a cluster has."""
+    x = make(np.random.RandomState(hd), dtype, [1], [ctx], 1, 1, hd, 16)
+    check(x, run(x))
+
+
+def test_one_row_for_all_nodes():
+    """Rows that are one row in memory (expanded), for few nodes and for as many as tiles of 128 rows are filled with."""
+    r = np.random.RandomState(8)
+    for n in (5, 40):
+        x = make(r, torch.bfloat16, [n], [70], 8, 2, 64, 16)
+        for name in ("q", "k_new", "v_new"):
+            x[name] = x[name][:1].expand(n, -1)
+        check(x, run(x))
+
+
 def test_an_empty_cache():
     """Trees of requests without a committed token, over a pool without pages."""
     r = np.random.RandomState(4)
