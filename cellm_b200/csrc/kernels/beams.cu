@@ -435,15 +435,21 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
 }
 
 // ---------------------------------------------------------------- reordering
-template <int KMAX, typename W, typename Place>
-__device__ __forceinline__ void reorder_unit(int beams, const int* parents, const Place& place) {
+// One unit of all beams: out of source(k), into target(k), below zero: that beam's stays. The places lie in shared memory and are read
+// again for the stores: kept in registers they would take more of those than the units do.
+template <int KMAX, typename W, typename Source, typename Target>
+__device__ __forceinline__ void reorder_unit(int beams, W* base, const Source& source, const Target& target) {
     W held[KMAX];
 #pragma unroll
-    for (int k = 0; k < KMAX; ++k)
-        if (k < beams && parents[k] >= 0) held[k] = *place(parents[k]);
+    for (int k = 0; k < KMAX; ++k) {
+        if (k >= beams) continue;
+        const long long at = source(k);
+        if (at >= 0) held[k] = base[at];
+    }
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int k = 0; k < KMAX; ++k)
-        if (k < beams && parents[k] >= 0) *place(k) = held[k];
+        if (k < beams && source(k) >= 0) base[target(k)] = held[k];
 }
 
 // The parents of request r into shared memory: -1 for a beam that stays as it is (its own parent, none, or one that is reported).
@@ -456,12 +462,13 @@ __device__ __forceinline__ void read_parents(int* to, const int* parents, int r,
 }
 
 // grid (blocks over a slot's units, items, requests); state [items][slots][units] of W. Bound by memory: 8 requests of 8 beams that all
-// move, 10 layers of 1 MB a state, 1 GB in all: 177 us, 89 % of a plain copy's rate.
+// move, 10 layers of 1 MB a state, 1 GB in all: 147 us, 7.0 TB/s (a parent of several beams is read once; 176 us with every beam's two
+// places in registers, three blocks an SM). 16 beams 7.2 TB/s, 32 beams (206 registers, a block an SM) 5.5.
 template <int KMAX, typename W>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, KMAX <= 8 ? 4 : 1)
 reorder_states_kernel(W* state, const int* __restrict__ slot_ids, const int* __restrict__ parents, int beams, int slots, long long units, int* __restrict__ err) {
     __shared__ int from[MAX_BEAMS];
-    __shared__ long long slot_at[MAX_BEAMS];
+    __shared__ long long slot_at[MAX_BEAMS], source_at[MAX_BEAMS];
     pdl_wait();
     const int r = blockIdx.z;
     read_parents(from, parents, r, beams, err);
@@ -473,11 +480,11 @@ reorder_states_kernel(W* state, const int* __restrict__ slot_ids, const int* __r
     }
     __syncthreads();
     // a beam without a slot, or whose parent has none, is left alone
-    if (threadIdx.x < beams && from[threadIdx.x] >= 0 && (slot_at[threadIdx.x] < 0 || slot_at[from[threadIdx.x]] < 0)) from[threadIdx.x] = -1;
+    if (threadIdx.x < beams) source_at[threadIdx.x] = from[threadIdx.x] >= 0 && slot_at[threadIdx.x] >= 0 ? slot_at[from[threadIdx.x]] : -1;
     __syncthreads();
     W* item = state + (long long)blockIdx.y * slots * units;
     for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256)
-        reorder_unit<KMAX, W>(beams, from, [&](int k) { return item + slot_at[k] + u; });
+        reorder_unit<KMAX, W>(beams, item + u, [&](int k) { return source_at[k]; }, [&](int k) { return slot_at[k]; });
 }
 
 // What reorder_pages works on: up to two pools [items][pages][nkv][page_size][units] of W that share their pages.
@@ -485,19 +492,18 @@ struct PagedPools {
     void* pool[2];
     int units[2], pools;
 };
-constexpr int PAGE_ROWS = 8;                  // rows of a beam that a block looks up and moves at a time
 
 // grid (blocks over rows, items * pools, requests); a beam's row of the block table names the pages of its rows. Rows starts[r] ..
 // ends[r] - 1 of every beam of request r take those of its parent. An entry of -1 is a page that was given back: its rows are passed
-// over. The places of PAGE_ROWS rows of all beams are looked up once, into shared memory. Bound by memory: 16 requests of 8 beams, 1 GB
-// read and written: 162 us, 95 % of a plain copy's rate (275 us with neighbouring threads on a position's heads, which lie far apart;
+// over. The places of ROWS rows of all beams are looked up once, into shared memory. Bound by memory: 16 requests of 8 beams, 1 GB
+// read and written: 160 us, 96 % of a plain copy's rate (275 us with neighbouring threads on a position's heads, which lie far apart;
 // 219 us with a launch a pool).
-template <int KMAX, typename W>
+template <int KMAX, int ROWS, typename W>
 __global__ void __launch_bounds__(256)
 reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, int bt_stride, const int* __restrict__ starts, const int* __restrict__ ends,
                      const int* __restrict__ parents, int beams, int pages, int nkv, int page_size, int* __restrict__ err) {
     __shared__ int from[MAX_BEAMS];
-    __shared__ long long row_at[KMAX][PAGE_ROWS];        // a row's place in its item, in units; -1: it has none
+    __shared__ long long row_at[KMAX][ROWS], source_at[KMAX][ROWS];        // a row's place in its item, in units; -1: it has none
     pdl_wait();
     const int r = blockIdx.z, which = blockIdx.y % p.pools;
     const unsigned units = (unsigned)(which ? p.units[1] : p.units[0]);
@@ -506,29 +512,27 @@ reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, in
     if (end < ends[r] && threadIdx.x == 0) atomicOr(err, CELLM_DEV_BAD_PAGE);
     const unsigned per_row = (unsigned)nkv * units, head = (unsigned)page_size * units;
     W* item = static_cast<W*>(which ? p.pool[1] : p.pool[0]) + (size_t)(blockIdx.y / p.pools) * pages * per_row * page_size;
-    for (int at = begin + blockIdx.x * PAGE_ROWS; at < end; at += gridDim.x * PAGE_ROWS) {
-        const unsigned rows = min(PAGE_ROWS, end - at);
+    for (int at = begin + blockIdx.x * ROWS; at < end; at += gridDim.x * ROWS) {
+        const unsigned rows = min(ROWS, end - at);
         __syncthreads();
-        for (int i = threadIdx.x; i < beams * PAGE_ROWS; i += 256) {
-            const int k = i / PAGE_ROWS, j = i % PAGE_ROWS;
+        for (int i = threadIdx.x; i < beams * ROWS; i += 256) {
+            const int k = i / ROWS, j = i % ROWS;
             if (j >= (int)rows) continue;
             const int page = block_table[((long long)r * beams + k) * bt_stride + (at + j) / page_size];
             if (page >= pages) atomicOr(err, CELLM_DEV_BAD_PAGE);
             row_at[k][j] = page < 0 || page >= pages ? -1 : ((long long)page * nkv * page_size + (at + j) % page_size) * units;
         }
         __syncthreads();
+        for (int i = threadIdx.x; i < beams * ROWS; i += 256) {
+            const int k = i / ROWS, j = i % ROWS;
+            if (j < (int)rows) source_at[k][j] = from[k] >= 0 && row_at[k][j] >= 0 ? row_at[from[k]][j] : -1;
+        }
+        __syncthreads();
         // neighbouring threads take a head's rows one behind the other, which lie so on their page
-        for (unsigned u = threadIdx.x; u < PAGE_ROWS * per_row; u += 256) {
-            const unsigned x = u % units, j = u / units % PAGE_ROWS, h = u / units / PAGE_ROWS;
+        for (unsigned u = threadIdx.x; u < ROWS * per_row; u += 256) {
+            const unsigned x = u % units, j = u / units % ROWS, h = u / units / ROWS;
             if (j >= rows) continue;
-            W* place = item + (size_t)h * head + x;
-            W held[KMAX];
-#pragma unroll
-            for (int k = 0; k < KMAX; ++k)
-                if (k < beams && from[k] >= 0 && row_at[from[k]][j] >= 0 && row_at[k][j] >= 0) held[k] = place[row_at[from[k]][j]];
-#pragma unroll
-            for (int k = 0; k < KMAX; ++k)
-                if (k < beams && from[k] >= 0 && row_at[from[k]][j] >= 0 && row_at[k][j] >= 0) place[row_at[k][j]] = held[k];
+            reorder_unit<KMAX, W>(beams, item + (size_t)h * head + x, [&](int k) { return source_at[k][j]; }, [&](int k) { return row_at[k][j]; });
         }
     }
 }
@@ -537,8 +541,9 @@ template <typename W>
 int launch_states(void* state, const int* slot_ids, const int* parents, int requests, int beams, int items, int slots, long long bytes, int* err,
                   cudaStream_t stream) {
     const long long units = bytes / (long long)sizeof(W);
-    const unsigned blocks = (unsigned)std::min<long long>((units + 255) / 256, 4096);
-    const dim3 grid(blocks, (unsigned)items, (unsigned)requests);
+    long long blocks = std::min<long long>((units + 255) / 256, 4096);
+    if (blocks * items * requests > 4096) blocks = (blocks + 1) / 2;                        // (two units a thread, one behind the other)
+    const dim3 grid((unsigned)blocks, (unsigned)items, (unsigned)requests);
 #define GO(K_) CELLM_RUN((reorder_states_kernel<K_, W>), grid, 256, 0, stream, (W*)state, slot_ids, parents, beams, slots, units, err)
     if (beams <= 4) GO(4);
     else if (beams <= 8) GO(8);
@@ -552,14 +557,18 @@ template <typename W>
 int launch_pages(PagedPools p, const int* block_table, int bt_stride, const int* starts, const int* ends, const int* parents, int requests, int beams,
                  int items, int pages, int nkv, int page_size, int sms, int* err, cudaStream_t stream) {
     for (int i = 0; i < p.pools; ++i) p.units[i] /= (int)sizeof(W);
-    const long long most = ((long long)bt_stride * page_size + PAGE_ROWS - 1) / PAGE_ROWS, rest = (long long)items * p.pools * requests;
-    const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>(most, 64ll * sms / rest));
+    const long long most = (long long)bt_stride * page_size, rest = (long long)items * p.pools * requests;
+    // Few beams have little to move between two look-ups: 32 rows at a time where that leaves every SM two blocks (2 beams, 330 MB: 68 us
+    // for 84 with 8; 4 beams 76 for 82; 8 beams 86 for 81).
+    const int rows = beams <= 4 && most * rest > 64ll * sms ? 32 : 8;
+    const unsigned blocks = (unsigned)std::max<long long>(1, std::min<long long>((most + rows - 1) / rows, 128ll * sms / rest));
     const dim3 grid(blocks, (unsigned)(items * p.pools), (unsigned)requests);
-#define GO(K_) CELLM_RUN((reorder_pages_kernel<K_, W>), grid, 256, 0, stream, p, block_table, bt_stride, starts, ends, parents, beams, pages, nkv, page_size, err)
-    if (beams <= 4) GO(4);
-    else if (beams <= 8) GO(8);
-    else if (beams <= 16) GO(16);
-    else GO(32);
+#define GO(K_, R_) CELLM_RUN((reorder_pages_kernel<K_, R_, W>), grid, 256, 0, stream, p, block_table, bt_stride, starts, ends, parents, beams, pages, nkv, page_size, err)
+    if (beams <= 4 && rows == 32) GO(4, 32);
+    else if (beams <= 4) GO(4, 8);
+    else if (beams <= 8) GO(8, 8);
+    else if (beams <= 16) GO(16, 8);
+    else GO(32, 8);
 #undef GO
     return CELLM_OK;
 }
@@ -626,7 +635,8 @@ CELLM_API int cellm_reorder_pages(void* k_pool, int k_bytes, void* v_pool, int v
     const PagedPools p = {{k_pool, v_pool}, {k_bytes, v_bytes}, v_pool ? 2 : 1};
     const uintptr_t at = (uintptr_t)k_pool | (uintptr_t)k_bytes | (v_pool ? (uintptr_t)v_pool | (uintptr_t)v_bytes : 0);
 #define GO(W_) return launch_pages<W_>(p, block_table, bt_stride, starts, ends, parents, requests, beams, items, pages, nkv, page_size, sms, err, stream)
-    if (at % 16 == 0) GO(uint4);
+    if (at % 16 == 0 && beams <= 16) GO(uint4);
+    if (at % 8 == 0) GO(uint2);              // (32 beams in units of 16 bytes leave no registers for a second block: 117 us for 103)
     if (at % 4 == 0) GO(uint32_t);
     if (at % 2 == 0) GO(uint16_t);
 #undef GO

@@ -164,6 +164,29 @@ def test_cached_rows_follow_their_beams(dtype, R, K, items, nkv, page, hd, vd):
     assert e.item() == 0 and all(torch.equal(p, w) for p, w in zip(pools, want))
 
 
+@pytest.mark.parametrize("K", [2, 3, 4, 20])
+@pytest.mark.parametrize("hd", [8, 4, 2])
+def test_pages_of_many_rows(K, hd):
+    """Enough rows that blocks look many of them up at a time; starts and ends inside and outside of such runs; units of 16, 8 and 4 bytes."""
+    from cellm_b200 import ops
+    r = np.random.RandomState(K + hd)
+    R, items, nkv, page, entries = 6, 3, 2, 16, 50
+    pool = torch.randn(items, R * K * entries, nkv, page, hd, device=DEV).to(torch.bfloat16)
+    table, parents = r.permutation(R * K * entries).reshape(R * K, entries), some_parents(r, R, K)
+    starts, ends = [0, 33, 500, 7, 64, 799], [800, 797, 501, 7, 96, 800]
+    places = torch.from_numpy(table[:, np.arange(800) // page] * page + np.arange(800) % page).to(DEV)      # of every beam's rows, in a pool of single rows
+    rows = pool.permute(0, 2, 1, 3, 4).reshape(items * nkv, -1, hd)
+    want = rows.clone()
+    for q in range(R):
+        for k in range(K):
+            if parents[q, k] >= 0:
+                to, src = (places[q * K + x, starts[q]:ends[q]] for x in (k, int(parents[q, k])))
+                want[:, to] = rows[:, src]
+    e = err_word()
+    ops.reorder_pages(pool, None, ints(table), ints(starts), ints(ends), ints(parents), e)
+    assert e.item() == 0 and torch.equal(pool.permute(0, 2, 1, 3, 4).reshape(items * nkv, -1, hd), want)
+
+
 def test_bad_parents_slots_and_pages_are_reported_and_passed_over():
     from cellm_b200 import ops
     state = torch.arange(5.0, device=DEV).repeat(2, 1).unsqueeze(2).contiguous()
