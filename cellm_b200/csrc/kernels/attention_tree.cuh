@@ -4,8 +4,8 @@
 
 struct TreeArgs {
     void* out;                    // [T, nh * hd]
-    float* part_o;                // [nsplit, T * nh, hd], where the keys are cut
-    float* part_ml;               // [nsplit, T * nh, 2]
+    float* part_o;                // [pieces, T * nh, hd], where pieces meet in the workspace
+    float* part_ml;               // [pieces, T * nh, 2]
     const void *q, *k_new, *v_new;   // rows of node t at q + t * q_ld, k_new + t * k_ld, ...
     long long q_ld, k_ld, v_ld;   // in elements
     const int* parents;           // [T]
