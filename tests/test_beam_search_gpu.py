@@ -1,6 +1,7 @@
 """Beam search through the engine against a search over the plain 64-bit model: scores of every place, sums of log probabilities of what
 comes back, ends of sequence, prompts in portions, several prompts at once, windows (Padadra), and what it refuses."""
 import dataclasses
+import importlib
 import re
 
 import pytest
@@ -134,6 +135,31 @@ def test_windows_give_back_the_same_pages_of_all_beams(tmp_path):
     got = tight.beam_search([prompt], beams=4, max_new_tokens=12, stop_eos=False)[0]
     assert [b.score for b in got] == pytest.approx([b.score for b in want], abs=2e-3)
     assert tight.stats()["free_pages"] == tight.stats()["total_pages"]
+
+
+@pytest.mark.parametrize("config", ["a", "b", "c", "d"])
+@pytest.mark.parametrize("design", ["vezalorn", "tufadra", "padadra", "bozovik", "tikizen", "gonozen"])
+def test_beams_of_every_design(tmp_path, design, config):
+    """Caches of every kind in the order of the beams: what a search says of its beams is what one run over prompt and beam says. Either
+    run is off by some 1e-5 of the logits' size (32 bits), a token's log probability by twice that: far below 2e-3 over nine tokens;
+    a state or a row of another beam's moves a score by hundredths at least."""
+    from cellm_b200 import Engine
+    from cellm_b200.engine.step import StepEntry
+    made = importlib.import_module(f"test_{design}_gpu")
+    folder = made.write_model(tmp_path / "m", made.CONFIGS[config], 31)
+    eng = Engine(folder, dtype="float32", tokens_per_block=8, total_blocks=160, max_num_seqs=10, prefill_chunk=16)
+    V = eng.plan.vocab_size
+    prompts = [[(11 * i + 5) % V for i in range(45)], [7 % V, 3 % V]]
+    out = eng.beam_search(prompts, beams=5, max_new_tokens=9, stop_eos=False)
+    assert eng.stats()["free_pages"] == eng.stats()["total_pages"]
+    for prompt, found in zip(prompts, out):
+        assert len(found) == 5 and len({tuple(b.tokens) for b in found}) == 5
+        for n, b in enumerate(found):
+            eng.cache.add(10 ** 6 + n)
+            whole = prompt + b.tokens[:-1]
+            lp = torch.log_softmax(eng.runner.run([StepEntry(10 ** 6 + n, whole, list(range(len(prompt) - 1, len(whole))))]).double(), -1)
+            eng.cache.release(10 ** 6 + n)
+            assert b.score == pytest.approx(float(lp[range(9), b.tokens].sum()), abs=2e-3)
 
 
 def test_refusals(folders):
