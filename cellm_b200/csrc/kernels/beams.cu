@@ -435,22 +435,33 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
 }
 
 // ---------------------------------------------------------------- reordering
-// One unit of all beams: out of source(k), into target(k), below zero: that beam's stays. The places lie in shared memory and are read
-// again for the stores: kept in registers they would take more of those than the units do.
-template <int KMAX, typename W, typename Source, typename Target>
-__device__ __forceinline__ void reorder_unit(int beams, W* base, const Source& source, const Target& target) {
-    W held[KMAX];
+// U units of all beams, `step` apart, of which the first `left` exist: out of source(k), into target(k), below zero: that beam's stay.
+// The places lie in shared memory and are read again for the stores: kept in registers they would take more of those than the units do.
+template <int KMAX, int U, typename W, typename Source, typename Target>
+__device__ __forceinline__ void reorder_units(int beams, W* base, int step, int left, const Source& source, const Target& target) {
+    W held[KMAX][U];
 #pragma unroll
     for (int k = 0; k < KMAX; ++k) {
         if (k >= beams) continue;
         const long long at = source(k);
-        if (at >= 0) held[k] = base[at];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (at >= 0 && i < left) held[k][i] = base[at + i * step];
     }
     asm volatile("" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < KMAX; ++k)
-        if (k < beams && source(k) >= 0) base[target(k)] = held[k];
+    for (int k = 0; k < KMAX; ++k) {
+        if (k >= beams || source(k) < 0) continue;
+        const long long at = target(k);
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+            if (i < left) base[at + i * step] = held[k][i];
+    }
 }
+// Units narrower than 16 bytes that a thread of reorder_states has under way at once: what 32 registers hold of all beams (2 beams in units
+// of 4 bytes, 336 MB: 58 us; 185 with one, which leaves too few bytes under way).
+template <int KMAX, typename W>
+constexpr int UNITS_AT_ONCE = KMAX >= 32 || sizeof(W) == 16 ? 1 : 32 / KMAX;
 
 // The parents of request r into shared memory: -1 for a beam that stays as it is (its own parent, none, or one that is reported).
 __device__ __forceinline__ void read_parents(int* to, const int* parents, int r, int beams, int* err) {
@@ -483,8 +494,9 @@ reorder_states_kernel(W* state, const int* __restrict__ slot_ids, const int* __r
     if (threadIdx.x < beams) source_at[threadIdx.x] = from[threadIdx.x] >= 0 && slot_at[threadIdx.x] >= 0 ? slot_at[from[threadIdx.x]] : -1;
     __syncthreads();
     W* item = state + (long long)blockIdx.y * slots * units;
-    for (long long u = (long long)blockIdx.x * 256 + threadIdx.x; u < units; u += (long long)gridDim.x * 256)
-        reorder_unit<KMAX, W>(beams, item + u, [&](int k) { return source_at[k]; }, [&](int k) { return slot_at[k]; });
+    constexpr int U = UNITS_AT_ONCE<KMAX, W>;
+    for (long long u = (long long)blockIdx.x * (256 * U) + threadIdx.x; u < units; u += (long long)gridDim.x * (256 * U))
+        reorder_units<KMAX, U, W>(beams, item + u, 256, U == 1 ? 1 : (int)min((long long)U, (units - u + 255) / 256), [&](int k) { return source_at[k]; }, [&](int k) { return slot_at[k]; });
 }
 
 // What reorder_pages works on: up to two pools [items][pages][nkv][page_size][units] of W that share their pages.
@@ -532,7 +544,7 @@ reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, in
         for (unsigned u = threadIdx.x; u < ROWS * per_row; u += 256) {
             const unsigned x = u % units, j = u / units % ROWS, h = u / units / ROWS;
             if (j >= rows) continue;
-            reorder_unit<KMAX, W>(beams, item + (size_t)h * head + x, [&](int k) { return source_at[k][j]; }, [&](int k) { return row_at[k][j]; });
+            reorder_units<KMAX, 1, W>(beams, item + (size_t)h * head + x, 0, 1, [&](int k) { return source_at[k][j]; }, [&](int k) { return row_at[k][j]; });
         }
     }
 }
@@ -541,10 +553,12 @@ template <typename W>
 int launch_states(void* state, const int* slot_ids, const int* parents, int requests, int beams, int items, int slots, long long bytes, int* err,
                   cudaStream_t stream) {
     const long long units = bytes / (long long)sizeof(W);
-    long long blocks = std::min<long long>((units + 255) / 256, 4096);
-    if (blocks * items * requests > 4096) blocks = (blocks + 1) / 2;                        // (two units a thread, one behind the other)
-    const dim3 grid((unsigned)blocks, (unsigned)items, (unsigned)requests);
-#define GO(K_) CELLM_RUN((reorder_states_kernel<K_, W>), grid, 256, 0, stream, (W*)state, slot_ids, parents, beams, slots, units, err)
+    auto grid = [&](int at_once) {
+        long long blocks = std::min<long long>((units + 256 * at_once - 1) / (256 * at_once), 4096);
+        if (at_once == 1 && blocks * items * requests > 4096) blocks = (blocks + 1) / 2;        // (two units a thread, one behind the other)
+        return dim3((unsigned)blocks, (unsigned)items, (unsigned)requests);
+    };
+#define GO(K_) CELLM_RUN((reorder_states_kernel<K_, W>), grid(UNITS_AT_ONCE<K_, W>), 256, 0, stream, (W*)state, slot_ids, parents, beams, slots, units, err)
     if (beams <= 4) GO(4);
     else if (beams <= 8) GO(8);
     else if (beams <= 16) GO(16);

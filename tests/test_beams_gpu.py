@@ -137,6 +137,25 @@ def test_states_follow_their_beams(dtype, R, K, items, shape):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("K", [2, 4, 7, 13, 20])
+@pytest.mark.parametrize("width", [2047, 2049, 4098, 5001, 70001])
+def test_states_of_odd_widths(dtype, K, width):
+    """Units of 2, 4 and 8 bytes, several of them a thread, and the last of a slot's among them."""
+    from cellm_b200 import ops
+    r = np.random.RandomState(width + K)
+    state = torch.randn(2, 2 * K + 1, width, device=DEV).to(dtype)
+    at, parents = r.permutation(2 * K + 1)[:2 * K], some_parents(r, 2, K)
+    want = state.clone()
+    for q in range(2):
+        for k in range(K):
+            if parents[q, k] >= 0:
+                want[:, at[q * K + k]] = state[:, at[q * K + parents[q, k]]]
+    e = err_word()
+    ops.reorder_states(state, ints(at), ints(parents), e)
+    assert torch.equal(state, want) and e.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("R,K,items,nkv,page,hd,vd", [(1, 4, 6, 8, 16, 64, 64), (3, 5, 1, 1, 3, 17, 17), (2, 32, 2, 2, 8, 32, 32), (2, 3, 2, 1, 16, 576, 0), (4, 9, 3, 2, 16, 96, 128)])
 def test_cached_rows_follow_their_beams(dtype, R, K, items, nkv, page, hd, vd):
     from cellm_b200 import ops
