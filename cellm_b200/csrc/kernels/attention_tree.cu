@@ -110,10 +110,11 @@ __device__ __forceinline__ void finish_rows(const TreeArgs& a, const TreeTile& t
 // warp its bandwidth was at 72 %). 32-bit rows on 16-byte borders (FAST) come in by cp.async, the next block while one is worked on;
 // others element by element. A block of 64 keys for 48 rows of 64 takes 10,000 cycles alone on an SM: 3,400 for the scores and 3,000 for
 // the output (their multiply-adds would be 3,072 of an SM's), 2,200 to issue the copies, 1,100 for the softmax. Five trees of 13 nodes
-// behind windows of 1,024 keys, 24 heads over 8: 31 us.
+// behind windows of 1,024 keys, 24 heads over 8: 31 us. Tiles of 16 rows take 32 keys at a time, so that an SM holds four: 29 trees of one
+// node behind 1,590 keys 92 us for 105 with 64, 16 behind 8,000 keys 178 for 249, one tree of 5 nodes behind 4,000 keys 29 for 26.
 template <int HDP, int RG, bool FAST>
 struct PlainTile {
-    static constexpr int RT = 16 * RG, KT = HDP <= 64 ? 64 : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
+    static constexpr int RT = 16 * RG, KT = HDP <= 64 ? (RG == 1 ? 32 : 64) : HDP <= 128 ? 32 : 16, LD = HDP + 4, ST = FAST ? 2 : 1;
     static constexpr int KG = RG == 3 || HDP > 128 ? 2 : 4, WK = KT / KG, THREADS = 32 * RG * KG, PLD = 20;
     static constexpr int KV = KT * LD;                                   // floats of a block's keys, and of its values
     static constexpr int O_FLOATS = KG * RT * (HDP + 2), RING = ST * 2 * KV > O_FLOATS ? ST * 2 * KV : O_FLOATS;     // the outputs meet where the ring was
@@ -760,8 +761,9 @@ TreePlan tree_plan(int B, int most, int nh, int nkv, int hd, int keys, int dtype
     }
     const bool mma = dtype == CELLM_BF16 && (hd == 32 || hd == 64 || hd == 96 || hd == 128);
     const int tile = mma ? (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) : dtype == CELLM_F32 ? plain_rows(rows, hd) : 32;
-    const int an_sm = hd <= 32 ? (mma ? 4 : 3) : mma && hd == 64 ? 3 : 2;     // blocks that an SM holds, by their shared memory
-    const int block = mma || hd <= 64 ? 64 : hd <= 128 ? 32 : 16;
+    const bool few = !mma && tile == 16 && hd <= 64;                          // (32-bit tiles of 16 rows)
+    const int an_sm = few ? 4 : hd <= 32 ? (mma ? 4 : 3) : mma && hd == 64 ? 3 : 2;     // blocks that an SM holds, by their shared memory
+    const int block = few ? 32 : mma || hd <= 64 ? 64 : hd <= 128 ? 32 : 16;
     const int n = pieces((long long)B * nkv * ((rows + tile - 1) / tile), (keys + block - 1) / block, (long long)an_sm * sms, true);
     return {false, n, n > CLUSTER_MAX ? n : 0};
 }
