@@ -19,7 +19,10 @@
 namespace {
 
 // ---------------------------------------------------------------- a tile's results
+// The barrier's forms here are executed by a warp as a whole; what comes before may have taken its lanes through loops of different
+// lengths (two rows a warp, columns that are no multiple of 32), so they meet first.
 __device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }

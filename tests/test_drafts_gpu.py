@@ -284,6 +284,18 @@ def test_one_node_behind_a_long_context(dtype, hd, ctx):
     check(x, run(x))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,nodes,nh,nkv", [(40, 3, 3, 1), (72, 5, 1, 1), (33, 1, 5, 1), (96, 7, 3, 3), (200, 3, 1, 1), (64, 1, 3, 1)])
+@pytest.mark.parametrize("ctx", [130, 300, 517])
+def test_pieces_of_a_cluster_share_rows_unevenly(dtype, hd, nodes, nh, nkv, ctx):
+    """Two to eight pieces that merge in a cluster, each a share of the rows that is one row longer for one half of a warp than for the
+    other, rows whose last columns only some lanes hold."""
+    x = make(np.random.RandomState(hd + ctx), dtype, [nodes, nodes], [ctx, ctx - 70], nh, nkv, hd, 16)
+    out = run(x)
+    check(x, out)
+    assert torch.equal(run(x), out)
+
+
 def test_one_row_for_all_nodes():
     """Rows that are one row in memory (expanded), for few nodes and for as many as tiles of 128 rows are filled with."""
     r = np.random.RandomState(8)
