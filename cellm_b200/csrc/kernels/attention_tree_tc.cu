@@ -18,8 +18,11 @@
 // warp a tile (240), the next half block's scores loaded under this half's exponentials (304, more code than the instruction cache
 // holds) and fewer barriers a block (246) were slower.
 //
-// Every wait on an mbarrier is bounded: a role that gives up sets CELLM_DEV_WAIT_TIMEOUT and an abort flag; the CTA frees its tensor
-// memory and returns.
+// Every wait on an mbarrier is bounded: a role that gives up sets CELLM_DEV_WAIT_TIMEOUT and an abort flag; the CTA then waits (bounded
+// again) for the copies and products it has under way, frees its tensor memory and returns. The lanes of a warp wait together, by one
+// instruction on one barrier, so they give up together.
+#include <climits>
+
 #include "attention_tree.cuh"
 #include "pairs.cuh"
 #include "tcgen05_attn.cuh"
@@ -42,8 +45,9 @@ struct TreeTcSmem {                    // starts on a 1024-byte boundary (checke
     uint64_t k_full[KV_STAGES], k_empty[KV_STAGES];
     uint64_t v_full[KV_STAGES], v_empty[KV_STAGES];
     uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
+    uint64_t drained;            // by the products that an abort has left under way
     uint32_t tmem_base;
-    int abort_flag;
+    int abort_flag, never, issued[2];     // never: no abort; issued: blocks of keys and of values asked for before an abort
 };
 
 __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
@@ -95,7 +99,8 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             mbar_init(&sm.s_full[t], 1), mbar_init(&sm.s_empty[t], 128);
             mbar_init(&sm.p_full[t], 128), mbar_init(&sm.pv_done[t], 1);
         }
-        sm.abort_flag = 0;
+        mbar_init(&sm.drained, 1);
+        sm.abort_flag = sm.never = 0, sm.issued[0] = sm.issued[1] = INT_MAX;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         for (const CUtensorMap* map : {&map_q, &map_k, &map_v, &map_kn, &map_vn}) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
@@ -148,7 +153,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 bool ok = true;
                 if (lane == 0) ok = mbar_wait(keys ? &sm.k_empty[st] : &sm.v_empty[st], ((uint32_t)(j / KV_STAGES) & 1u) ^ 1u, abort_flag);
                 ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-                if (!ok) { if (lane == 0) { *abort_flag = 1; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } break; }
+                if (!ok) { if (lane == 0) { *abort_flag = 1; sm.issued[warp >> 1] = j; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } break; }
                 if (lane == 0) mbar_expect_tx(full, bytes);
                 __syncwarp();
                 if (have) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, paged_map, 0, (page * a.nkv + t.kvh) * a.page_size, full);
@@ -400,6 +405,19 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) {            // what is under way must not outlive this CTA's memory
+        if ((warp == 0 || warp == 2) && lane == 0 && live) {
+            const int issued = min(sm.issued[warp >> 1], n_blk);
+            if (warp == 0) mbar_wait(&sm.q_full, 0, &sm.never);
+            for (int j = max(0, issued - KV_STAGES); j < issued; ++j)
+                mbar_wait(warp == 0 ? &sm.k_full[j % KV_STAGES] : &sm.v_full[j % KV_STAGES], (uint32_t)(j / KV_STAGES) & 1u, &sm.never);
+        }
+        if (warp == 1 && elect_one()) {      // the lane that issued the products
+            umma_commit(&sm.drained);
+            mbar_wait(&sm.drained, 0, &sm.never);
+        }
+        __syncthreads();
+    }
     if (warp == 1) tmem_dealloc(tmem, TMEM_COLUMNS);
 }
 
