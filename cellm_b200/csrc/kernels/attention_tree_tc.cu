@@ -136,19 +136,22 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int* bt = a.block_table + (size_t)t.b * a.bt_stride;
             const int pages_per_block = TN / a.page_size;
             const CUtensorMap *paged_map = keys ? &map_k : &map_v, *node_map = keys ? &map_kn : &map_vn;
-            // lane i brings page i of a block; its entry of the table is asked for a block ahead. -2: nothing of it is seen
-            auto entry = [&](int j) {
+            // lane i brings page i of a block, if something of it is seen; its entry of the table is asked for a block ahead. A page that
+            // is none is reported and read from behind the pool's end, which is zeros.
+            const int behind = a.num_pages * a.nkv * a.page_size;
+            auto seen = [&](int j) {
                 const int key0 = (first + begin + j) * TN + lane * a.page_size;
-                return j < n_blk && begin + j < committed && lane < pages_per_block && key0 < t.ctx && key0 + a.page_size > lo ? bt[key0 / a.page_size] : -2;
+                return j < n_blk && begin + j < committed && lane < pages_per_block && key0 < t.ctx && key0 + a.page_size > lo;
             };
+            auto entry = [&](int j) { return seen(j) ? bt[((first + begin + j) * TN + lane * a.page_size) / a.page_size] : 0; };
             int next = entry(0);
             for (int j = 0; j < n_blk; ++j) {
                 const int st = j % KV_STAGES, blk = begin + j, page = next;
                 uint64_t* full = keys ? &sm.k_full[st] : &sm.v_full[st];
                 uint8_t* dst = keys ? sm.k[st] : sm.v[st];
                 next = entry(j + 1);
-                const bool paged = blk < committed, have = paged && page >= 0 && page < a.num_pages;
-                if (keys && page != -2 && !have) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                const bool paged = blk < committed, have = seen(j), none = page < 0 || page >= a.num_pages;
+                if (keys && have && none) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
                 const uint32_t bytes = paged ? (uint32_t)__popc(__ballot_sync(0xffffffffu, have)) * (uint32_t)a.page_size * HD * 2 : TN * HD * 2;
                 bool ok = true;
                 if (lane == 0) ok = mbar_wait(keys ? &sm.k_empty[st] : &sm.v_empty[st], ((uint32_t)(j / KV_STAGES) & 1u) ^ 1u, abort_flag);
@@ -156,7 +159,7 @@ attention_tree_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 if (!ok) { if (lane == 0) { *abort_flag = 1; sm.issued[warp >> 1] = j; atomicOr(a.err, CELLM_DEV_WAIT_TIMEOUT); } break; }
                 if (lane == 0) mbar_expect_tx(full, bytes);
                 __syncwarp();
-                if (have) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, paged_map, 0, (page * a.nkv + t.kvh) * a.page_size, full);
+                if (have) tma_load_2d(dst + (size_t)lane * a.page_size * HD * 2, paged_map, 0, none ? behind : (page * a.nkv + t.kvh) * a.page_size, full);
                 else if (!paged && lane == 0) tma_load_3d(dst, node_map, 0, t.kvh, t.t_base + (blk - committed) * TN, full);
             }
         }

@@ -48,7 +48,8 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     int32 [T] (see the module's text); pools [pages, nkv, page size, hd]; request b owns nodes cu_seqlens[b] .. cu_seqlens[b + 1], at
     most 256, and `tree_lens` is the host's copy of their numbers. `max_ctx`: the longest context if the host knows it (0: what the
     block table can name). float32 or bfloat16, heads of up to 256. Returns [T, nh * hd]; rows of no tree hold nothing of meaning. A row of K or V
-    that is not finite may reach every node of its tree. Nothing is read or written of padding and of page entries that no node sees."""
+    that is not finite may reach every node of its tree. Nothing is read or written of padding and of page entries that no node sees. A
+    page out of range that a node does see is reported in `err`, and its keys and values are zeros."""
     dtype, index, shape, table, T, B = q.dtype, q.get_device(), k_pool.shape, block_table.shape, q.shape[0], len(tree_lens)
     if index < 0 or dtype not in DTYPE_TAG or len(shape) != 4:
         raise ValueError("attention_tree: float32 or bfloat16 rows on the GPU over pools [pages, kv heads, page size, head size]")

@@ -184,6 +184,63 @@ def test_bad_pages_and_trees_are_reported_and_left_out(dtype):
     assert e.item() == 2
 
 
+def with_zeros(x, bad):
+    """The same trees with zeros on entries bad[b] of their requests' tables."""
+    pools = {z: x[z].clone() for z in "kv"}
+    for b, entries in enumerate(bad):
+        for z in "kv":
+            pools[z][[x["table"][b, e] for e in entries]] = 0.0
+    return dict(x, **pools)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes,nh,nkv,hd,page", [(6, 4, 2, 64, 16), (6, 4, 2, 128, 16), (13, 3, 1, 40, 5), (5, 2, 1, 256, 16), (70, 2, 1, 64, 16), (20, 8, 2, 64, 16),
+                                                  (40, 4, 1, 64, 128), (50, 6, 2, 64, 8)])
+@pytest.mark.parametrize("ctxs", [[100, 50, 37], [400, 1, 300]])
+def test_bad_pages_count_as_zeros(dtype, nodes, nh, nkv, hd, page, ctxs):
+    """Keys and values of a page that is none are zeros, in all of the kernels: the first, a middle one and the last page, all pages of a
+    request, a page in every second place; the trees beside them as without."""
+    check_bad_pages(np.random.RandomState(nodes + page + ctxs[0]), dtype, nodes, nh, nkv, hd, page, ctxs)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes,nh,nkv,hd", [(9, 8, 2, 64), (2, 2, 1, 128), (3, 1, 1, 48)])
+def test_bad_pages_in_front_of_pieces(dtype, nodes, nh, nkv, hd):
+    check_bad_pages(np.random.RandomState(nodes), dtype, nodes, nh, nkv, hd, 16, [2600, 130, 2100])
+
+
+def check_bad_pages(r, dtype, nodes, nh, nkv, hd, page, ctxs):
+    x = make(r, dtype, [nodes] * 3, ctxs, nh, nkv, hd, page)
+    good = run(x)
+    last = [-(-c // page) - 1 for c in ctxs]
+    for bad in ([{0}, set(), set()], [{last[0] // 2, last[0]}, set(), {0, last[2]}], [set(), set(range(last[1] + 1)), set(range(0, last[2], 2))]):
+        y = dict(x, table=x["table"].copy())
+        for b, entries in enumerate(bad):
+            for i, e in enumerate(sorted(entries)):
+                y["table"][b, e] = (-1, x["k"].shape[0], 10 ** 6, -2 ** 31)[i % 4]
+        e = err_word()
+        out = run(y, err=e)
+        assert e.item() == 2
+        check(with_zeros(x, bad), out)
+        for b in range(3):
+            if not bad[b]:
+                assert torch.equal(out[b * nodes:(b + 1) * nodes], good[b * nodes:(b + 1) * nodes])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes,hd", [(6, 64), (6, 128), (6, 40), (70, 64)])
+def test_a_bad_page_inside_a_window(dtype, nodes, hd):
+    """Every node's window holds the whole page, and begins inside another."""
+    x = make(np.random.RandomState(nodes + hd), dtype, [nodes], [100], 4, 2, hd, 16)
+    x["parents"] = [-1] + [0] * (nodes - 1)
+    y = dict(x, table=x["table"].copy())
+    y["table"][0, 4] = -1                               # keys 64 .. 79; the nodes see those from 52 or 53 on
+    e = err_word()
+    out = run(y, 49, err=e)
+    assert e.item() == 2
+    check(with_zeros(x, [{4}]), out, 49)
+
+
 def test_a_captured_call_follows_its_inputs():
     r = np.random.RandomState(8)
     x = make(r, torch.bfloat16, [9, 14], [700, 300], 8, 2, 64, 16)
