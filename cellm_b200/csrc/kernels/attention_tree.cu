@@ -205,7 +205,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
 #pragma unroll
         for (int it = 0; it < (FAST ? ITERS : 0); ++it) {
             const int blk = begin + i, at = threadIdx.x + it * L::THREADS, j = (first + blk) * KT + at / CHUNKS;
-            entry[it] = at < PIECES && i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
+            entry[it] = at < PIECES && i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -1;
         }
     };
     auto load = [&](int i) {
@@ -219,13 +219,12 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
                 const float *k = static_cast<const float*>(a.k_pool), *v = static_cast<const float*>(a.v_pool);
                 bool have = chunk * 4 < hd;
                 if (blk < committed) {
-                    const int page = entry[it];
+                    const int page = entry[it], j = (first + blk) * KT + row;
                     if (page >= 0 && page < a.num_pages) {
-                        const int j = (first + blk) * KT + row;
                         const size_t off = (size_t)page * page_elems + ((size_t)t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * hd + chunk * 4;
                         if (have) k += off, v += off;
                     } else {
-                        if (page != -2) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
+                        if (j >= lo && j < t.ctx) atomicOr(a.err, CELLM_DEV_BAD_PAGE);
                         have = false;
                     }
                 } else {
@@ -425,7 +424,7 @@ attention_tree_mma_kernel(const TreeArgs a) {
 #pragma unroll
         for (int it = 0; it < ITERS; ++it) {
             const int blk = begin + i, j = (first + blk) * BN + row_of(it);
-            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -2;
+            entry[it] = i < n_blk && blk < committed && j >= lo && j < t.ctx ? bt[shift >= 0 ? j >> shift : j / a.page_size] : -1;
         }
     };
     auto load_kv = [&](int i) {
@@ -442,7 +441,7 @@ attention_tree_mma_kernel(const TreeArgs a) {
                     if (page >= 0 && page < a.num_pages) {
                         const size_t off = (size_t)page * page_elems + ((size_t)t.kvh * a.page_size + (shift >= 0 ? j & (a.page_size - 1) : j % a.page_size)) * HD + chunk * 8;
                         k += off, v += off, have = true;
-                    } else if (page != -2) {
+                    } else if (j >= lo && j < t.ctx) {
                         atomicOr(a.err, CELLM_DEV_BAD_PAGE);
                     }
                 } else {

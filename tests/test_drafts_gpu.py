@@ -241,6 +241,22 @@ def test_a_bad_page_inside_a_window(dtype, nodes, hd):
     check(with_zeros(x, [{4}]), out, 49)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("nodes,hd", [(6, 64), (6, 128), (6, 40), (70, 64)])
+@pytest.mark.parametrize("entry", [-2, -3, -2 ** 31, 2 ** 31 - 1])
+def test_every_page_that_is_none_is_reported(dtype, nodes, hd, entry):
+    x = make(np.random.RandomState(nodes + hd), dtype, [nodes], [100], 4, 2, hd, 16)
+    for at in (0, 3, 6):
+        y = dict(x, table=x["table"].copy())
+        y["table"][0, at] = entry
+        e = err_word()
+        check(with_zeros(x, [{at}]), run(y, err=e))
+        assert e.item() == 2
+    y = dict(x, table=x["table"].copy())
+    y["table"][0, 0] = entry                                # in front of the window: nothing of it is looked at
+    check(x, run(y, 60), 60)
+
+
 def test_a_captured_call_follows_its_inputs():
     r = np.random.RandomState(8)
     x = make(r, torch.bfloat16, [9, 14], [700, 300], 8, 2, 64, 16)
