@@ -57,9 +57,10 @@ __device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
 }
 // 2^x of two numbers without the special-function units: x = n + f with |f| <= 1/2, n out of the rounding of an addition, 2^f = 1 + f
 // P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.8e-6 relative, a thousandth of what rounding
-// the weight to bfloat16 costs. What lies below -126, -inf too, gives 2^-126.
+// the weight to bfloat16 costs. What lies at -127 or below, -inf too, gives 0: a key that is not seen has no weight. (Between -127 and -126
+// the exponent's field is 0 and the result a denormal below 2^-126.)
 __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-    x = pair_of(fmaxf(low_of(x), -126.f), fmaxf(high_of(x), -126.f));
+    x = pair_of(fmaxf(low_of(x), -127.f), fmaxf(high_of(x), -127.f));
     const uint64_t r = add2(x, pair_of(12582912.f, 12582912.f)), n = add2(r, pair_of(-12582912.f, -12582912.f));
     const uint64_t f = fma2(n, pair_of(-1.f, -1.f), x);
     uint64_t p = pair_of(0.00958284828811884f, 0.00958284828811884f);

@@ -257,6 +257,29 @@ def test_every_page_that_is_none_is_reported(dtype, nodes, hd, entry):
     check(x, run(y, 60), 60)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 128, 40])
+@pytest.mark.parametrize("nodes,window", [(12, 0), (12, 20), (40, 0), (40, 20), (140, 20)])
+def test_what_a_node_does_not_see_has_no_weight(dtype, hd, nodes, window):
+    """Keys and values near the type's largest, finite, of nodes on other branches and of keys in front of a window: the outputs of the
+    nodes that do not see them are what they are with zeros there, bit for bit."""
+    r = np.random.RandomState(nodes + hd + window)
+    x = make(r, dtype, [nodes], [100], 4, 2, hd, 16)
+    x["parents"] = [-1] + [0] * (nodes - 1)
+    big = [i for i in range(1, nodes) if i % 5 == 2 or i % 16 == 1]             # (some at every place of a run of 16)
+    seen_by = set(big)
+    outs = []
+    for value in (0.0, 0.99 * torch.finfo(dtype).max):
+        y = dict(x, k_new=x["k_new"].clone(), v_new=x["v_new"].clone(), k=x["k"].clone(), v=x["v"].clone())
+        for i in big:
+            y["k_new"][i], y["v_new"][i] = value, -value
+        if window:                                          # key 81 stands in node 0's window alone
+            y["k"][x["table"][0, 5], :, 1], y["v"][x["table"][0, 5], :, 1] = value, value
+        outs.append(run(y, window))
+    others = [i for i in range(1 if window else 0, nodes) if i not in seen_by]
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[1][others], outs[0][others])
+
+
 def test_a_captured_call_follows_its_inputs():
     r = np.random.RandomState(8)
     x = make(r, torch.bfloat16, [9, 14], [700, 300], 8, 2, 64, 16)
