@@ -6,14 +6,16 @@
 //                      of its 2,048 exponentials.
 //   beam_pick_kernel   a block a request: the rows' log-sums, a lower bound of the worst wanted score out of the lanes' maxima
 //                      (the keep-th largest maximum of 128 disjoint sets of them), and the logits of the few lanes that reach it.
-// Scores of different beams are compared, so the sums behind them must be good to more than a logit's own rounding: the
-// exponentials carry an error of about 2^-25 each, their sums over lanes are 64-bit, and a score is the 64-bit sum
-// s + ((x - max) - log sum exp(x - max)).
+// Scores of different beams are compared, so the sums behind them must be good to more than a logit's own rounding, and where a row's
+// mass lies in many equal logits the errors of its exponentials add up: an exponential is off by 1.1e-7 of itself at most (mostly by
+// 2^-25), eight are summed in 32 bits (another 1.8e-7 at most), the rest in 64, and a score is the 64-bit sum
+// s + ((x - max) - log sum exp(x - max)), good to 3e-7.
 //
 // Reordering is done in place: a thread reads its 16 bytes (or what the rows' alignment allows) of ALL beams of a request
 // before it writes any, and no other thread touches those places, so no copy of the states is needed and no order of blocks
 // matters.
 #include <algorithm>
+#include <climits>
 
 #include "mma_tiles.cuh"
 #include "pairs.cuh"
@@ -26,20 +28,23 @@ constexpr int HALF_VALUES = LANE_VALUES / 2;
 constexpr int ROW_WARPS = 4;
 constexpr int MAX_BEAMS = 32, MAX_KEEP = 64, MAX_VOCAB = 1 << 24;
 
-// Of one half part's logits: the largest, and the sum of exp(x - best).
+// Of one half part's logits: the largest, and the sum of exp(x - unit). The unit is power * log 2, or the best where power is BY_BEST.
 struct RowPart {
     float best;
+    int power;
     double sum;
 };
+constexpr int BY_BEST = INT_MIN;
+constexpr float BY_BEST_FROM = 32768.f;       // the best's magnitude from which on it is the unit: x - best is exact there for all that counts
 
-// exp(x - best) of two numbers, best the largest. d log2 e = n + f with |f| <= 1/2 comes out of the rounding of one addition and a
-// multiply-add; 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9. What matters lies
-// near the best, where d is exact. What is smaller than exp(-86), or not a number, adds exp(-86): nothing.
-__device__ __forceinline__ uint64_t exp_below(float a, float b, uint64_t minus_best) {
-    const uint64_t raw = add2(pair_of(a, b), minus_best), l2e = pair_of(1.4426950408889634f, 1.4426950408889634f);
-    const uint64_t d = pair_of(fmaxf(low_of(raw), -86.f), fmaxf(high_of(raw), -86.f));
-    const uint64_t magic = pair_of(12582912.f, 12582912.f);                  // 1.5 * 2^23: its sum holds a whole number in the low bits
-    const uint64_t r = fma2(d, l2e, magic), f = fma2(d, l2e, fma2(r, pair_of(-1.f, -1.f), magic));
+// 2^-p exp(x) of two numbers. x log2 e = n + f with |f| <= 1/2: n comes out of the rounding of a multiply-add whose addend (1.5 * 2^23 - p) also
+// takes p off, f out of two more that lose nothing of x (log2 e in two parts; x - best would be rounded where the two are far apart, and
+// alike for equal logits). 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9. What lies
+// below `least`, best - 86, or is not a number, adds exp(-86) of the best: nothing.
+__device__ __forceinline__ uint64_t exp_scaled(float a, float b, float least, uint64_t magic) {
+    const uint64_t x = pair_of(fmaxf(a, least), fmaxf(b, least)), l2e = pair_of(1.4426950408889634f, 1.4426950408889634f);
+    const uint64_t r = fma2(x, l2e, magic), rest = fma2(x, l2e, fma2(r, pair_of(-1.f, -1.f), magic));
+    const uint64_t f = fma2(x, pair_of(1.925963033500011537e-8f, 1.925963033500011537e-8f), rest);
     uint64_t p = pair_of(0.00015353357593994588f, 0.00015353357593994588f);
     p = fma2(p, f, pair_of(0.0013398876180872321f, 0.0013398876180872321f));
     p = fma2(p, f, pair_of(0.009618437848985195f, 0.009618437848985195f));
@@ -184,21 +189,33 @@ beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* 
         top = at.half ? fmaxf(top, mine) : mine;
         const float best = warp_max(mine);
         double sum = 0.0;
+        int power = BY_BEST;
         if (fabsf(best) < INFINITY) {                                         // (no logit at all, or one that has no meaning: no sum)
-            const uint64_t minus_best = pair_of(-best, -best);
-            uint64_t s0 = 0ull, s1 = 0ull;
+            float unit = best;
+            if (fabsf(best) < BY_BEST_FROM) {
+                unit = 0.f, power = __float2int_rn(best * 1.4426950408889634f);
+            } else {
 #pragma unroll
-            for (int k = 0; k < HALF_VALUES; k += 4) s0 = add2(s0, exp_below(x[k], x[k + 1], minus_best)), s1 = add2(s1, exp_below(x[k + 2], x[k + 3], minus_best));
-            s0 = add2(s0, s1);
-            sum = warp_sum_d((double)(low_of(s0) + high_of(s0)));
+                for (int k = 0; k < HALF_VALUES; ++k) x[k] -= best;
+            }
+            const float least = (best - unit) - 86.f, base = 12582912.f - (unit == 0.f ? (float)power : 0.f);
+            const uint64_t magic = pair_of(base, base);
+            auto quad = [&](int k) { return add2(exp_scaled(x[k], x[k + 1], least, magic), exp_scaled(x[k + 2], x[k + 3], least, magic)); };
+            auto eight = [&](int k) { return add2(quad(k), quad(k + 4)); };
+#pragma unroll
+            for (int k = 0; k < HALF_VALUES; k += 16) {                       // (by halves: equal numbers add up without a rounding)
+                const uint64_t s = add2(eight(k), eight(k + 8));
+                sum += (double)low_of(s) + (double)high_of(s);
+            }
+            sum = warp_sum_d(sum);
         }
         const long long part = (long long)at.row * parts + at.part;
-        if (lane == 0) sums[2 * part + at.half] = RowPart{best, sum};
+        if (lane == 0) sums[2 * part + at.half] = RowPart{best, power, sum};
         if (at.half) tops[part * 32 + lane] = top;
     }
 }
 
-// exp(d) for d <= 0 in 64 bits, to 2.0e-9: as exp_below. The picking block runs its code once, so what it calls is short.
+// exp(d) for d <= 1/2 in 64 bits, to 2.0e-9: as exp_scaled. The picking block runs its code once, so what it calls is short.
 __device__ __forceinline__ double exp_short(double d) {
     d = fmax(d, -600.0) * 1.4426950408889634074;
     const double n = rint(d), f = d - n;
@@ -214,6 +231,11 @@ __device__ __forceinline__ double exp_short(double d) {
 __device__ __forceinline__ double log_short(double s) {
     const double y = (double)logf((float)s);
     return y + (s * exp_short(-y) - 1.0);
+}
+
+// exp(unit - best) of a part's unit and the best of its row
+__device__ __forceinline__ double unit_over(const RowPart& w, float best) {
+    return exp_short((w.power == BY_BEST ? (double)w.best : w.power * 0.69314718055994530942) - (double)best);
 }
 
 constexpr int PICK_THREADS = 512, PICK_SETS = 128, PICK_ROOM = 1024, SUMS_HELD = 4, HELD = 16, HOT_ROOM = HELD * PICK_THREADS;
@@ -275,7 +297,7 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         RowPart w[SUMS_HELD];
 #pragma unroll
         for (int c = 0; c < SUMS_HELD; ++c) {
-            w[c] = RowPart{-INFINITY, 0.0};
+            w[c] = RowPart{-INFINITY, 0, 0.0};
             if (lane + c * 32 < 2 * parts) w[c] = p[lane + c * 32];
         }
         const double s = (double)scores[row];
@@ -288,9 +310,9 @@ beam_pick_kernel(float* __restrict__ out_scores, int* __restrict__ out_parents, 
         double sum = 0.0;
 #pragma unroll
         for (int c = 0; c < SUMS_HELD; ++c)
-            if (w[c].sum > 0.0) sum += w[c].sum * exp_short((double)w[c].best - (double)best);
+            if (w[c].sum > 0.0) sum += w[c].sum * unit_over(w[c], best);
         for (int i = lane + SUMS_HELD * 32; i < 2 * parts; i += 32)
-            if (p[i].sum > 0.0) sum += p[i].sum * exp_short((double)p[i].best - (double)best);
+            if (p[i].sum > 0.0) sum += p[i].sum * unit_over(p[i], best);
         sum = warp_sum_d(sum);
         if (lane == 0) {
             // nothing of a beam with no score, or of a row without a finite logit, is offered

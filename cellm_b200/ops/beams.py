@@ -18,7 +18,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, keep: int, done: Opt
     and equal ones by (k, v). logits [R * K, V] float32 or bfloat16 (rows may be strided; V up to 2^24), scores float32 [R, K], K and `keep` up
     to 32 and 64. done [R, K] bool: a finished beam offers itself alone, with token `pad`, at its score (its logits are not looked at).
     A beam with score -inf and a token with logit -inf (a NaN counts as one) are never chosen; logits of +inf have no meaning here.
-    Scores are compared in 64 bits; the sums behind them carry about 2^-25.
+    Scores are compared in 64 bits; the log-sums behind them are good to 3e-7, mostly to 2^-25.
 
     Returns (scores float32, parents int32, tokens int32), each [R, keep]; where a request has fewer continuations, -inf and -1."""
     index, shape, stride, pair = logits.get_device(), logits.shape, logits.stride(), scores.shape

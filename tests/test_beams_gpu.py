@@ -91,6 +91,27 @@ def test_rows_may_lie_apart_and_anywhere():
             check_selection(wide[:, lo:hi], scores, 6)
 
 
+# An exponential is off by 1.1e-7 of itself at most (its argument by two halves of 2^-25 units of log 2, the polynomial's last three
+# roundings by 2^-24, 2^-26 and less, its fit by 3e-9), sums of eight by three half steps of 2^-23; what follows is 64 bits.
+SUM_ERROR = 3.0e-7
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1024, 50257])
+@pytest.mark.parametrize("flat,top", [(0.1, 8.35), (1.3, 8.8), (-5.2, 1.9), (-40000.0, -39990.5), (32760.0, 32770.0), (0.3, 0.7)])
+def test_sums_of_flat_rows_with_an_outlier(dtype, V, flat, top):
+    """A row's mass several units below its largest logit, of equal logits: their errors have one sign. The beams' scores are their rows'
+    log-sums, so that what is left shows the error and not a score's own rounding."""
+    from cellm_b200 import ops
+    row = torch.full((V,), flat, dtype=dtype)
+    row[::1024] = top
+    exact = row.double()
+    z = torch.logsumexp(exact, 0) - exact.max()
+    start = z.float()
+    got, _, tokens = ops.beam_select(row.to(DEV).unsqueeze(0), start.view(1, 1).to(DEV), 1)
+    assert tokens.item() == 0 and abs(float(got) - float(start.double() - z)) <= SUM_ERROR
+
+
 def test_a_captured_selection_follows_its_inputs():
     from cellm_b200 import ops
     logits, scores = torch.randn(8, 9000, device=DEV), torch.zeros(2, 4, device=DEV)
