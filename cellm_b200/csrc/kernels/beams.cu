@@ -39,16 +39,17 @@ constexpr float BY_BEST_FROM = 32768.f;       // the best's magnitude from which
 
 // 2^-p exp(x) of two numbers. x log2 e = n + f with |f| <= 1/2: n comes out of the rounding of a multiply-add whose addend (1.5 * 2^23 - p) also
 // takes p off, f out of two more that lose nothing of x (log2 e in two parts; x - best would be rounded where the two are far apart, and
-// alike for equal logits). 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error) to 2.0e-9. What lies
+// alike for equal logits). 2^f = 1 + f P(f), P fitted (weighted least squares, reweighted towards the largest error)
+// with its first coefficient and then one after the other rounded to 32 bits: 3.0e-9 with the coefficients as they stand. What lies
 // below `least`, best - 86, or is not a number, adds exp(-86) of the best: nothing.
 __device__ __forceinline__ uint64_t exp_scaled(float a, float b, float least, uint64_t magic) {
     const uint64_t x = pair_of(fmaxf(a, least), fmaxf(b, least)), l2e = pair_of(1.4426950408889634f, 1.4426950408889634f);
     const uint64_t r = fma2(x, l2e, magic), rest = fma2(x, l2e, fma2(r, pair_of(-1.f, -1.f), magic));
     const uint64_t f = fma2(x, pair_of(1.925963033500011537e-8f, 1.925963033500011537e-8f), rest);
-    uint64_t p = pair_of(0.00015353357593994588f, 0.00015353357593994588f);
-    p = fma2(p, f, pair_of(0.0013398876180872321f, 0.0013398876180872321f));
-    p = fma2(p, f, pair_of(0.009618437848985195f, 0.009618437848985195f));
-    p = fma2(p, f, pair_of(0.055503323674201965f, 0.055503323674201965f));
+    uint64_t p = pair_of(0.00015326462744269520f, 0.00015326462744269520f);
+    p = fma2(p, f, pair_of(0.0013390806270763278f, 0.0013390806270763278f));
+    p = fma2(p, f, pair_of(0.0096185058355331421f, 0.0096185058355331421f));
+    p = fma2(p, f, pair_of(0.055503599345684052f, 0.055503599345684052f));
     p = fma2(p, f, pair_of(0.24022647738456726f, 0.24022647738456726f));
     p = fma2(p, f, pair_of(0.6931471824645996f, 0.6931471824645996f));
     p = fma2(p, f, pair_of(1.0f, 1.0f));
@@ -215,16 +216,16 @@ beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* 
     }
 }
 
-// exp(d) for d <= 1/2 in 64 bits, to 2.0e-9: as exp_scaled. The picking block runs its code once, so what it calls is short.
+// exp(d) for d <= 1/2 in 64 bits, to 2.0e-9: as exp_scaled, with the fit's own coefficients. The picking block runs its code once, so what it calls is short.
 __device__ __forceinline__ double exp_short(double d) {
     d = fmax(d, -600.0) * 1.4426950408889634074;
     const double n = rint(d), f = d - n;
-    double p = 0.00015353357593994588;
-    p = fma(p, f, 0.0013398876180872321);
-    p = fma(p, f, 0.009618437848985195);
-    p = fma(p, f, 0.055503323674201965);
-    p = fma(p, f, 0.24022647738456726);
-    p = fma(p, f, 0.6931471824645996);
+    double p = 0.00015353361911178411;
+    p = fma(p, f, 0.0013398874414638218);
+    p = fma(p, f, 0.0096184373576691552);
+    p = fma(p, f, 0.055503324711243029);
+    p = fma(p, f, 0.2402264791362882);
+    p = fma(p, f, 0.69314720285506826);
     return fma(p, f, 1.0) * __hiloint2double((1023 + (int)n) << 20, 0);
 }
 // log(s) for s >= 1/2: the 32-bit logarithm and one step of Newton's method

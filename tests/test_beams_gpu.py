@@ -112,6 +112,45 @@ def test_sums_of_flat_rows_with_an_outlier(dtype, V, flat, top):
     assert tokens.item() == 0 and abs(float(got) - float(start.double() - z)) <= SUM_ERROR
 
 
+def left_of(row):
+    """What beam_select leaves of a score that is the row's log-sum below its largest logit, against the same in 64 bits: the error of the
+    kernels' log-sum."""
+    from cellm_b200 import ops
+    exact = row.double()
+    z = torch.logsumexp(exact, 0) - exact.max()
+    start = z.float()
+    got, _, _ = ops.beam_select(row.to(DEV).unsqueeze(0), start.view(1, 1).to(DEV), 1)
+    return abs(float(got) - float(start.double() - z))
+
+
+def test_logarithms_of_sums():
+    """Rows of zeros, whose exponentials and sums are exact: log V where log2 V lies halfway between whole numbers, the exponential's far
+    end. Its fit is good to 2.0e-9, the 32-bit logarithm's error enters squared."""
+    for V in (181, 362, 23170, 46341):
+        assert left_of(torch.zeros(V)) <= 2.5e-9, V
+
+
+def test_exponentials_of_a_narrow_range():
+    """65,536 logits whose exponentials lie at the polynomial's far end. Single roundings (1.1e-7 at most) average out to less than 3e-9 of six
+    deviations; the error of its fit (3.0e-9, and 2.0e-9 of the logarithm) does not, nor does the last rounding of its argument: x times
+    log2 e's second part, 1.9e-8 x, is nearly the same for all of them and is added to a multiple of 2^-25, half a step of which is
+    2^-26 log 2 = 1.03e-8 of an exponential. 1.84e-8 in all."""
+    torch.manual_seed(5)
+    for n in (0, 3, -7):
+        row = ((n + 0.44 + 0.06 * torch.rand(65536, dtype=torch.float64)) * math.log(2)).float()
+        assert left_of(row) <= 1.84e-8, n
+        row = ((n - 0.5 + 0.06 * torch.rand(65536, dtype=torch.float64)) * math.log(2)).float()
+        assert left_of(row) <= 1.84e-8, n
+
+
+def test_exponentials_of_a_range_without_that_rounding():
+    """The same between 3.0782 and 3.1192 in magnitude, whose log2 leave 0.441 to 0.4999 above or below whole numbers, and of which log2 e's
+    second part makes 1.989 to 2.0155 steps of 2^-25: 5e-10 are lost. 8.5e-9 in all."""
+    torch.manual_seed(6)
+    for sign in (1, -1):
+        assert left_of((sign * (3.0782 + 0.041 * torch.rand(65536, dtype=torch.float64))).float()) <= 8.5e-9, sign
+
+
 def test_a_captured_selection_follows_its_inputs():
     from cellm_b200 import ops
     logits, scores = torch.randn(8, 9000, device=DEV), torch.zeros(2, 4, device=DEV)
