@@ -490,7 +490,7 @@ constexpr int UNITS_AT_ONCE = KMAX >= 32 || sizeof(W) == 16 ? 1 : 32 / KMAX;
 __device__ __forceinline__ void read_parents(int* to, const int* parents, int r, int beams, int* err) {
     if (threadIdx.x < beams) {
         int p = parents[r * beams + threadIdx.x];
-        if (p >= beams) { atomicOr(err, CELLM_DEV_BAD_SLOT); p = -1; }
+        if (p >= beams || p < -1) { atomicOr(err, CELLM_DEV_BAD_SLOT); p = -1; }
         to[threadIdx.x] = p < 0 || p == threadIdx.x ? -1 : p;
     }
 }
@@ -544,7 +544,7 @@ reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, in
     const unsigned units = (unsigned)(which ? p.units[1] : p.units[0]);
     read_parents(from, parents, r, beams, err);
     const int begin = max(0, starts[r]), end = (int)min((long long)ends[r], (long long)bt_stride * page_size);
-    if (end < ends[r] && threadIdx.x == 0) atomicOr(err, CELLM_DEV_BAD_PAGE);
+    if ((end < ends[r] || starts[r] < 0) && threadIdx.x == 0) atomicOr(err, CELLM_DEV_BAD_PAGE);
     const unsigned per_row = (unsigned)nkv * units, head = (unsigned)page_size * units;
     W* item = static_cast<W*>(which ? p.pool[1] : p.pool[0]) + (size_t)(blockIdx.y / p.pools) * pages * per_row * page_size;
     for (int at = begin + blockIdx.x * ROWS; at < end; at += gridDim.x * ROWS) {
@@ -554,7 +554,7 @@ reorder_pages_kernel(const PagedPools p, const int* __restrict__ block_table, in
             const int k = i / ROWS, j = i % ROWS;
             if (j >= (int)rows) continue;
             const int page = block_table[((long long)r * beams + k) * bt_stride + (at + j) / page_size];
-            if (page >= pages) atomicOr(err, CELLM_DEV_BAD_PAGE);
+            if (page >= pages || page < -1) atomicOr(err, CELLM_DEV_BAD_PAGE);
             row_at[k][j] = page < 0 || page >= pages ? -1 : ((long long)page * nkv * page_size + (at + j) % page_size) * units;
         }
         __syncthreads();

@@ -286,6 +286,23 @@ def test_bad_parents_slots_and_pages_are_reported_and_passed_over():
     assert e.item() == 2 | 4 and pool[0, :, 0].tolist()[1] == [[1.0] * 4, [3.0] * 4] and pool[0, :, 0].tolist()[5] == [[5.0] * 4, [1.0] * 4]
 
 
+def test_negative_parents_pages_and_rows_are_reported_too():
+    """-1 says that a beam stays and that a page was given back; anything below it, and a row before the first, is out of range: reported
+    and passed over as the other end's."""
+    from cellm_b200 import ops
+    state = torch.arange(5.0, device=DEV).repeat(2, 1).unsqueeze(2).contiguous()
+    for parent, said in ((-1, 0), (-2, 4), (-2 ** 31, 4)):
+        e = err_word()
+        ops.reorder_states(state, ints([3, 1, 4]), ints([[0, parent, 2]]), e)
+        assert e.item() == said and state[0].flatten().tolist() == [0, 1, 2, 3, 4]
+    base = torch.arange(6.0, device=DEV).view(1, 6, 1, 1, 1).repeat(1, 1, 1, 2, 4).contiguous()
+    for table, start, parents, said, rows in (([[0, 1], [2, 3], [4, 5]], 0, [1, -2, 2], 4, [2, 3, 2, 3, 4, 5]), ([[0, 1], [2, -1], [4, 5]], 0, [0, 2, 2], 0, [0, 1, 4, 3, 4, 5]),
+                                              ([[0, 1], [2, -2], [4, 5]], 0, [0, 2, 2], 2, [0, 1, 4, 3, 4, 5]), ([[0, 1], [2, 3], [4, 5]], -3, [2, 1, 2], 2, [4, 5, 2, 3, 4, 5])):
+        pool, e = base.clone(), err_word()
+        ops.reorder_pages(pool, None, ints(table), ints([start]), ints([4]), ints([parents]), e)
+        assert e.item() == said and pool[0, :, 0, 0, 0].tolist() == rows and pool[0, :, 0, 1, 3].tolist() == rows
+
+
 def test_a_search_through_its_steps():
     """Beams of two requests over a cache with states and pages, six steps: selection, then reordering, each beam writing its token into its
     state and its rows; at the end every beam's state and rows spell the tokens of its own history."""
