@@ -244,8 +244,8 @@ class Engine:
                     stop_eos: bool = True) -> list[list[BeamOutput]]:
         """The best `beams` continuations of each prompt, best first: in every step the beams of a prompt that have the highest sums of log
         probabilities go on, and one that chose the end-of-sequence token (with `stop_eos`) stands as it is. The final order is by that
-        sum divided by length ** length_penalty. Fewer than `beams` come back where there are no more. Every beam takes a state slot and
-        pages of its own (len(prompts) * beams <= max_num_seqs); OutOfPages where the pool is too small. The engine must have no
+        sum divided by length ** length_penalty. Fewer than `beams` come back where there are no more. Every beam that goes
+        on takes a state slot and pages of its own (len(prompts) * beams <= max_num_seqs); OutOfPages where the pool is too small. The engine must have no
         unfinished requests."""
         return beam_search(self, prompts, beams, max_new_tokens, length_penalty, stop_eos)
 

@@ -162,6 +162,79 @@ def test_beams_of_every_design(tmp_path, design, config):
             assert b.score == pytest.approx(float(lp[range(9), b.tokens].sum()), abs=2e-3)
 
 
+@pytest.mark.parametrize("name", list(CONFIGS))
+def test_finished_beams_need_no_pages(folders, name):
+    """A pool that holds what the beams that go on read, and no more: the others' caches are given back. The same beams as a large pool
+    gives."""
+    from cellm_b200 import Engine
+    cfg, w = plain.load_folder(folders[name])
+    prompt, K, steps, ps = [7, 8, 200, 31, 90], 4, 24, 2
+    make = lambda pages, eos: Engine(folders[name], dtype="float32", tokens_per_block=ps, total_blocks=pages, max_num_seqs=K)
+    wide = make(400, None)
+    free = wide.beam_search([prompt], beams=K, max_new_tokens=steps, stop_eos=False)[0]
+    tried = 0
+    for eos in dict.fromkeys(t for b in free for t in b.tokens[1:6]):
+        wide.plan = dataclasses.replace(wide.plan, eos_token_id=eos)
+        want = wide.beam_search([prompt], beams=K, max_new_tokens=steps)[0]
+        # the beams that go on after each token, by a plain search
+        need, found = 0, [(0.0, [], False)]
+        for at in range(steps):
+            nxt = []
+            for s, toks, d in found:
+                if d:
+                    nxt.append((s, toks, True))
+                    continue
+                lp = log_probs(cfg, w, prompt + toks)[-1]
+                top = lp.topk(K)
+                nxt += [(s + float(v), toks + [int(t)], int(t) == eos) for v, t in zip(top.values, top.indices)]
+            found = sorted(nxt, key=lambda f: -f[0])[:K]
+            live = sum(not d for _, _, d in found)
+            if not live:
+                break
+            if at + 1 < steps:
+                need = max(need, live * (-(-(len(prompt) + at + 1) // ps)))
+        need = max(need, -(-len(prompt) // ps))
+        if need >= K * (-(-(len(prompt) + steps - 1) // ps)) - 2:
+            continue
+        tried += 1
+        tight = make(need, eos)
+        tight.plan = dataclasses.replace(tight.plan, eos_token_id=eos)
+        got = tight.beam_search([prompt], beams=K, max_new_tokens=steps)[0]
+        assert [b.tokens for b in got] == [b.tokens for b in want]
+        check(cfg, w, prompt, got, K, steps, eos)
+        assert tight.stats()["free_pages"] == tight.stats()["total_pages"] and tight.stats()["free_slots"] == K
+    assert tried
+
+
+@pytest.mark.parametrize("design", ["vezalorn", "tufadra", "padadra", "bozovik", "tikizen", "gonozen"])
+def test_beams_that_end_in_every_design(tmp_path, design):
+    """Caches of every kind given back by beams that end, beside another prompt's beams; scores as in the test above."""
+    from cellm_b200 import Engine
+    from cellm_b200.engine.step import StepEntry
+    made = importlib.import_module(f"test_{design}_gpu")
+    folder = made.write_model(tmp_path / "m", made.CONFIGS["a"], 31)
+    eng = Engine(folder, dtype="float32", tokens_per_block=8, total_blocks=160, max_num_seqs=10, prefill_chunk=16)
+    V = eng.plan.vocab_size
+    prompts = [[(11 * i + 5) % V for i in range(45)], [7 % V, 3 % V]]
+    free = eng.beam_search(prompts, beams=5, max_new_tokens=9, stop_eos=False)
+    ended = 0
+    for eos in dict.fromkeys(t for found in free for b in found for t in b.tokens[:4]):
+        eng.plan = dataclasses.replace(eng.plan, eos_token_id=eos)
+        out = eng.beam_search(prompts, beams=5, max_new_tokens=9)
+        assert eng.stats()["free_pages"] == eng.stats()["total_pages"] and eng.stats()["free_slots"] == 10
+        for prompt, found in zip(prompts, out):
+            assert len(found) == 5 and len({tuple(b.tokens) for b in found}) == 5
+            ended += sum(b.finished for b in found)
+            for n, b in enumerate(found):
+                assert b.finished == (b.tokens[-1] == eos) and eos not in b.tokens[:-1] and (b.finished or len(b.tokens) == 9)
+                eng.cache.add(10 ** 6 + n)
+                whole = prompt + b.tokens[:-1]
+                lp = torch.log_softmax(eng.runner.run([StepEntry(10 ** 6 + n, whole, list(range(len(prompt) - 1, len(whole))))]).double(), -1)
+                eng.cache.release(10 ** 6 + n)
+                assert b.score == pytest.approx(float(lp[range(len(b.tokens)), b.tokens].sum()), abs=2e-3)
+    assert ended
+
+
 def test_refusals(folders):
     from cellm_b200 import Engine, SamplingParams
     from cellm_b200.cache.manager import OutOfPages
