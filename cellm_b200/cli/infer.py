@@ -15,17 +15,27 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt", help="prompt text (uses the tokenizer to encode and decode)")
     ap.add_argument("--seq", type=int, default=8, help="prompt length (token ids 0..seq-1 unless --tokens)")
     ap.add_argument("--gen", type=int, default=8, help="number of generated tokens")
-    ap.add_argument("--temperature", type=float, default=0.8, help="sampling temperature (0 = greedy)")
-    ap.add_argument("--top-k", type=int, default=40, help="sample from the top K tokens (0 = all)")
+    ap.add_argument("--temperature", type=float, default=None, help="sampling temperature (0 = greedy; default 0.8)")
+    ap.add_argument("--top-k", type=int, default=None, help="sample from the top K tokens (0 = all; default 40)")
     ap.add_argument("--seed", type=int, default=None, help="RNG seed for sampling")
-    ap.add_argument("--repeat-penalty", type=float, default=1.05, help="repetition penalty (1.0 disables)")
-    ap.add_argument("--repeat-window", type=int, default=64, help="recent token window for the penalty")
+    ap.add_argument("--repeat-penalty", type=float, default=None, help="repetition penalty (1.0 disables; default 1.05)")
+    ap.add_argument("--repeat-window", type=int, default=None, help="recent token window for the penalty (default 64)")
     ap.add_argument("--tokens", help="comma-separated token ids (overrides --seq)")
-    ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams (0: sampling or greedy); prints every beam, best first")
-    ap.add_argument("--length-penalty", type=float, default=1.0, help="beams are ranked by log probability / length ** this")
+    ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams (0: sampling or greedy), by log probability alone: without a temperature, top-k, seed or "
+                                                         "repetition penalty; prints every beam, best first")
+    ap.add_argument("--length-penalty", type=float, default=None, help="beams are ranked by log probability / length ** this (default 1.0)")
     ap.add_argument("--stop-eos", type=lambda s: s.lower() not in ("0", "false", "no"), default=True,
                     help="stop when the EOS token is produced")
     args = ap.parse_args(argv)
+    if args.beams:
+        given = [o for o in ("--temperature", "--top-k", "--seed", "--repeat-penalty", "--repeat-window") if getattr(args, o[2:].replace("-", "_")) is not None]
+        if given:
+            ap.error(f"--beams goes by log probability alone: it does not take {', '.join(given)}")
+    elif args.length_penalty is not None:
+        ap.error("--length-penalty ranks beams: it needs --beams")
+    for name, value in (("temperature", 0.8), ("top_k", 40), ("repeat_penalty", 1.05), ("repeat_window", 64), ("length_penalty", 1.0)):
+        if getattr(args, name) is None:
+            setattr(args, name, value)
 
     from .. import Engine, SamplingParams
     t0 = time.time()

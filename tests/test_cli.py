@@ -40,6 +40,15 @@ def test_tools_offer_their_options(tool, options):
         assert o in p.stdout, f"{tool} --help does not name {o}"
 
 
+@pytest.mark.parametrize("given", [["--temperature", "0.5"], ["--top-k", "3"], ["--seed", "1"], ["--repeat-penalty", "1.05"], ["--repeat-window", "8"]])
+def test_infer_refuses_what_a_beam_search_does_not_do(given, capsys):
+    from cellm_b200.cli import infer
+    for args, word in ((["--beams", "3", *given], given[0]), (["--length-penalty", "0.6"], "--length-penalty")):
+        with pytest.raises(SystemExit) as e:
+            infer.main(["--model", "/nowhere", *args])
+        assert e.value.code == 2 and word in capsys.readouterr().err.splitlines()[-1]
+
+
 def test_infer_wants_a_model():
     p = subprocess.run([sys.executable, os.path.join(ROOT, "bin", "infer")], capture_output=True, text=True, timeout=120)
     assert p.returncode != 0 and "--model" in (p.stderr + p.stdout)
