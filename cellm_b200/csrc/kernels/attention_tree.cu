@@ -381,7 +381,7 @@ attention_tree_plain_kernel(const TreeArgs a, int quads) {
 // Four warps take 16 * RG rows through blocks of 64 keys that all threads bring in with cp.async (a ring of ST stages, one barrier
 // a block). RG groups of 16 rows share a block; the 4 / RG warps of a group take its keys in equal parts, each with a softmax
 // state of its own, and meet in shared memory at the end. Few rows (small trees) so still use every warp. One tree of 8 nodes behind 500
-// keys, 32 heads over 8: 8.9 us in a CUDA graph, bound by latency (the copies' first block, the merge); with many long trees by issue
+// keys, 32 heads over 8: 9.2 us in a CUDA graph, bound by latency (the copies' first block, the merge); with many long trees by issue
 // slots (42 %) and waits for shared memory, which is why those go to tcgen05.
 template <int HD, int RG>
 struct MmaTile {
@@ -747,6 +747,9 @@ int pieces(long long tiles, int key_blocks, long long at_once, bool clusters) {
 //   8 nodes (32 rows)    1,024 keys 10.0 12.0 | 12.7 15.3 | 33.9 30.5     4,096 keys 18.8 16.3 | 24.8 27.0 | 105 77
 //   12 nodes (48 rows)   1,024 keys 10.7 12.5 | 14.2 15.4 | 39.7 30.8     4,096 keys 21.3 17.1 | 30.9 27.3 | 127 77
 //   25 nodes (100 rows)  1,024 keys 12.3 12.9 | 21.8 15.6 | 76.2 31.2     4,096 keys 24.0 18.7 | 54.9 28.2 | 226 77
+// The number of trees, on which the table depends too, does not enter: the rule gives away up to 9 us where many small trees stand behind
+// fewer than 2,048 keys (32 of 12 nodes 39.7 for 30.8, 32 of 8 33.9 for 30.5), 2 us for 8 of 8 nodes behind 4,096 (27.0 for 24.8) and 0.6
+// for one of 25 behind 1,024. Fewer than 1,024 keys were not measured.
 bool tc_pays(int rows, int keys) { return rows > 64 || (rows > 16 && keys >= 2048); }
 
 struct TreePlan {

@@ -138,9 +138,9 @@ __device__ __forceinline__ void ring_read(float (&x)[HALF_VALUES], const Ring<T>
 }
 
 // tops [rows][parts * 32], sums [rows][parts * 2]. The warps of a grid that fills the SMs take parts in turn, the next halves on their
-// way through a ring of the warp's own while it works on one. 512 rows of 65,536 32-bit logits (134 MB): 29 us,
-// 4.6 TB/s, with 56 % of the issue slots taken: neither limit is reached, a warp's halves wait in turn for memory and for one another's
-// instructions (pick included, 83 us with the warps loading in step, 51 with the ring and exponentials of any sign, 42 with those below
+// way through a ring of the warp's own while it works on one. 512 rows of 65,536 32-bit logits (134 MB): 31 us,
+// 4.3 TB/s, with 56 % of the issue slots taken: neither limit is reached, a warp's halves wait in turn for memory and for one another's
+// instructions (pick included 40 us; 16-bit logits, 67 MB, 36 us; steps on the way, with an exponential of fewer bits: 83 us with the warps loading in step, 51 with the ring and exponentials of any sign, 42 with those below
 // the best alone).
 template <typename T>
 __global__ void __launch_bounds__(ROW_WARPS * 32, Ring<T>::BLOCKS)
@@ -216,7 +216,8 @@ beam_rows_kernel(float* __restrict__ tops, RowPart* __restrict__ sums, const T* 
     }
 }
 
-// exp(d) for d <= 1/2 in 64 bits, to 2.0e-9: as exp_scaled, with the fit's own coefficients. The picking block runs its code once, so what it calls is short.
+// exp(d) for d <= 1/2 in 64 bits, to 2.0e-9: as exp_scaled, with the fit's own coefficients. The picking block runs its code once, so what
+// it calls is short.
 __device__ __forceinline__ double exp_short(double d) {
     d = fmax(d, -600.0) * 1.4426950408889634074;
     const double n = rint(d), f = d - n;
@@ -655,7 +656,7 @@ CELLM_API int cellm_reorder_states(void* state, const int* slot_ids, const int* 
     const uintptr_t at = (uintptr_t)state | (uintptr_t)bytes;
 #define GO(W_) return launch_states<W_>(state, slot_ids, parents, requests, beams, items, slots, bytes, err, stream)
     if (at % 16 == 0) GO(uint4);
-    if (at % 4 == 0) GO(uint32_t);
+    if (at % 4 == 0) GO(uint32_t);           // (8-byte borders too: in units of 4 bytes, several a thread, 2 beams move at 5.8 TB/s)
     if (at % 2 == 0) GO(uint16_t);
 #undef GO
     return CELLM_ERR_ALIGN;

@@ -49,7 +49,9 @@ def attention_tree(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pa
     most 256, and `tree_lens` is the host's copy of their numbers. `max_ctx`: the longest context if the host knows it (0: what the
     block table can name). float32 or bfloat16, heads of up to 256. Returns [T, nh * hd]; rows of no tree hold nothing of meaning. A row of K or V
     that is not finite may reach every node of its tree. Nothing is read or written of padding and of page entries that no node sees. A
-    page out of range that a node does see is reported in `err`, and its keys and values are zeros."""
+    page out of range that a node does see is reported in `err`, and its keys and values are zeros. Scores, maxima and sums are 32-bit;
+    in bfloat16 with heads of 32, 64, 96 or 128 the softmax's weights are rounded to bfloat16 before they meet the values, an error of up to
+    2^-8 of the weighted values' magnitudes beside the output's own rounding."""
     dtype, index, shape, table, T, B = q.dtype, q.get_device(), k_pool.shape, block_table.shape, q.shape[0], len(tree_lens)
     if index < 0 or dtype not in DTYPE_TAG or len(shape) != 4:
         raise ValueError("attention_tree: float32 or bfloat16 rows on the GPU over pools [pages, kv heads, page size, head size]")
